@@ -74,8 +74,9 @@ int oscar_set_rotation_path(int path);
 /* Synchronises `stream`, returns and clears the device-side bounds flag of the
  * current device: 0 = clean, otherwise a bitmask (1 = slot out of range,
  * 2 = block-table entry out of range, 8 = merge target row out of range,
- * 16 = a tensor-core decode wait timed out, 32 = more history splits per
- * request than the tensor-core merge holds).
+ * 16 = a bounded wait of an attention kernel timed out, 32 = more history splits per
+ * request than the tensor-core merge holds, 64 = a position outside the cos /
+ * sin table).
  * Debug/test helper; the hot path never synchronises. */
 int oscar_device_error(void* stream);
 
@@ -327,6 +328,92 @@ int oscar_decode_layer_step(const void* q, const void* k, const void* v, int32_t
 /* Bytes of oscar_decode_layer_step's scratch before the attention workspace. */
 int64_t oscar_decode_layer_step_scratch(int64_t n_tokens, int32_t num_q_heads, int32_t num_kv_heads,
                                         int32_t head_dim, int32_t dtype);
+
+/* ------------------------------------------------------------------------
+ * The 16-bit paged layer: a layer whose cache holds plain bf16 / fp16 keys and
+ * values (the MTP draft layers beside the INT2 ones).  No counterpart in the
+ * reference, which leaves these layers to the engine.
+ *
+ * Caches are [num_blocks, block_size, num_kv_heads, head_dim] with strides in
+ * ELEMENTS (rows of head_dim contiguous, 16-byte aligned; pages, tokens and
+ * heads at any stride, e.g. the K half of a [blocks, 2, ...] pool), head_dim
+ * 64, 128 or 256, any block size.  Slots and positions are int64.
+ *
+ * oscar_qk_norm_rope: RMS norm of every query and key head, position rotation
+ * and cache write in one pass.  Per head x:
+ *   y = x * rsqrt(mean(x^2) + eps) * (w + weight_offset)
+ *   the first rot_dim dims of y rotate by (cos, sin) = row positions[t] of
+ *   cos_sin [max_positions, rot_dim] (cosines, then sines): pairs
+ *   (i, i + rot_dim / 2), or (2 i, 2 i + 1) with `interleaved`
+ * in fp32, rounded once.  q -> out_q; k -> out_k (may be NULL with caches) and
+ * with caches k -> k_cache, v -> v_cache at slot_mapping[t] (slot < 0: not
+ * written).  Weights and cos_sin are fp32 or of the heads' type.  out_q / out_k
+ * may be q / k.  A position outside the table latches device error 64 and a
+ * slot outside the cache bit 1; neither is written.  rot_dim: a multiple of
+ * 16.  v, out_k and the caches may be NULL. */
+int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                       int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                       int64_t v_head_stride, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                       int32_t num_kv_heads, int32_t head_dim, const void* q_weight, const void* k_weight,
+                       int32_t weight_dtype, float eps, float weight_offset, const void* cos_sin,
+                       int32_t cos_sin_dtype, int64_t cos_sin_stride, int64_t max_positions, int32_t rot_dim,
+                       int32_t interleaved, const int64_t* positions, void* out_q, int64_t out_q_token_stride,
+                       int64_t out_q_head_stride, void* out_k, int64_t out_k_token_stride, int64_t out_k_head_stride,
+                       void* k_cache, void* v_cache, int64_t num_blocks, int32_t block_size, int64_t k_stride_block,
+                       int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_block, int64_t v_stride_token,
+                       int64_t v_stride_head, const int64_t* slot_mapping, void* stream);
+
+/* Attention of each request's new tokens over its paged 16-bit cache, which
+ * already holds their keys and values: query i of request r sees keys
+ * [0, seqs[r] - q_len + i] (q_len = qsl[r + 1] - qsl[r]); a row that sees none
+ * gets 0 and LSE -inf.  out [n, Hq, D] in the queries' type, lse [n, Hq] fp32
+ * natural log.  qsl / seqs: HOST int32.  Slots past seqs[r] may hold anything.
+ * A non-finite value row reaches every row of its request whose 64-key (or
+ * 128-key) tile it shares, also the earlier ones of the same chunk.
+ *
+ * weights (or NULL): fp32 [num_blocks, num_kv_heads, block_size] contiguous,
+ * the keys' accumulated attention weights.  For every key p < seqs[r]:
+ *   mass = sum over the heads of the group and the request's last `observe`
+ *          tokens of exp(score - lse)
+ *   weights += mass for a key older than the chunk, weights = mass for the
+ *   chunk's own keys (their slots have just been rewritten).
+ * Requests may share pages of history (their masses add up); the order of
+ * these additions is not fixed, everything else is deterministic.
+ *
+ * workspace: 16-byte aligned, at least oscar_paged_attention_workspace() bytes
+ * of the same lists (< 0: invalid lists). */
+int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,
+                          int64_t n_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          const void* k_cache, const void* v_cache, int64_t num_blocks, int32_t block_size,
+                          int64_t k_stride_block, int64_t k_stride_token, int64_t k_stride_head,
+                          int64_t v_stride_block, int64_t v_stride_token, int64_t v_stride_head,
+                          const int32_t* block_table, int64_t bt_rows, int64_t bt_cols, int64_t bt_stride,
+                          const int32_t* qsl, const int32_t* seqs, int32_t num_requests, float scale, float* weights,
+                          int32_t observe, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                          void* stream);
+
+int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs, int32_t num_requests,
+                                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t weighted);
+
+/* Eviction by accumulated weight.  Each request with more than `keep` cached
+ * tokens keeps, per kv head, its first `sink`, its last `recent` and of the
+ * tokens between them the keep - sink - recent heaviest (ties: the lower
+ * position; a NaN weight is above every number), in order.  Their K, V and
+ * weight slots move to positions 0, 1, ... of the pages of dst_table, or of
+ * block_table itself (dst_table NULL: in place).  Shorter requests keep all.
+ * The new length is min(seqs[r], keep).  seqs: HOST.  kept
+ * [num_requests, num_kv_heads, kept_cols] int32: the kept positions, -1 past
+ * a request's list.  Pages written here must belong to one request of the call
+ * only, and dst pages must not be source pages (unless dst_table is NULL).
+ * The pages' keys carry their position rotation with them. */
+int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t num_blocks, int32_t block_size,
+                      int32_t num_kv_heads, int64_t k_stride_block, int64_t k_stride_token, int64_t k_stride_head,
+                      int64_t v_stride_block, int64_t v_stride_token, int64_t v_stride_head, float* weights,
+                      const int32_t* block_table, int64_t bt_rows, int64_t bt_cols, int64_t bt_stride,
+                      const int32_t* dst_table, int64_t dst_rows, int64_t dst_cols, int64_t dst_stride,
+                      const int32_t* seqs, int32_t num_requests, int32_t keep, int32_t sink, int32_t recent,
+                      int32_t* kept, int32_t kept_cols, void* stream);
 
 #ifdef __cplusplus
 }

@@ -62,6 +62,17 @@ SIGNATURES = {
                                                _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _I64,
                                                _P, _P, _I32, _I32, _I32, _F32, _P, _P, _P, _I64, _P, _I64,
                                                _P, _I64, _P]),
+    "oscar_qk_norm_rope": (ctypes.c_int, [_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64, _I32, _I32, _I32,
+                                          _P, _P, _I32, _F32, _F32, _P, _I32, _I64, _I64, _I32, _I32, _P, _P, _I64,
+                                          _I64, _P, _I64, _I64, _P, _P, _I64, _I32, _I64, _I64, _I64, _I64, _I64,
+                                          _I64, _P, _P]),
+    "oscar_paged_attention": (ctypes.c_int, [_P, _I64, _I64, _I32, _I64, _I32, _I32, _I32, _P, _P, _I64, _I32, _I64,
+                                             _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I32, _F32,
+                                             _P, _I32, _P, _P, _P, _I64, _P]),
+    "oscar_paged_attention_workspace": (ctypes.c_int64, [_P, _P, _I32, _I32, _I32, _I32, _I32]),
+    "oscar_evict_cache": (ctypes.c_int, [_P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
+                                         _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _I32, _I32, _I32, _I32, _P, _I32,
+                                         _P]),
     "oscar_decode_layer_step_scratch": (ctypes.c_int64, [_I64, _I32, _I32, _I32, _I32]),
 }
 

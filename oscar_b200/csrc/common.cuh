@@ -12,8 +12,9 @@ namespace oscar {
 
 // Device-side bounds latch: kernels OR a bit in and skip the offending access.
 // 1 = slot / block id out of range, 2 = block-table entry out of range,
-// 8 = merge target row out of range.
-__device__ unsigned int g_bounds_error;
+// 8 = merge target row out of range, 64 = position outside the cos / sin table.
+// One per translation unit; oscar_device_error reads them all.
+static __device__ unsigned int g_bounds_error;
 
 OSCAR_DEVINL void flag_error(unsigned int bit) { atomicOr(&g_bounds_error, bit); }
 

@@ -5,15 +5,11 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
-#include <mutex>
-#include <string>
-#include <utility>
 #include <queue>
 #include <vector>
 
 #include "../../include/oscar_b200.h"
+#include "host.h"
 #include "attention.cuh"
 #include "cont_tc.cuh"
 #include "decode.cuh"
@@ -25,62 +21,17 @@
 
 namespace {
 
-thread_local std::string g_last_error;
-std::atomic<uint64_t> g_launches{0};
+using oscar_host::cuda_status;
+using oscar_host::device_info;
+using oscar_host::encode_tiled;
+using oscar_host::EncodeTiledFn;
+using oscar_host::fail;
+using oscar_host::g_last_error;
+using oscar_host::g_launches;
+using oscar_host::launch_pdl;
+
 std::atomic<int> g_rotate_path{0};  // 0 auto, 1 16-row FMA tiles, 2 tensor cores, 3 128-row FMA tiles (where each applies)
 std::atomic<int> g_attention_path{0};  // 0 auto, 1 tile only, 2 mma.sync decode, 3 tensor-core decode (where eligible)
-
-int fail(int code, const char* fmt, ...) {
-  char buf[512];
-  va_list ap;
-  va_start(ap, fmt);
-  vsnprintf(buf, sizeof(buf), fmt, ap);
-  va_end(ap);
-  g_last_error = buf;
-  return code;
-}
-
-int cuda_status(const char* what, int launches = 1) {
-  g_launches.fetch_add((uint64_t)launches, std::memory_order_relaxed);
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return fail(OSCAR_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-  return OSCAR_OK;
-}
-
-// Launch with programmatic stream serialisation: the kernel may start while the
-// previous kernel of the stream finishes; it waits (pdl_wait) before reading
-// anything that kernel writes.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
-                       Args&&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
-struct DeviceInfo {
-  int sms = 0;
-};
-
-DeviceInfo& device_info() {
-  static thread_local int cached_dev = -1;
-  static thread_local DeviceInfo info;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev != cached_dev) {
-    cudaDeviceGetAttribute(&info.sms, cudaDevAttrMultiProcessorCount, dev);
-    cached_dev = dev;
-  }
-  return info;
-}
 
 inline int clip_index(float ratio, int d) {
   if (!(ratio > 0.0f)) return -1;
@@ -119,7 +70,9 @@ int oscar_device_error(void* stream) {
   unsigned int v = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&v, oscar::g_bounds_error, sizeof(v)) != cudaSuccess) return -OSCAR_ERR_CUDA;
   cudaMemcpyToSymbol(oscar::g_bounds_error, &zero, sizeof(zero));
-  return (int)v;
+  const int paged = oscar_host::take_paged16_error();
+  if (paged < 0) return paged;
+  return (int)v | paged;
 }
 
 // ---------------------------------------------------------------------------
@@ -572,23 +525,6 @@ int run_decode_rows(const oscar::AttnArgs& a, const std::vector<ReqInfo>& reqs, 
 }
 
 // ---- tensor-core decode path (decode_tc.cuh)
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static std::once_flag once;
-  static EncodeTiledFn fn = nullptr;
-  std::call_once(once, [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(f);
-  });
-  return fn;
-}
-
 // A paged cache viewed as a 2D byte matrix [num_blocks * bs tokens, token stride]
 // with boxes of `box_x` bytes x `box_y` tokens.
 bool make_cache_map(CUtensorMap* map, const uint8_t* base, int64_t num_blocks, int bs, int64_t token_stride,

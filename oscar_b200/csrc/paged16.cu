@@ -1,0 +1,486 @@
+// C ABI of the 16-bit paged attention layer (declarations and contracts:
+// include/oscar_b200.h): head norm + rotation + cache write, attention over
+// the paged cache with the keys' accumulated weights, eviction by weight.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "../../include/oscar_b200.h"
+#include "evict.cuh"
+#include "head_norm.cuh"
+#include "host.h"
+#include "paged.cuh"
+
+namespace oscar_host {
+
+int take_paged16_error() {
+  unsigned int v = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&v, oscar::g_bounds_error, sizeof(v)) != cudaSuccess) return -OSCAR_ERR_CUDA;
+  cudaMemcpyToSymbol(oscar::g_bounds_error, &zero, sizeof(zero));
+  return (int)v;
+}
+
+}  // namespace oscar_host
+
+namespace {
+
+using oscar_host::cuda_status;
+using oscar_host::device_info;
+using oscar_host::encode_tiled;
+using oscar_host::fail;
+using oscar_host::launch_pdl;
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+bool half_dtype(int32_t dtype) { return dtype == OSCAR_DTYPE_BF16 || dtype == OSCAR_DTYPE_F16; }
+
+bool kernel_head_dim(int32_t d) { return d == 64 || d == 128 || d == 256; }
+
+// One cache of [num_blocks, block_size, hk, D] elements with strides in elements.
+int check_cache(const char* what, const void* cache, int64_t num_blocks, int32_t bs, int32_t hk, int32_t d, int64_t sb,
+                int64_t st, int64_t sh) {
+  if (num_blocks < 0 || num_blocks >= INT_MAX || bs < 1 || hk < 1)
+    return fail(OSCAR_ERR_INVALID, "%s: invalid cache geometry", what);
+  if (num_blocks > 0 && !cache) return fail(OSCAR_ERR_INVALID, "%s: null cache", what);
+  // (a dimension of one element has no stride of its own)
+  if (!aligned16(cache) || ((num_blocks > 1 ? sb : 0) | (bs > 1 ? st : 0) | (hk > 1 ? sh : 0)) % 8)
+    return fail(OSCAR_ERR_INVALID, "%s: cache rows must be 16-byte aligned", what);
+  if ((hk > 1 && sh < d) || (bs > 1 && st < d) || (num_blocks > 1 && sb < d))
+    return fail(OSCAR_ERR_INVALID, "%s: cache rows overlap", what);
+  return OSCAR_OK;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+namespace {
+
+template <typename T>
+void launch_head_norm(const oscar::HeadNormArgs& a, int d, cudaStream_t s) {
+  const int heads = a.hq + a.hk + (a.v_cache != nullptr ? a.hk : 0);
+  const int64_t per = 256 / d;  // tokens per warp
+  const int64_t items = (a.n + per - 1) / per * ((heads + oscar::kHnHeads - 1) / oscar::kHnHeads);
+  constexpr int kWarps = oscar::kHnThreads / 32;
+  const dim3 grid((unsigned)((items + kWarps - 1) / kWarps)), block(oscar::kHnThreads);
+  if (d == 256) launch_pdl(oscar::head_norm_kernel<T, 256>, grid, block, 0, s, a);
+  else if (d == 128) launch_pdl(oscar::head_norm_kernel<T, 128>, grid, block, 0, s, a);
+  else launch_pdl(oscar::head_norm_kernel<T, 64>, grid, block, 0, s, a);
+}
+
+}  // namespace
+
+extern "C" int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                                  int64_t k_token_stride, int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                                  int64_t v_head_stride, int32_t dtype, int64_t n_tokens, int32_t num_q_heads,
+                                  int32_t num_kv_heads, int32_t head_dim, const void* q_weight, const void* k_weight,
+                                  int32_t weight_dtype, float eps, float weight_offset, const void* cos_sin,
+                                  int32_t cos_sin_dtype, int64_t cos_sin_stride, int64_t max_positions,
+                                  int32_t rot_dim, int32_t interleaved, const int64_t* positions, void* out_q,
+                                  int64_t out_q_token_stride, int64_t out_q_head_stride, void* out_k,
+                                  int64_t out_k_token_stride, int64_t out_k_head_stride, void* k_cache, void* v_cache,
+                                  int64_t num_blocks, int32_t block_size, int64_t k_stride_block,
+                                  int64_t k_stride_token, int64_t k_stride_head, int64_t v_stride_block,
+                                  int64_t v_stride_token, int64_t v_stride_head, const int64_t* slot_mapping,
+                                  void* stream) {
+  if (!half_dtype(dtype)) return fail(OSCAR_ERR_UNSUPPORTED, "qk_norm_rope: heads must be bf16 or fp16");
+  if (!kernel_head_dim(head_dim))
+    return fail(OSCAR_ERR_UNSUPPORTED, "qk_norm_rope: head_dim %d: kernels exist for 64, 128, 256", head_dim);
+  if (n_tokens < 0 || num_q_heads < 1 || num_kv_heads < 1 || num_q_heads > 4096 || num_kv_heads > 4096 ||
+      max_positions < 1)
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: invalid geometry");
+  if (rot_dim < 16 || rot_dim > head_dim || rot_dim % 16)
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: rot_dim %d must be a multiple of 16 of at most head_dim", rot_dim);
+  if ((weight_dtype != OSCAR_DTYPE_F32 && weight_dtype != dtype) ||
+      (cos_sin_dtype != OSCAR_DTYPE_F32 && cos_sin_dtype != dtype))
+    return fail(OSCAR_ERR_UNSUPPORTED, "qk_norm_rope: weights and cos / sin must be fp32 or of the heads' type");
+  if (!(eps >= 0.0f) || !std::isfinite(eps) || !std::isfinite(weight_offset))
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: eps must be finite and not negative");
+  if ((k_cache == nullptr) != (v_cache == nullptr) || (k_cache == nullptr) != (slot_mapping == nullptr))
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: caches and slot_mapping come together");
+  if (k_cache != nullptr) {
+    int st = check_cache("qk_norm_rope", k_cache, num_blocks, block_size, num_kv_heads, head_dim, k_stride_block,
+                         k_stride_token, k_stride_head);
+    if (!st)
+      st = check_cache("qk_norm_rope", v_cache, num_blocks, block_size, num_kv_heads, head_dim, v_stride_block,
+                       v_stride_token, v_stride_head);
+    if (st) return st;
+  }
+  if (n_tokens == 0) return OSCAR_OK;
+  if (k_cache == nullptr && out_k == nullptr) return fail(OSCAR_ERR_INVALID, "qk_norm_rope: the keys have no destination");
+  if (!q || !k || !q_weight || !k_weight || !cos_sin || !positions || !out_q || (k_cache != nullptr && !v))
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: null pointer");
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out_q) || !aligned16(out_k) ||
+      !aligned16(q_weight) || !aligned16(k_weight) || !aligned16(cos_sin) ||
+      (q_token_stride | q_head_stride | k_token_stride | k_head_stride | out_q_token_stride | out_q_head_stride) % 8 ||
+      (v != nullptr && (v_token_stride | v_head_stride) % 8) ||
+      (out_k != nullptr && (out_k_token_stride | out_k_head_stride) % 8) || cos_sin_stride % 8 || cos_sin_stride < rot_dim)
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: heads, weights and cos / sin rows must be 16-byte aligned");
+  oscar::HeadNormArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_tok = q_token_stride, a.q_head = q_head_stride;
+  a.k_tok = k_token_stride, a.k_head = k_head_stride;
+  a.v_tok = v_token_stride, a.v_head = v_head_stride;
+  a.out_q = out_q, a.out_k = out_k;
+  a.oq_tok = out_q_token_stride, a.oq_head = out_q_head_stride;
+  a.ok_tok = out_k_token_stride, a.ok_head = out_k_head_stride;
+  a.wq = q_weight, a.wk = k_weight;
+  a.w_f32 = weight_dtype == OSCAR_DTYPE_F32;
+  a.eps = eps, a.offset = weight_offset;
+  a.cos_sin = cos_sin;
+  a.cs_f32 = cos_sin_dtype == OSCAR_DTYPE_F32;
+  a.cs_stride = cos_sin_stride, a.max_pos = max_positions;
+  a.rot = rot_dim, a.interleaved = interleaved != 0;
+  a.positions = positions;
+  a.n = n_tokens, a.hq = num_q_heads, a.hk = num_kv_heads;
+  a.k_cache = k_cache, a.v_cache = v_cache;
+  a.num_blocks = num_blocks, a.bs = block_size;
+  a.kcb = k_stride_block, a.kct = k_stride_token, a.kch = k_stride_head;
+  a.vcb = v_stride_block, a.vct = v_stride_token, a.vch = v_stride_head;
+  a.slots = slot_mapping;
+  const int heads = a.hq + 2 * a.hk;
+  if (n_tokens > (int64_t)INT_MAX / heads) return fail(OSCAR_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens for one launch");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == OSCAR_DTYPE_BF16) launch_head_norm<__nv_bfloat16>(a, head_dim, s);
+  else launch_head_norm<__half>(a, head_dim, s);
+  return cuda_status("head_norm_kernel");
+}
+
+// ---------------------------------------------------------------------------
+namespace {
+
+constexpr int kFewRows = 32;  // query rows of a (request, kv head) in one block of the split kernel
+
+// Workspace of one launch of the split kernel, in this order.
+struct PagedSpace {
+  int64_t stats, part_ml, part_o, scores;  // bytes
+  int64_t total() const { return stats + part_ml + part_o + scores; }
+};
+inline int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
+
+// The requests [r0, ..) of a call that fit one launch: at most kPgReqs, those with
+// few rows or those with many.  Returns the index after the last one looked at.
+struct PagedBatch {
+  oscar::PagedPlan plan;
+  int rows;  // rows per block of the split kernel
+};
+int paged_batch(PagedBatch& b, int r0, bool few, const int32_t* qsl, const int32_t* seqs, int num, int group, int hk,
+                int sms) {
+  oscar::PagedPlan& p = b.plan;
+  p.num_req = 0;
+  int most = 0, r = r0;
+  for (; r < num && p.num_req < oscar::kPgReqs; ++r) {
+    const int64_t len = qsl[r + 1] - qsl[r], rows = len * group;
+    if (len == 0 || (rows <= kFewRows) != few) continue;
+    const int i = p.num_req++;
+    p.req_id[i] = r;
+    p.q_start[i] = qsl[r];
+    p.q_len[i] = (int)len;
+    p.seq[i] = seqs[r];
+    most = std::max<int64_t>(most, std::min<int64_t>(rows, kFewRows));
+  }
+  b.rows = most <= 16 ? 16 : kFewRows;
+  int64_t tiles = 0;
+  for (int i = 0; i < p.num_req; ++i) {
+    p.tile_begin[i] = tiles;
+    const int64_t blocks = ((int64_t)p.q_len[i] * group + b.rows - 1) / b.rows;
+    tiles += blocks * hk * std::max<int64_t>(1, ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys);
+  }
+  p.tile_begin[p.num_req] = tiles;
+  p.total_tiles = tiles;
+  p.ctas = (int)std::min<int64_t>(std::max(sms, 1), tiles);
+  return r;
+}
+
+PagedSpace paged_space(const PagedBatch& b, bool few, int64_t n, int hq, int d, bool weighted) {
+  PagedSpace s{};
+  if (weighted) s.stats = round256(n * hq * (int64_t)sizeof(float2));
+  s.part_ml = round256((int64_t)2 * b.plan.ctas * b.rows * sizeof(float2));
+  s.part_o = round256((int64_t)2 * b.plan.ctas * b.rows * d * sizeof(float));
+  if (weighted && few) s.scores = b.plan.total_tiles * b.rows * oscar::kPgKeys * (int64_t)sizeof(float);
+  return s;
+}
+
+int check_paged(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int64_t n_tokens, int32_t hq, int32_t hk) {
+  if (hq < 1 || hk < 1 || hq % hk || hq > 4096) return fail(OSCAR_ERR_INVALID, "paged_attention: Hq must be a multiple of Hk");
+  if (num_requests < 0 || !qsl || (num_requests > 0 && !seqs) || qsl[0] != 0 || qsl[num_requests] != n_tokens)
+    return fail(OSCAR_ERR_INVALID, "paged_attention: invalid query layout");
+  for (int r = 0; r < num_requests; ++r)
+    if (qsl[r] > qsl[r + 1] || seqs[r] < 0)
+      return fail(OSCAR_ERR_INVALID, "paged_attention: query starts must not fall and lengths not be negative");
+  return OSCAR_OK;
+}
+
+// The cache as a 4D map (dims, heads, tokens of a page, pages) in boxes of 64 dims x `box` tokens.
+bool paged_map(CUtensorMap* map, const void* base, int dtype, int64_t num_blocks, int bs, int hk, int d, int64_t sb,
+               int64_t st, int64_t sh, int box) {
+  const auto fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)hk, (cuuint64_t)bs, (cuuint64_t)num_blocks};
+  // a dimension of one element has no stride of its own
+  const cuuint64_t strides[3] = {(cuuint64_t)(hk > 1 ? sh : d) * 2, (cuuint64_t)(bs > 1 ? st : d) * 2,
+                                 (cuuint64_t)(num_blocks > 1 ? sb : d) * 2};
+  const cuuint32_t boxes[4] = {64, 1, (cuuint32_t)box, 1};
+  const cuuint32_t step[4] = {1, 1, 1, 1};
+  return fn(map, dtype == OSCAR_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+            const_cast<void*>(base), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) ==
+         CUDA_SUCCESS;
+}
+
+// dynamic shared memory above 48 KB has to be asked for once per kernel and device
+template <auto Kernel>
+void allow_smem(size_t bytes) {
+  static thread_local int set_dev = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (set_dev == dev) return;
+  cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  set_dev = dev;
+}
+
+struct PagedCall {
+  oscar::PagedArgs args;
+  CUtensorMap kmap, vmap;
+  const void* k_cache;
+  int64_t kcb, kct, kch;
+  int64_t n;
+  cudaStream_t stream;
+};
+
+template <int D, typename T, int NRT>
+int launch_split(const PagedCall& c, const PagedBatch& b, bool few) {
+  const oscar::PagedArgs& a = c.args;
+  const oscar::PagedPlan& p = b.plan;
+  constexpr size_t smem = sizeof(oscar::PagedSmem<D, NRT>);
+  allow_smem<oscar::paged_split_kernel<D, T, NRT>>(smem);
+  launch_pdl(oscar::paged_split_kernel<D, T, NRT>, dim3(p.ctas), dim3(oscar::kPgThreads), smem, c.stream, a, p, c.kmap,
+             c.vmap);
+  int st = cuda_status("paged_split_kernel");
+  if (st) return st;
+  bool divided = false;
+  for (int i = 0; i < p.num_req && !divided; ++i) {
+    // a unit of request i lies in one CTA's range unless a range begins inside it
+    const int64_t nt = std::max<int64_t>(1, ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys);
+    for (int64_t u = p.tile_begin[i]; u < p.tile_begin[i + 1] && !divided; u += nt)
+      divided = ((u + 1) * p.ctas - 1) / p.total_tiles != ((u + nt) * p.ctas - 1) / p.total_tiles;
+  }
+  if (divided) {
+    const int last = p.num_req - 1;
+    const int64_t rows = ((int64_t)p.q_start[last] + p.q_len[last] - p.q_start[0]) * a.hq;
+    launch_pdl(oscar::paged_combine_kernel<D, T, 16 * NRT>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, c.stream, a,
+               p, rows);
+    st = cuda_status("paged_combine_kernel");
+    if (st) return st;
+  }
+  if (a.weights == nullptr) return OSCAR_OK;
+  if (few) {
+    launch_pdl(oscar::paged_mass_kernel<16 * NRT>, dim3((unsigned)p.total_tiles), dim3(oscar::kPgKeys), 0, c.stream, a, p);
+    return cuda_status("paged_mass_kernel");
+  }
+  oscar::PagedPlan keys = p;
+  int64_t tiles = 0;
+  for (int i = 0; i < p.num_req; ++i) {
+    keys.tile_begin[i] = tiles;
+    tiles += ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys;
+  }
+  keys.tile_begin[p.num_req] = tiles;
+  if (tiles == 0) return OSCAR_OK;
+  launch_pdl(oscar::paged_mass_rows_kernel<D, T>, dim3((unsigned)tiles, (unsigned)a.hk), dim3(32 * oscar::kPgWarps),
+             (size_t)oscar::kPgKeys * D * 2, c.stream, a, keys, reinterpret_cast<const T*>(c.k_cache), c.kcb, c.kct, c.kch);
+  return cuda_status("paged_mass_rows_kernel");
+}
+
+template <int D, typename T>
+int launch_paged(const PagedCall& c, const PagedBatch& b, bool few) {
+  return b.rows <= 16 ? launch_split<D, T, 1>(c, b, few) : launch_split<D, T, 2>(c, b, few);
+}
+
+template <typename T>
+int launch_paged_d(int d, const PagedCall& c, const PagedBatch& b, bool few) {
+  if (d == 256) return launch_paged<256, T>(c, b, few);
+  if (d == 128) return launch_paged<128, T>(c, b, few);
+  return launch_paged<64, T>(c, b, few);
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs, int32_t num_requests,
+                                        int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                                        int32_t weighted) {
+  if (num_requests < 0 || !qsl || check_paged(qsl, seqs, num_requests, qsl[num_requests], num_q_heads, num_kv_heads) ||
+      !kernel_head_dim(head_dim))
+    return -1;
+  int64_t need = 0;
+  PagedBatch b;
+  for (int few = 0; few < 2; ++few)
+    for (int r = 0; r < num_requests;) {
+      r = paged_batch(b, r, few, qsl, seqs, num_requests, num_q_heads / num_kv_heads, num_kv_heads, device_info().sms);
+      if (b.plan.num_req > 0)
+        need = std::max(need, paged_space(b, few, qsl[num_requests], num_q_heads, head_dim, weighted != 0).total());
+    }
+  return need;
+}
+
+int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,
+                          int64_t n_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          const void* k_cache, const void* v_cache, int64_t num_blocks, int32_t block_size,
+                          int64_t k_stride_block, int64_t k_stride_token, int64_t k_stride_head,
+                          int64_t v_stride_block, int64_t v_stride_token, int64_t v_stride_head,
+                          const int32_t* block_table, int64_t bt_rows, int64_t bt_cols, int64_t bt_stride,
+                          const int32_t* qsl, const int32_t* seqs, int32_t num_requests, float scale, float* weights,
+                          int32_t observe, void* out, float* lse, void* workspace, int64_t workspace_bytes,
+                          void* stream) {
+  if (!half_dtype(dtype)) return fail(OSCAR_ERR_UNSUPPORTED, "paged_attention: queries must be bf16 or fp16");
+  if (!kernel_head_dim(head_dim))
+    return fail(OSCAR_ERR_UNSUPPORTED, "paged_attention: head_dim %d: kernels exist for 64, 128, 256", head_dim);
+  int st = check_paged(qsl, seqs, num_requests, n_tokens, num_q_heads, num_kv_heads);
+  if (st) return st;
+  if (!std::isfinite(scale) || scale <= 0.0f) return fail(OSCAR_ERR_INVALID, "paged_attention: scale must be positive and finite");
+  if (weights != nullptr && observe < 1) return fail(OSCAR_ERR_INVALID, "paged_attention: observe must be at least 1");
+  st = check_cache("paged_attention", k_cache, num_blocks, block_size, num_kv_heads, head_dim, k_stride_block,
+                   k_stride_token, k_stride_head);
+  if (!st)
+    st = check_cache("paged_attention", v_cache, num_blocks, block_size, num_kv_heads, head_dim, v_stride_block,
+                     v_stride_token, v_stride_head);
+  if (st) return st;
+  bool any = false;
+  for (int r = 0; r < num_requests; ++r) {
+    if (qsl[r + 1] == qsl[r] || seqs[r] == 0) continue;
+    any = true;
+    if (((int64_t)seqs[r] + block_size - 1) / block_size > bt_cols)
+      return fail(OSCAR_ERR_INVALID, "paged_attention: block table cannot cover the sequence");
+  }
+  if (bt_rows < num_requests || bt_cols < 0 || bt_stride < bt_cols)
+    return fail(OSCAR_ERR_INVALID, "paged_attention: missing request block-table rows");
+  if (any && (!block_table || num_blocks < 1))
+    return fail(OSCAR_ERR_INVALID, "paged_attention: a sequence needs caches and a block table");
+  if (n_tokens == 0) return OSCAR_OK;
+  if (!q || !out || !lse) return fail(OSCAR_ERR_INVALID, "paged_attention: null pointer");
+  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (q_token_stride | q_head_stride) % 8)
+    return fail(OSCAR_ERR_INVALID, "paged_attention: query rows, output and workspace must be 16-byte aligned");
+  PagedCall c{};
+  oscar::PagedArgs& a = c.args;
+  a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;
+  a.out = out, a.lse = lse;
+  a.hq = num_q_heads, a.hk = num_kv_heads, a.group = num_q_heads / num_kv_heads;
+  a.num_blocks = num_blocks, a.bs = block_size;
+  a.box = std::min(oscar::kPgKeys, block_size & -block_size);
+  a.table = block_table, a.table_stride = bt_stride;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.weights = weights;
+  a.observe = weights != nullptr ? observe : 0;
+  c.k_cache = k_cache, c.kcb = k_stride_block, c.kct = k_stride_token, c.kch = k_stride_head;
+  c.n = n_tokens;
+  c.stream = reinterpret_cast<cudaStream_t>(stream);
+  // without any key nothing is loaded: the maps only have to be valid
+  const void* kb = any ? k_cache : q;
+  const void* vb = any ? v_cache : q;
+  const int64_t nb = any ? num_blocks : 1;
+  if (!paged_map(&c.kmap, kb, dtype, nb, block_size, num_kv_heads, head_dim, k_stride_block, k_stride_token, k_stride_head, a.box) ||
+      !paged_map(&c.vmap, vb, dtype, nb, block_size, num_kv_heads, head_dim, v_stride_block, v_stride_token, v_stride_head, a.box))
+    return fail(OSCAR_ERR_INVALID, "paged_attention: the caches' strides do not fit a tensor map");
+  PagedBatch b;
+  for (int few = 0; few < 2; ++few)
+    for (int r = 0; r < num_requests;) {
+      r = paged_batch(b, r, few, qsl, seqs, num_requests, a.group, num_kv_heads, device_info().sms);
+      if (b.plan.num_req == 0) continue;
+      const PagedSpace space = paged_space(b, few, n_tokens, num_q_heads, head_dim, weights != nullptr);
+      if (workspace_bytes < space.total() || !workspace)
+        return fail(OSCAR_ERR_INVALID, "paged_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
+                    (long long)space.total());
+      uint8_t* at = reinterpret_cast<uint8_t*>(workspace);
+      a.stats = weights != nullptr ? reinterpret_cast<float2*>(at) : nullptr;
+      a.part_ml = reinterpret_cast<float2*>(at + space.stats);
+      a.part_o = reinterpret_cast<float*>(at + space.stats + space.part_ml);
+      a.scores = space.scores ? reinterpret_cast<float*>(at + space.stats + space.part_ml + space.part_o) : nullptr;
+      st = dtype == OSCAR_DTYPE_BF16 ? launch_paged_d<__nv_bfloat16>(head_dim, c, b, few)
+                                     : launch_paged_d<__half>(head_dim, c, b, few);
+      if (st) return st;
+    }
+  return OSCAR_OK;
+}
+
+// ---------------------------------------------------------------------------
+int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t num_blocks, int32_t block_size,
+                      int32_t num_kv_heads, int64_t k_stride_block, int64_t k_stride_token, int64_t k_stride_head,
+                      int64_t v_stride_block, int64_t v_stride_token, int64_t v_stride_head, float* weights,
+                      const int32_t* block_table, int64_t bt_rows, int64_t bt_cols, int64_t bt_stride,
+                      const int32_t* dst_table, int64_t dst_rows, int64_t dst_cols, int64_t dst_stride,
+                      const int32_t* seqs, int32_t num_requests, int32_t keep, int32_t sink, int32_t recent,
+                      int32_t* kept, int32_t kept_cols, void* stream) {
+  if (!kernel_head_dim(head_dim))
+    return fail(OSCAR_ERR_UNSUPPORTED, "evict_cache: head_dim %d: kernels exist for 64, 128, 256", head_dim);
+  if (keep < 1 || sink < 0 || recent < 0 || (int64_t)sink + recent > keep)
+    return fail(OSCAR_ERR_INVALID, "evict_cache: keep must be at least 1 and hold the sink and recent tokens");
+  if (num_requests < 0 || (num_requests > 0 && !seqs) || num_kv_heads < 1 || num_kv_heads > 255)
+    return fail(OSCAR_ERR_INVALID, "evict_cache: invalid geometry");
+  int st = check_cache("evict_cache", k_cache, num_blocks, block_size, num_kv_heads, head_dim, k_stride_block,
+                       k_stride_token, k_stride_head);
+  if (!st)
+    st = check_cache("evict_cache", v_cache, num_blocks, block_size, num_kv_heads, head_dim, v_stride_block,
+                     v_stride_token, v_stride_head);
+  if (st) return st;
+  const bool in_place = dst_table == nullptr;
+  int most = 0;
+  bool any = false;
+  for (int r = 0; r < num_requests; ++r) {
+    if (seqs[r] < 0) return fail(OSCAR_ERR_INVALID, "evict_cache: lengths must not be negative");
+    const int n = std::min(seqs[r], keep);
+    most = std::max(most, n);
+    any = any || n > 0;
+    if (((int64_t)seqs[r] + block_size - 1) / block_size > bt_cols)
+      return fail(OSCAR_ERR_INVALID, "evict_cache: block table cannot cover the sequence");
+    if (!in_place && ((int64_t)n + block_size - 1) / block_size > dst_cols)
+      return fail(OSCAR_ERR_INVALID, "evict_cache: destination table cannot cover the kept keys");
+  }
+  if (bt_rows < num_requests || bt_stride < bt_cols || (!in_place && (dst_rows < num_requests || dst_stride < dst_cols)))
+    return fail(OSCAR_ERR_INVALID, "evict_cache: missing request block-table rows");
+  if (kept_cols < most) return fail(OSCAR_ERR_INVALID, "evict_cache: the list of kept keys has %d places, %d needed", kept_cols, most);
+  if (!any) return OSCAR_OK;
+  if (!weights || !block_table || !kept || num_blocks < 1) return fail(OSCAR_ERR_INVALID, "evict_cache: null pointer");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  oscar::EvictArgs a{};
+  a.k = reinterpret_cast<uint8_t*>(k_cache), a.v = reinterpret_cast<uint8_t*>(v_cache);
+  a.kb = 2 * k_stride_block, a.kt = 2 * k_stride_token, a.kh = 2 * k_stride_head;
+  a.vb = 2 * v_stride_block, a.vt = 2 * v_stride_token, a.vh = 2 * v_stride_head;
+  a.weights = weights;
+  a.num_blocks = num_blocks, a.bs = block_size, a.hk = num_kv_heads;
+  a.row_bytes = 2 * head_dim;
+  a.table = block_table, a.table_stride = bt_stride;
+  a.dst = in_place ? block_table : dst_table, a.dst_stride = in_place ? bt_stride : dst_stride;
+  a.keep = keep, a.sink = sink, a.recent = recent;
+  a.kept = kept, a.kept_stride = kept_cols;
+  oscar::EvictPlan p;
+  for (int r = 0; r < num_requests;) {
+    p.num_req = 0;
+    int longest = 0, moved = 0;
+    for (; r < num_requests && p.num_req < oscar::kEvReqs; ++r) {
+      p.req_id[p.num_req] = r;
+      p.seq[p.num_req++] = seqs[r];
+      if (seqs[r] <= oscar::kEvCached) longest = std::max(longest, seqs[r]);
+      moved = std::max(moved, std::min(seqs[r], keep));
+    }
+    allow_smem<oscar::evict_select_kernel>(oscar::kEvCached * sizeof(float));
+    launch_pdl(oscar::evict_select_kernel, dim3(p.num_req, num_kv_heads), dim3(oscar::kEvThreads),
+               std::max(16, longest * (int)sizeof(float)), s, a, p);
+    st = cuda_status("evict_select_kernel");
+    if (st) return st;
+    if (moved == 0) continue;
+    if (in_place) {
+      launch_pdl(oscar::evict_move_kernel, dim3(p.num_req * num_kv_heads, 2, a.row_bytes / 128),
+                 dim3(oscar::kEvMoveThreads), 0, s, a, p);
+      st = cuda_status("evict_move_kernel");
+    } else {
+      const int rows = oscar::kEvMoveThreads / (a.row_bytes / 16) * 4;
+      launch_pdl(oscar::evict_copy_kernel, dim3((moved + rows - 1) / rows, p.num_req * num_kv_heads),
+                 dim3(oscar::kEvMoveThreads), 0, s, a, p);
+      st = cuda_status("evict_copy_kernel");
+    }
+    if (st) return st;
+  }
+  return OSCAR_OK;
+}
+
+}  // extern "C"

@@ -10,6 +10,10 @@ Mirrors the reference's kernel entry points for the hot path:
                           (split-KV across GPUs)
   * ``merge_slab``        kernels/slab_attention.py:341-373
 
+and has the attention step of a 16-bit paged layer (the MTP draft layers,
+which the reference leaves to the engine): ``qk_norm_rope``,
+``paged_attention`` and ``evict_cache``.
+
 Layout problems raise ValueError with the reference's messages; every call
 is asynchronous on the current CUDA stream and never synchronises the host.
 There is no CPU path: CPU tensors raise.
@@ -396,6 +400,193 @@ def merge_slab(output, lse, part, part_lse, start, ids) -> None:
     check(_native.lib().oscar_merge_slab(output.data_ptr(), lse.data_ptr(), output.shape[0], part.data_ptr(),
                                          _DTYPES[part.dtype],
                                          part_lse.data_ptr(), n, hq, d, int(start), _ptr(ids_t), _stream(dev)))
+
+
+# ---------------------------------------------------------------------------
+# the 16-bit paged layer
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    """[n, heads, D] with contiguous, 16-byte aligned head vectors (a copy of t where its layout has none)."""
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _cache16(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, hk: int, d: int) -> None:
+    for t in (k_cache, v_cache):
+        if t.ndim != 4 or t.shape[2] != hk or t.shape[3] != d or t.shape != k_cache.shape:
+            raise ValueError(f"{name}: caches must be [blocks, tokens, {hk}, {d}] and alike")
+        if t.dtype != dtype:
+            raise ValueError(f"{name}: the caches must have the heads' type {dtype}, got {t.dtype}")
+        if t.stride(3) != 1:
+            raise ValueError(f"{name}: cache rows must be contiguous in the last dim")
+
+
+def _host_ints(values) -> np.ndarray:
+    if isinstance(values, torch.Tensor):
+        values = values.cpu().numpy()
+    return np.ascontiguousarray(values, dtype=np.int32)
+
+
+def _table32(name: str, table: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    if table.ndim != 2:
+        raise ValueError(f"{name}: the block table must be [requests, pages]")
+    if table.dtype != torch.int32:
+        table = table.to(torch.int32)
+    return table if table.stride(1) == 1 else table.contiguous()
+
+
+def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight_offset: float = 0.0,
+                 interleaved: bool = False, k_cache=None, v_cache=None, slot_mapping=None, out_q=None, out_k=None):
+    """RMS norm of every query and key head, position rotation and (with
+    caches) the write of the step's keys and values to a 16-bit paged cache,
+    in one pass.
+
+    q [n, Hq, D], k / v [n, Hk, D] (bf16 or fp16; views of a fused projection
+    are fine); weights [D] and ``cos_sin`` [max_positions, rot] (cosines, then
+    sines) in fp32 or the heads' type; ``positions`` [n].  ``weight_offset``
+    1 is the zero-centred weight (1 + w).  Pairs (i, i + rot/2) rotate, or
+    neighbours (2i, 2i + 1) with ``interleaved``.  Without caches the keys come
+    back (v is not needed); with them k and v go to ``slot_mapping`` (slots
+    < 0 are skipped) and the keys come back only into a given ``out_k``.
+    Returns (out_q, out_k)."""
+    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+        raise ValueError("qk_norm_rope: q [n, Hq, D] and k [n, Hk, D] of one type are needed")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"qk_norm_rope: unsupported type {q.dtype}")
+    n, hq, d = q.shape
+    hk = k.shape[1]
+    write = k_cache is not None
+    if write != (v_cache is not None) or write != (slot_mapping is not None) or (write and v is None):
+        raise ValueError("qk_norm_rope: v, caches and slot_mapping come together")
+    dev = _require_cuda(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, slot_mapping, out_q, out_k)
+    if q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype != k_weight.dtype:
+        raise ValueError(f"qk_norm_rope: the weights must be two [{d}] tensors of one type")
+    if cos_sin.ndim != 2 or positions.ndim != 1 or positions.shape[0] != n:
+        raise ValueError("qk_norm_rope: cos_sin [max_positions, rot] and positions [n] are needed")
+    for t in (q_weight, cos_sin):
+        if t.dtype not in (torch.float32, q.dtype):
+            raise ValueError("qk_norm_rope: weights and cos_sin must be fp32 or of the heads' type")
+    q, k = _rows16(q), _rows16(k)
+    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
+    cos_sin = cos_sin if cos_sin.stride(1) == 1 and cos_sin.stride(0) % 8 == 0 else cos_sin.contiguous()
+    positions = positions.to(torch.int64).contiguous()
+    if out_q is None:
+        out_q = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+    if out_k is None and not write:
+        out_k = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
+    for t, heads in ((out_q, hq), (out_k, hk)):
+        if t is not None and (t.shape != (n, heads, d) or t.dtype != q.dtype or t.stride(2) != 1):
+            raise ValueError(f"qk_norm_rope: outputs must be [{n}, {heads}, {d}] rows of {q.dtype}")
+    nb = bs = 1
+    ks = vs = (d, d, d)
+    vt = (0, 0)
+    if write:
+        if v.shape != k.shape or v.dtype != q.dtype:
+            raise ValueError("qk_norm_rope: v must match k")
+        v = _rows16(v)
+        vt = v.stride()
+        _cache16("qk_norm_rope", k_cache, v_cache, q.dtype, hk, d)
+        nb, bs = k_cache.shape[:2]
+        ks, vs = k_cache.stride(), v_cache.stride()
+        slot_mapping = slot_mapping.to(torch.int64).contiguous()
+        if slot_mapping.numel() < n:
+            raise ValueError("slot_mapping shorter than the token count")
+    qt, kt, oq = q.stride(), k.stride(), out_q.stride()
+    ok = (0, 0) if out_k is None else out_k.stride()
+    check(_native.lib().oscar_qk_norm_rope(
+        q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], _ptr(v) if write else None, vt[0], vt[1],
+        _DTYPES[q.dtype], n, hq, hk, d, q_weight.data_ptr(), k_weight.data_ptr(), _DTYPES[q_weight.dtype], float(eps),
+        float(weight_offset), cos_sin.data_ptr(), _DTYPES[cos_sin.dtype], cos_sin.stride(0), cos_sin.shape[0],
+        cos_sin.shape[1], 1 if interleaved else 0, positions.data_ptr(), out_q.data_ptr(), oq[0], oq[1], _ptr(out_k),
+        ok[0], ok[1], _ptr(k_cache), _ptr(v_cache), nb, bs, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        _ptr(slot_mapping), _stream(dev)))
+    return out_q, out_k
+
+
+def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=None, observe: int | None = None, out=None):
+    """Attention of each request's new tokens (one or thousands) over a paged
+    16-bit cache that already holds them: query i of request r sees keys
+    [0, seqs[r] - q_len + i].  Returns (out [n, Hq, D] in q's type, lse [n, Hq]
+    fp32 natural log); a row that sees no key is 0 with lse -inf.
+
+    q [n, Hq, D]; caches [blocks, tokens, Hk, D] of q's type (strided views
+    are fine); ``table`` [requests, pages]; ``qsl`` / ``seqs`` are host lists
+    or int32 arrays as in ``slab_attention``.
+
+    ``weights`` [blocks, Hk, tokens] fp32 accumulates the attention weight of
+    every cached key, summed over the heads of its group and the last
+    ``observe`` tokens of each request (None: all): keys older than the chunk
+    add it to what they have, the chunk's own keys start from it."""
+    if q.ndim != 3 or k_cache.ndim != 4 or k_cache.shape[2] < 1 or q.shape[1] % k_cache.shape[2]:
+        raise ValueError("paged_attention: q [n, Hq, D] with Hq a multiple of the caches' heads is needed")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"paged_attention: unsupported query type {q.dtype}")
+    n, hq, d = q.shape
+    nb, bs, hk = k_cache.shape[:3]
+    dev = _require_cuda(q, k_cache, v_cache, table, weights, out)
+    _cache16("paged_attention", k_cache, v_cache, q.dtype, hk, d)
+    qsl_a, seqs_a = _host_ints(qsl), _host_ints(seqs)
+    if qsl_a.ndim != 1 or seqs_a.ndim != 1 or qsl_a.size != seqs_a.size + 1 or qsl_a[0] != 0 or qsl_a[-1] != n:
+        raise ValueError("paged_attention: invalid query layout")
+    table = _table32("paged_attention", table, dev)
+    if weights is not None and (weights.shape != (nb, hk, bs) or weights.dtype != torch.float32
+                                or not weights.is_contiguous()):
+        raise ValueError(f"paged_attention: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")
+    if observe is not None and (weights is None or int(observe) < 1):
+        raise ValueError("paged_attention: observe needs weights and at least one token")
+    q = _rows16(q)
+    if out is None:
+        out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
+    elif out.shape != (n, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError(f"paged_attention: out must be contiguous [{n}, {hq}, {d}] of {q.dtype}")
+    lse = torch.empty(n, hq, dtype=torch.float32, device=dev)
+    lib = _native.lib()
+    qsl_p, seqs_p, b = qsl_a.ctypes.data, seqs_a.ctypes.data, seqs_a.size
+    need = lib.oscar_paged_attention_workspace(qsl_p, seqs_p, b, hq, hk, d, 0 if weights is None else 1)
+    if need < 0:
+        check(_native.ERR_INVALID)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
+    ks, vs, qs = k_cache.stride(), v_cache.stride(), q.stride()
+    check(lib.oscar_paged_attention(
+        q.data_ptr(), qs[0], qs[1], _DTYPES[q.dtype], n, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs,
+        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(), table.shape[0], table.shape[1], table.stride(0),
+        qsl_p, seqs_p, b, float(scale), _ptr(weights), 0x7FFFFFFF if observe is None else min(int(observe), 0x7FFFFFFF),
+        out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, _stream(dev)))
+    return out, lse
+
+
+def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int = 0, recent: int = 0, dst_table=None):
+    """Cuts every request with more than ``keep`` cached tokens down to
+    ``keep``, per kv head: the first ``sink``, the last ``recent`` and the
+    heaviest of the others by ``weights`` [blocks, Hk, tokens] stay in order
+    (ties: the lower position).  Their K, V and weight slots move to the front
+    of the request's pages, or to the pages of ``dst_table`` (for pages shared
+    with other requests, which must not be overwritten).  ``seqs``: host list.
+    Returns the kept positions [requests, Hk, min(keep, max(seqs))] int32 (-1
+    past a request's list); the new lengths are min(seqs, keep)."""
+    if k_cache.ndim != 4:
+        raise ValueError("evict_cache: caches must be [blocks, tokens, heads, D]")
+    nb, bs, hk, d = k_cache.shape
+    if k_cache.dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"evict_cache: unsupported cache type {k_cache.dtype}")
+    dev = _require_cuda(k_cache, v_cache, weights, table, dst_table)
+    _cache16("evict_cache", k_cache, v_cache, k_cache.dtype, hk, d)
+    if weights.shape != (nb, hk, bs) or weights.dtype != torch.float32 or not weights.is_contiguous():
+        raise ValueError(f"evict_cache: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")
+    seqs_a = _host_ints(seqs)
+    if seqs_a.ndim != 1:
+        raise ValueError("evict_cache: seqs must be a list of lengths")
+    table = _table32("evict_cache", table, dev)
+    dst = None if dst_table is None else _table32("evict_cache", dst_table, dev)
+    cols = max(0, min(int(keep), int(seqs_a.max(initial=0))))
+    kept = torch.empty(seqs_a.size, hk, cols, dtype=torch.int32, device=dev)
+    ks, vs = k_cache.stride(), v_cache.stride()
+    check(_native.lib().oscar_evict_cache(
+        k_cache.data_ptr(), v_cache.data_ptr(), d, nb, bs, hk, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        weights.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], table.stride(0), _ptr(dst),
+        0 if dst is None else dst.shape[0], 0 if dst is None else dst.shape[1], 0 if dst is None else dst.stride(0),
+        seqs_a.ctypes.data, seqs_a.size, int(keep), int(sink), int(recent), kept.data_ptr(), cols, _stream(dev)))
+    return kept
 
 
 _PATHS = {"auto": 0, "tile": 1, "decode": 2, "tensor": 3}

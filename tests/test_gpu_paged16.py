@@ -1,0 +1,537 @@
+"""The 16-bit paged layer on the GPU against plain 64-bit implementations: head
+norm + rotation + cache write, attention over the paged cache, the keys'
+accumulated weights, eviction by weight.
+
+Tolerances (u: unit roundoff of the type, half of its eps, 2^-8 bf16, 2^-11 fp16):
+  * attention output: the probabilities are rounded to the type for the P V
+    product and the result once more, so |err| <= u (sum p |v| + |o|); scores
+    carry fp32 errors of at most SCORE (below), worth 2 SCORE sum p |v|; fp16
+    probabilities under 2^-14 of the largest lose at most 2^-25 each.
+  * LSE and weights: a score is a sum of D products in fp32, error at most
+    D 2^-24 sum |q k| scale < 2^-24 * 256 * 260 / 16 < 2.6e-4 for N(0, 1)
+    inputs (sum |q k| < 260 at D 256); a weight is a sum of exp(score - lse)
+    with a relative error of twice that.
+  * head norm: fp32 throughout, one rounding: u |y| + 4e-6 |largest partner|."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_helpers import need_gpu
+
+pytestmark = pytest.mark.gpu
+
+U = {t: torch.finfo(t).eps / 2 for t in (torch.bfloat16, torch.float16)}
+SCORE = 2.6e-4
+
+
+def randn(gen, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=gen, device="cuda").to(dtype)
+
+
+def make_pool(gen, seqs, page, hk, d, dtype, *, spare=3, layout="plain", poison=True):
+    """Caches whose pages lie in random order; slots no request owns hold NaN / inf."""
+    need = [-(-s // page) for s in seqs]
+    blocks = sum(need) + spare
+    perm = torch.randperm(blocks, generator=gen, device="cuda").to(torch.int32)
+    width = max(max(need, default=0), 1) + 2
+    table = torch.full((len(seqs), width), -7, dtype=torch.int32, device="cuda")
+    at = 0
+    for r, n in enumerate(need):
+        table[r, :n] = perm[at:at + n]
+        at += n
+    if layout == "plain":
+        kc, vc = randn(gen, blocks, page, hk, d, dtype=dtype), randn(gen, blocks, page, hk, d, dtype=dtype)
+    elif layout == "halves":  # K and V of a block adjacent
+        pool = randn(gen, blocks, 2, page, hk, d, dtype=dtype)
+        kc, vc = pool[:, 0], pool[:, 1]
+    else:  # heads before tokens
+        kc = randn(gen, blocks, hk, page, d, dtype=dtype).transpose(1, 2)
+        vc = randn(gen, blocks, hk, page, d, dtype=dtype).transpose(1, 2)
+    if poison:
+        owned = torch.zeros(blocks, page, dtype=torch.bool, device="cuda")
+        for r, s in enumerate(seqs):
+            p = torch.arange(s, device="cuda")
+            owned[table[r].long()[p // page], p % page] = True
+        for c, bad in ((kc, math.nan), (vc, math.inf)):
+            c.masked_fill_(~owned[:, :, None, None], bad)
+    return kc, vc, table
+
+
+def gather(cache, table, r, seq):
+    p = torch.arange(seq, device="cuda")
+    page = cache.shape[1]
+    return cache[table[r].long()[p // page], p % page]
+
+
+def attention64(q, kc, vc, table, lens, seqs, scale, observe=None):
+    """(out, sum p |v|, lse, [mass per request [hk, seq]]) in 64 bits."""
+    n, hq, d = q.shape
+    hk = kc.shape[2]
+    g = hq // hk
+    out = torch.zeros(n, hq, d, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(out)
+    lse = torch.full((n, hq), -math.inf, dtype=torch.float64, device="cuda")
+    masses, at = [], 0
+    for r, (m, seq) in enumerate(zip(lens, seqs)):
+        mass = torch.zeros(hk, seq, dtype=torch.float64, device="cuda")
+        if m and seq:
+            k, v = gather(kc, table, r, seq).double(), gather(vc, table, r, seq).double()
+            qq = q[at:at + m].double().view(m, hk, g, d)
+            x = torch.einsum("mhgd,khd->mhgk", qq, k) * scale
+            sees = (seq - m + 1 + torch.arange(m, device="cuda"))[:, None]
+            x = x.masked_fill((torch.arange(seq, device="cuda")[None] >= sees)[:, None, None], -math.inf)
+            z = torch.logsumexp(x, -1)
+            p = torch.where(x == -math.inf, 0.0, torch.exp(x - torch.where(z == -math.inf, 0.0, z)[..., None]))
+            out[at:at + m] = torch.einsum("mhgk,khd->mhgd", p, v).reshape(m, hq, d)
+            size[at:at + m] = torch.einsum("mhgk,khd->mhgd", p, v.abs()).reshape(m, hq, d)
+            lse[at:at + m] = z.reshape(m, hq)
+            mass = p[max(0, m - (observe or m)):].sum((0, 2))
+        masses.append(mass)
+        at += m
+    return out, size, lse, masses
+
+
+def check_attention(q, out, lse, want, seqs):
+    o, size, z, _ = want
+    u = U[q.dtype]
+    tiny = max(seqs, default=0) * 2.0**-25 * 6.0 if q.dtype == torch.float16 else 0.0
+    bound = u * (size + o.abs()) * 1.01 + 2 * SCORE * size + tiny
+    off = (out.double() - o).abs()
+    assert torch.isfinite(out.float()).all()
+    assert (off <= bound).all(), float((off - bound).max())
+    empty = z == -math.inf
+    assert torch.equal(lse == -math.inf, empty)
+    assert (out[empty] == 0).all()
+    assert ((lse.double() - z)[~empty].abs() <= SCORE).all()
+
+
+# (new tokens, cached lengths, options)
+CASES = [
+    ([1], [1], dict()),
+    ([1], [64], dict()),
+    ([1], [8192], dict()),
+    ([4] * 3, [3000, 65, 4], dict()),
+    ([1, 0, 3, 2, 4], [1500, 700, 128, 2, 129], dict(page=16)),
+    ([4, 4], [2049, 700], dict(hq=6, hk=1)),
+    ([2, 1], [900, 333], dict(hq=24, hk=4, d=128, dtype=torch.float16, page=48)),
+    ([3, 1], [1000, 63], dict(hq=8, hk=8, d=64, dtype=torch.float16, page=32)),
+    ([1, 5], [700, 77], dict(hq=16, hk=2, d=128, page=5)),                 # pages no box of two tokens divides
+    ([7], [7], dict(hq=32, hk=1, d=64, page=1)),                            # every token its own page
+    ([5, 3], [2, 0], dict()),                                               # rows that see no key
+    ([300], [300], dict(hq=24, hk=4)),                                      # a prompt
+    ([130, 1, 33], [1130, 900, 33], dict(hq=12, hk=2, page=784)),           # a chunk beside decode
+    ([257], [1281], dict(hq=24, hk=4, dtype=torch.float16)),
+    ([200, 129], [200, 1000], dict(hq=24, hk=4, d=128, dtype=torch.float16, page=16)),
+    ([511], [3100], dict(hq=10, hk=2, d=64, page=64)),
+    ([128], [4096], dict(hq=8, hk=2, d=128, page=24)),
+    ([40], [100], dict(hq=40, hk=1, d=256, page=128)),
+    ([3], [20000], dict(hq=8, hk=1, d=256)),
+]
+
+
+def make_call(lens, seqs, opts, seed=0):
+    o = dict(hq=24, hk=4, d=256, dtype=torch.bfloat16, page=128, layout="plain")
+    o.update(opts)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    kc, vc, table = make_pool(gen, seqs, o["page"], o["hk"], o["d"], o["dtype"], layout=o["layout"])
+    q = randn(gen, sum(lens), o["hq"], o["d"], dtype=o["dtype"])
+    qsl = np.concatenate([[0], np.cumsum(lens)]).astype(np.int32)
+    return q, kc, vc, table, qsl, o["d"] ** -0.5
+
+
+@pytest.mark.parametrize("lens,seqs,opts", CASES)
+def test_paged_attention(lens, seqs, opts):
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, opts)
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl.tolist(), seqs, scale)
+    check_attention(q, out, lse, attention64(q, kc, vc, table, lens, seqs, scale), seqs)
+    assert out.dtype == q.dtype and lse.dtype == torch.float32
+    again, lse2 = kernels.paged_attention(q, kc, vc, table, qsl, np.asarray(seqs, np.int32), scale)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert kernels.device_error(dev) == 0
+
+
+@pytest.mark.parametrize("layout", ["halves", "heads"])
+@pytest.mark.parametrize("lens,seqs", [([2, 4], [300, 1025]), ([150], [700])])
+def test_paged_attention_strided(layout, lens, seqs):
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict(layout=layout, page=32))
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    fused = randn(gen, q.shape[0], q.shape[1] + 8, q.shape[2], dtype=q.dtype)
+    view = fused[:, 3:3 + q.shape[1]]
+    view.copy_(q)
+    out, lse = kernels.paged_attention(view, kc, vc, table, qsl, seqs, scale)
+    check_attention(q, out, lse, attention64(q, kc, vc, table, lens, seqs, scale), seqs)
+
+
+def test_paged_attention_many_requests():
+    """More requests than one launch holds, decode and chunks mixed."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    lens = [1 + (i % 3) + (60 if i % 97 == 5 else 0) for i in range(600)]
+    seqs = [n + (i * 37) % 301 for i, n in enumerate(lens)]
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict(hq=4, hk=2, d=64, page=16))
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    check_attention(q, out, lse, attention64(q, kc, vc, table, lens, seqs, scale), seqs)
+
+
+def test_paged_attention_large_scores():
+    """Scores that grow along the keys move the running maximum again and again."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    for lens, seqs in (([2], [2000]), ([200], [2000])):
+        q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict(hq=4, hk=2, d=128))
+        for p in range(0, 2000, 64):
+            blk, off = int(table[0, p // 128]), p % 128
+            kc[blk, off] = kc[blk, off] * (1 + p / 250)
+        out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+        o, size, z, _ = attention64(q, kc, vc, table, lens, seqs, scale)
+        # scores reach 9 times N(0, 1) ones
+        bound = U[q.dtype] * (size + o.abs()) * 1.01 + 18 * SCORE * size
+        assert ((out.double() - o).abs() <= bound).all()
+        assert ((lse.double() - z).abs() <= 9 * SCORE).all()
+
+
+def test_paged_attention_nan_key_and_value():
+    """A NaN key makes the rows that see it NaN and leaves other requests alone."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    lens, seqs = [1, 1], [200, 130]
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict())
+    kc[int(table[0, 0]), 5, 0, 3] = math.nan
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    assert torch.isnan(out[0, :6]).all() and torch.isnan(lse[0, :6]).all()
+    assert torch.isfinite(out[0, 6:]).all() and torch.isfinite(out[1]).all()
+
+
+def test_paged_attention_bad_block_is_flagged():
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    for lens in ([1], [100]):
+        q, kc, vc, table, qsl, scale = make_call(lens, [400], dict())
+        table[0, 1] = kc.shape[0] + 5
+        kernels.paged_attention(q, kc, vc, table, qsl, [400], scale)
+        assert kernels.device_error(dev) & 2
+    assert kernels.device_error(dev) == 0
+
+
+def test_paged_attention_other_stream_and_preallocated_out():
+    from oscar_b200 import kernels
+
+    need_gpu()
+    lens, seqs = [4, 4], [3000, 500]
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict())
+    want, _ = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out = torch.full_like(q, math.nan)
+        got, _ = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale, out=out)
+    side.synchronize()
+    assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
+
+
+WEIGHT_CASES = [
+    ([1], [1000], None, dict()),
+    ([4, 1, 0, 2], [2000, 65, 70, 1], None, dict()),
+    ([4, 3], [700, 90], 2, dict(hq=24, hk=4, d=128, dtype=torch.float16, page=48)),
+    ([5], [3], None, dict(hq=8, hk=2, d=64, page=16)),
+    ([150, 1], [700, 300], None, dict()),
+    ([300], [300], 64, dict(hq=12, hk=2, d=128, page=16)),
+    ([90, 64], [1200, 64], 17, dict(hq=8, hk=1, d=64, dtype=torch.float16, page=5)),
+    ([40], [30], None, dict()),
+]
+
+
+@pytest.mark.parametrize("lens,seqs,observe,opts", WEIGHT_CASES)
+def test_key_weights(lens, seqs, observe, opts):
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, opts)
+    nb, page, hk = kc.shape[:3]
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    start = torch.rand(nb, hk, page, generator=gen, device="cuda")
+    weights = start.clone()
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale, weights=weights, observe=observe)
+    want = attention64(q, kc, vc, table, lens, seqs, scale, observe)
+    check_attention(q, out, lse, want, seqs)
+    plain, _ = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    assert torch.equal(out, plain)
+    touched = torch.zeros(nb, page, dtype=torch.bool, device="cuda")
+    for r, (m, seq) in enumerate(zip(lens, seqs)):
+        if m == 0:
+            continue
+        p = torch.arange(seq, device="cuda")
+        blk, off = table[r].long()[p // page], p % page
+        touched[blk, off] = True
+        old = torch.where(p < seq - m, start[blk, :, off].T.double(), 0.0)
+        mass = want[3][r]
+        got = weights[blk, :, off].T.double()
+        assert ((got - old - mass).abs() <= 2 * SCORE * mass + 2.0**-23 * (old + mass)).all()
+    untouched = ~touched[:, None, :].expand_as(weights)
+    assert torch.equal(weights[untouched], start[untouched])
+    assert kernels.device_error(dev) == 0
+
+
+def test_key_weights_of_shared_history_add_up():
+    from oscar_b200 import kernels
+
+    need_gpu()
+    lens, seqs = [1, 1], [200, 200]
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict(page=64))
+    table[1, :3] = table[0, :3]  # 192 tokens of shared prefix
+    weights = torch.zeros(kc.shape[0], 4, 64, device="cuda")
+    kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale, weights=weights)
+    masses = attention64(q, kc, vc, table, lens, seqs, scale)[3]
+    p = torch.arange(192, device="cuda")
+    got = weights[table[0].long()[p // 64], :, p % 64].T.double()
+    want = masses[0][:, :192] + masses[1][:, :192]
+    assert ((got - want).abs() <= 2 * SCORE * want + 2.0**-23).all()
+
+
+# ---------------------------------------------------------------------------
+def rope64(x, w, offset, eps, cos_sin, positions, interleaved):
+    x = x.double()
+    rot = cos_sin.shape[1]
+    y = x / torch.sqrt(x.square().mean(-1, keepdim=True) + eps) * (w.double() + offset)
+    first = torch.arange(0, rot, 2) if interleaved else torch.arange(rot // 2)
+    second = first + (1 if interleaved else rot // 2)
+    row = cos_sin.double()[positions][:, None]
+    c, s = row[..., :rot // 2], row[..., rot // 2:]
+    z = y.clone()
+    z[..., first] = c * y[..., first] - s * y[..., second]
+    z[..., second] = s * y[..., first] + c * y[..., second]
+    reach = y.abs().amax(-1, keepdim=True)
+    return z, reach
+
+
+def check_rows(got, want, reach, dtype):
+    assert ((got.double() - want).abs() <= U[dtype] * want.abs() * 1.001 + 4e-6 * reach + 2.0**-25).all()
+
+
+ROPE_CASES = [
+    (1, dict()), (32, dict()), (1237, dict(hq=16, hk=2, d=128, rot=128, interleaved=True, dtype=torch.float16, offset=0.0)),
+    (7, dict(hq=5, hk=1, d=64, rot=16)), (65, dict(hq=8, hk=8, d=64, rot=64, dtype=torch.float16)),
+    (33, dict(hq=3, hk=3, d=128, rot=48, w_dtype=torch.float32, table_dtype=torch.bfloat16)),
+    (100, dict(rot=256)), (100, dict(rot=128, interleaved=True)), (511, dict(hq=6, hk=1, rot=64, page=16)),
+]
+
+
+def make_rope(n, opts, seed=3):
+    o = dict(hq=24, hk=4, d=256, rot=64, dtype=torch.bfloat16, interleaved=False, offset=1.0, page=128, w_dtype=None,
+             table_dtype=torch.float32)
+    o.update(opts)
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    dt, d = o["dtype"], o["d"]
+    qkv = randn(gen, n, o["hq"] + 2 * o["hk"], d, dtype=dt)
+    q, k, v = qkv.split([o["hq"], o["hk"], o["hk"]], dim=1)
+    wq, wk = (randn(gen, d).mul(0.1).add(1 - o["offset"]).to(o["w_dtype"] or dt) for _ in range(2))
+    angle = torch.arange(500, device="cuda", dtype=torch.float64)[:, None] * 1e4 ** (
+        -torch.arange(0, o["rot"], 2, device="cuda", dtype=torch.float64) / o["rot"])
+    cos_sin = torch.cat([angle.cos(), angle.sin()], -1).to(o["table_dtype"])
+    positions = torch.randint(0, 500, (n,), generator=gen, device="cuda")
+    return q, k, v, wq, wk, cos_sin, positions, o, gen
+
+
+@pytest.mark.parametrize("n,opts", ROPE_CASES)
+@pytest.mark.parametrize("layout", ["plain", "halves", "heads"])
+def test_qk_norm_rope(n, opts, layout):
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, k, v, wq, wk, cos_sin, positions, o, gen = make_rope(n, opts)
+    page, hk, d, dt = o["page"], o["hk"], o["d"], o["dtype"]
+    blocks = -(-n // page) + 2
+    kc, vc, _ = make_pool(gen, [0], page, hk, d, dt, spare=blocks, layout=layout, poison=False)
+    k0, v0 = kc.clone(), vc.clone()
+    slots = torch.randperm(blocks * page, generator=gen, device="cuda")[:n]
+    slots[::5] = -1
+    kw = dict(weight_offset=o["offset"], interleaved=o["interleaved"])
+    oq, ok = kernels.qk_norm_rope(q, k, v, wq, wk, 1e-6, cos_sin, positions, k_cache=kc, v_cache=vc, slot_mapping=slots, **kw)
+    assert ok is None
+    wantq, reachq = rope64(q, wq, o["offset"], 1e-6, cos_sin, positions, o["interleaved"])
+    wantk, reachk = rope64(k, wk, o["offset"], 1e-6, cos_sin, positions, o["interleaved"])
+    check_rows(oq, wantq, reachq, dt)
+    oq2, ok2 = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions.int(), **kw)
+    assert torch.equal(oq, oq2)
+    check_rows(ok2, wantk, reachk, dt)
+    live = slots >= 0
+    k0[slots[live] // page, slots[live] % page] = ok2[live]
+    v0[slots[live] // page, slots[live] % page] = v[live]
+    assert torch.equal(kc, k0) and torch.equal(vc, v0)
+    # in place, and keys returned beside the cache write
+    qc, kk = q.clone(), k.clone()
+    kernels.qk_norm_rope(qc, kk, v, wq, wk, 1e-6, cos_sin, positions, k_cache=kc, v_cache=vc, slot_mapping=slots,
+                         out_q=qc, out_k=kk, **kw)
+    assert torch.equal(qc, oq) and torch.equal(kk, ok2)
+    assert kernels.device_error(dev) == 0
+
+
+def test_qk_norm_rope_extremes():
+    """Zero heads stay zero, an inf or NaN stays in its head, no tokens is no work."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, k, v, wq, wk, cos_sin, positions, o, _ = make_rope(4, dict())
+    q = q.clone()
+    q[0, 0] = 0
+    q[1, 1, 7] = math.nan
+    q[2, 2] = 1e4
+    oq, _ = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions, weight_offset=1.0)
+    assert (oq[0, 0] == 0).all() and torch.isnan(oq[1, 1]).all()
+    rest = torch.ones(4, 24, dtype=torch.bool, device="cuda")
+    rest[1, 1] = False
+    assert torch.isfinite(oq[rest]).all()
+    empty, _ = kernels.qk_norm_rope(q[:0], k[:0], None, wq, wk, 1e-6, cos_sin, positions[:0])
+    assert empty.shape == (0, 24, 256)
+
+
+def test_qk_norm_rope_flags_bad_positions_and_slots():
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, k, v, wq, wk, cos_sin, positions, o, gen = make_rope(6, dict())
+    kc, vc, _ = make_pool(gen, [0], 128, 4, 256, torch.bfloat16, spare=1, poison=False)
+    k0 = kc.clone()
+    positions[2] = 500
+    positions[3] = -1
+    slots = torch.tensor([-1, 128, 2, 3, -1, -1], device="cuda")
+    kernels.qk_norm_rope(q, k, v, wq, wk, 1e-6, cos_sin, positions, k_cache=kc, v_cache=vc, slot_mapping=slots)
+    assert kernels.device_error(dev) == 64 | 1
+    assert torch.equal(kc, k0)
+
+
+# ---------------------------------------------------------------------------
+def kept64(w, keep, sink, recent):
+    """Kept positions of one head: numpy, stable, NaN above every number."""
+    n = w.size
+    if n <= keep:
+        return np.arange(n)
+    mid = np.arange(sink, n - recent)
+    rank = np.where(np.isnan(w[mid]), np.inf, w[mid].astype(np.float64))
+    nan_first = ~np.isnan(w[mid])
+    order = mid[np.lexsort((mid, -rank, nan_first))]
+    return np.sort(np.concatenate([np.arange(sink), order[:keep - sink - recent], np.arange(n - recent, n)]))
+
+
+EVICT_CASES = [
+    ([300], 100, 4, 10, dict()),
+    ([300, 20, 1000, 0, 101], 100, 0, 0, dict(page=16)),
+    ([5000, 4097, 4096], 4096, 64, 256, dict(hk=1)),
+    ([2500], 50, 25, 25, dict(hk=2, d=64, page=5, dtype=torch.float16)),     # nothing between sink and recent
+    ([777], 1, 0, 0, dict(hk=8, d=64, page=1)),
+    ([777], 776, 0, 1, dict(d=128, page=48, dtype=torch.float16)),
+    ([60000], 33000, 10, 100, dict(hk=1, d=64, page=64)),                    # more keys than shared memory holds
+]
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("values", ["spread", "ties", "zero", "signed"])
+@pytest.mark.parametrize("seqs,keep,sink,recent,opts", EVICT_CASES)
+def test_evict_cache(seqs, keep, sink, recent, opts, values, in_place):
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    o = dict(hk=4, d=256, dtype=torch.bfloat16, page=128)
+    o.update(opts)
+    page, hk = o["page"], o["hk"]
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    fresh = [-(-min(s, keep) // page) for s in seqs]
+    kc, vc, table = make_pool(gen, seqs, page, hk, o["d"], o["dtype"], spare=sum(fresh) + 1, poison=False)
+    nb = kc.shape[0]
+    w = torch.rand(nb, hk, page, generator=gen, device="cuda")
+    if values == "ties":
+        w = (w * 4).floor() / 4
+    elif values == "zero":
+        w = torch.zeros_like(w)
+    elif values == "signed":
+        w = w - 0.5
+        w[torch.rand(w.shape, generator=gen, device="cuda") < 0.02] = math.nan
+        w[torch.rand(w.shape, generator=gen, device="cuda") < 0.02] = -0.0
+        w[torch.rand(w.shape, generator=gen, device="cuda") < 0.02] = math.inf
+    dst = None
+    to = table
+    if not in_place:
+        used = set(int(x) for r, s in enumerate(seqs) for x in table[r, :-(-s // page)].tolist())
+        rest = [b for b in range(nb) if b not in used]
+        dst = torch.full((len(seqs), max(fresh) + 1), -1, dtype=torch.int32, device="cuda")
+        for r, n in enumerate(fresh):
+            dst[r, :n] = torch.tensor([rest.pop() for _ in range(n)], dtype=torch.int32)
+        to = dst
+    k0, v0, w0 = kc.clone(), vc.clone(), w.clone()
+    kept = kernels.evict_cache(kc, vc, w, table, seqs, keep, sink=sink, recent=recent, dst_table=dst)
+    assert kept.shape == (len(seqs), hk, min(keep, max(seqs)))
+    wk, wv, ww = k0.clone(), v0.clone(), w0.clone()
+    for r, seq in enumerate(seqs):
+        n = min(seq, keep)
+        p = torch.arange(seq, device="cuda")
+        blk, off = table[r].long()[p // page], p % page
+        j = torch.arange(n, device="cuda")
+        tb, tf = to[r].long()[j // page], j % page
+        for h in range(hk):
+            c = torch.from_numpy(kept64(w0[blk, h, off].cpu().numpy(), keep, sink, recent)).cuda()
+            assert torch.equal(kept[r, h, :n].long(), c)
+            assert (kept[r, h, n:] == -1).all()
+            wk[tb, tf, h] = k0[blk[c], off[c], h]
+            wv[tb, tf, h] = v0[blk[c], off[c], h]
+            ww[tb, h, tf] = w0[blk[c], h, off[c]]
+    assert torch.equal(kc, wk) and torch.equal(vc, wv)
+    assert torch.equal(w.view(torch.int32), ww.view(torch.int32))
+    assert kernels.device_error(dev) == 0
+
+
+def test_evict_strided_caches():
+    from oscar_b200 import kernels
+
+    need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    kc, vc, table = make_pool(gen, [500, 300], 32, 2, 128, torch.bfloat16, layout="halves", poison=False)
+    plain_k, plain_v = kc.contiguous(), vc.contiguous()
+    w = torch.rand(kc.shape[0], 2, 32, generator=gen, device="cuda")
+    w2 = w.clone()
+    a = kernels.evict_cache(kc, vc, w, table, [500, 300], 200, sink=3, recent=7)
+    b = kernels.evict_cache(plain_k, plain_v, w2, table, [500, 300], 200, sink=3, recent=7)
+    assert torch.equal(a, b) and torch.equal(kc, plain_k) and torch.equal(vc, plain_v) and torch.equal(w, w2)
+
+
+def test_offsets_past_32_bits():
+    """The used pages lie past 2^31 elements of the caches."""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    page, hk, d = 128, 4, 256
+    nb = 2**31 // (page * hk * d) + 40
+    kc, vc = (torch.empty(nb, page, hk, d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    w = torch.zeros(nb, hk, page, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    table = (nb - 1 - torch.arange(16, device="cuda", dtype=torch.int32))[None].contiguous()
+    small_table = torch.arange(15, -1, -1, device="cuda", dtype=torch.int32)[None].contiguous()
+    for lens, seq in (([3], 1999), ([200], 1999)):
+        kc[-16:] = randn(gen, 16, page, hk, d, dtype=torch.bfloat16)
+        vc[-16:] = randn(gen, 16, page, hk, d, dtype=torch.bfloat16)
+        q = randn(gen, lens[0], 24, d, dtype=torch.bfloat16)
+        sk, sv, sw = kc[-16:].clone(), vc[-16:].clone(), torch.zeros(16, hk, page, device="cuda")
+        w.zero_()
+        out, lse = kernels.paged_attention(q, kc, vc, table, [0, lens[0]], [seq], d**-0.5, weights=w)
+        want, lse2 = kernels.paged_attention(q, sk, sv, small_table, [0, lens[0]], [seq], d**-0.5, weights=sw)
+        assert torch.equal(out, want) and torch.equal(lse, lse2) and torch.equal(w[-16:], sw)
+        a = kernels.evict_cache(kc, vc, w, table, [seq], 700, sink=4, recent=64)
+        b = kernels.evict_cache(sk, sv, sw, small_table, [seq], 700, sink=4, recent=64)
+        assert torch.equal(a, b) and torch.equal(kc[-16:], sk) and torch.equal(vc[-16:], sv)
+    q, k, v, wq, wk, cos_sin, positions, o, gen = make_rope(9, dict())
+    slots = nb * page - 1 - torch.arange(9, device="cuda")
+    _, ok = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions)
+    kernels.qk_norm_rope(q, k, v, wq, wk, 1e-6, cos_sin, positions, k_cache=kc, v_cache=vc, slot_mapping=slots)
+    assert torch.equal(kc.view(-1, hk, d)[slots], ok) and torch.equal(vc.view(-1, hk, d)[slots], v)
+    assert kernels.device_error(dev) == 0
