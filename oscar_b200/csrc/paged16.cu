@@ -10,6 +10,7 @@
 #include "head_norm.cuh"
 #include "host.h"
 #include "paged.cuh"
+#include "paged_chunk.cuh"
 
 namespace oscar_host {
 
@@ -150,34 +151,90 @@ namespace {
 
 constexpr int kFewRows = 32;  // query rows of a (request, kv head) in one block of the split kernel
 
-// Workspace of one launch of the split kernel, in this order.
+// How a request's new tokens are attended: kFew in one block of the split
+// kernel, kChunk on the tensor-memory kernel, kWide (a group of more than 128
+// heads) in several blocks of the split kernel.
+enum PagedClass { kFew = 0, kChunk = 1, kWide = 2, kClasses = 3 };
+inline PagedClass paged_class(int64_t len, int group) {
+  if (len * group <= kFewRows) return kFew;
+  return group <= oscar::kPcRows ? kChunk : kWide;
+}
+
+// Workspace of one launch, in this order.
 struct PagedSpace {
   int64_t stats, part_ml, part_o, scores;  // bytes
   int64_t total() const { return stats + part_ml + part_o + scores; }
 };
 inline int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 
-// The requests [r0, ..) of a call that fit one launch: at most kPgReqs, those with
-// few rows or those with many.  Returns the index after the last one looked at.
+// The requests [r0, ..) of a call that fit one launch: at most kPgReqs of one
+// class.  Returns the index after the last one looked at.
 struct PagedBatch {
-  oscar::PagedPlan plan;
-  int rows;  // rows per block of the split kernel
+  PagedClass cls;
+  oscar::PagedPlan plan;   // kFew, kWide
+  int rows;                // rows per block of the split kernel
+  oscar::PcPlan chunk;     // kChunk
+  oscar::PcSplits splits;  // its divided units
+  int num() const { return cls == kChunk ? chunk.num_req : plan.num_req; }
 };
-int paged_batch(PagedBatch& b, int r0, bool few, const int32_t* qsl, const int32_t* seqs, int num, int group, int hk,
-                int sms) {
+
+template <int D>
+void plan_chunk(PagedBatch& b, int hk, int sms) {
+  oscar::PcPlan& p = b.chunk;
+  const int per = p.tokens * oscar::PcShape<D>::kM;
+  int64_t total = 0;
+  for (int i = 0; i < p.num_req; ++i)
+    for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb)
+      total += (int64_t)hk * oscar::pc_tiles<D>(p.q_len[i], p.seq[i], p.tokens, qb);
+  p.ctas = (int)std::min<int64_t>(std::min(std::max(sms, 1), oscar::kPcCtas), total);
+  b.splits.n = 0;
+  int64_t at = 0;  // tiles before the unit
+  int c = 0;       // CTAs begun
+  auto start_of = [&](int64_t i) { return total * i / p.ctas; };
+  for (int i = 0; i < p.num_req; ++i)
+    for (int h = 0; h < hk; ++h)
+      for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb) {
+        const int nt = oscar::pc_tiles<D>(p.q_len[i], p.seq[i], p.tokens, qb);
+        const bool at_start = c < p.ctas && start_of(c) == at;
+        const int first = at_start ? c : c - 1;  // the CTA that holds the unit's first tile
+        while (c < p.ctas && start_of(c) < at + nt) {
+          p.start[c] = oscar::PcStart{i, h, qb, (int)(start_of(c) - at)};
+          p.tiles[c] = (int)(start_of(c + 1) - start_of(c));
+          ++c;
+        }
+        if (c - 1 > first) b.splits.unit[b.splits.n++] = oscar::PcSplit{i, h, qb, first, c - 1};
+        at += nt;
+      }
+}
+
+int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const int32_t* seqs, int num, int group,
+                int hk, int d, int sms) {
   oscar::PagedPlan& p = b.plan;
-  p.num_req = 0;
-  int most = 0, r = r0;
-  for (; r < num && p.num_req < oscar::kPgReqs; ++r) {
-    const int64_t len = qsl[r + 1] - qsl[r], rows = len * group;
-    if (len == 0 || (rows <= kFewRows) != few) continue;
-    const int i = p.num_req++;
-    p.req_id[i] = r;
-    p.q_start[i] = qsl[r];
-    p.q_len[i] = (int)len;
-    p.seq[i] = seqs[r];
-    most = std::max<int64_t>(most, std::min<int64_t>(rows, kFewRows));
+  oscar::PcPlan& pc = b.chunk;
+  b.cls = cls;
+  p.num_req = pc.num_req = 0;
+  int64_t most = 0;
+  int r = r0, count = 0;
+  for (; r < num && count < oscar::kPgReqs; ++r) {
+    const int64_t len = qsl[r + 1] - qsl[r];
+    if (len == 0 || paged_class(len, group) != cls) continue;
+    const int i = count++;
+    (cls == kChunk ? pc.req_id : p.req_id)[i] = r;
+    (cls == kChunk ? pc.q_start : p.q_start)[i] = qsl[r];
+    (cls == kChunk ? pc.q_len : p.q_len)[i] = (int)len;
+    (cls == kChunk ? pc.seq : p.seq)[i] = seqs[r];
+    most = std::max(most, len * group);
   }
+  if (count == 0) return r;
+  if (cls == kChunk) {
+    pc.num_req = count;
+    pc.tokens = oscar::kPcRows / group;
+    if (d == 256) plan_chunk<256>(b, hk, sms);
+    else if (d == 128) plan_chunk<128>(b, hk, sms);
+    else plan_chunk<64>(b, hk, sms);
+    return r;
+  }
+  p.num_req = count;
   b.rows = most <= 16 ? 16 : kFewRows;
   int64_t tiles = 0;
   for (int i = 0; i < p.num_req; ++i) {
@@ -191,12 +248,14 @@ int paged_batch(PagedBatch& b, int r0, bool few, const int32_t* qsl, const int32
   return r;
 }
 
-PagedSpace paged_space(const PagedBatch& b, bool few, int64_t n, int hq, int d, bool weighted) {
+PagedSpace paged_space(const PagedBatch& b, int64_t n, int hq, int d, bool weighted) {
   PagedSpace s{};
   if (weighted) s.stats = round256(n * hq * (int64_t)sizeof(float2));
-  s.part_ml = round256((int64_t)2 * b.plan.ctas * b.rows * sizeof(float2));
-  s.part_o = round256((int64_t)2 * b.plan.ctas * b.rows * d * sizeof(float));
-  if (weighted && few) s.scores = b.plan.total_tiles * b.rows * oscar::kPgKeys * (int64_t)sizeof(float);
+  const int64_t pieces = b.cls == kChunk ? (int64_t)2 * b.chunk.ctas * oscar::kPcRows * (d == 256 ? 1 : 2)
+                                         : (int64_t)2 * b.plan.ctas * b.rows;
+  s.part_ml = round256(pieces * (int64_t)sizeof(float2));
+  s.part_o = round256(pieces * d * (int64_t)sizeof(float));
+  if (weighted && b.cls == kFew) s.scores = b.plan.total_tiles * b.rows * oscar::kPgKeys * (int64_t)sizeof(float);
   return s;
 }
 
@@ -227,6 +286,21 @@ bool paged_map(CUtensorMap* map, const void* base, int dtype, int64_t num_blocks
          CUDA_SUCCESS;
 }
 
+// The queries as a 3D map (dims, heads, tokens) in boxes of 64 dims x a kv head's group x `tokens`:
+// the rows (token, head in group) of a q-block's row tile.
+bool query_map(CUtensorMap* map, const void* q, int dtype, int64_t n, int hq, int d, int64_t tok, int64_t head, int group,
+               int tokens) {
+  const auto fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)hq, (cuuint64_t)n};
+  const cuuint64_t strides[2] = {(cuuint64_t)(hq > 1 ? head : d) * 2, (cuuint64_t)(n > 1 ? tok : d) * 2};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)group, (cuuint32_t)tokens};
+  const cuuint32_t step[3] = {1, 1, 1};
+  return fn(map, dtype == OSCAR_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(q), dims, strides, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // dynamic shared memory above 48 KB has to be asked for once per kernel and device
 template <auto Kernel>
 void allow_smem(size_t bytes) {
@@ -240,15 +314,37 @@ void allow_smem(size_t bytes) {
 
 struct PagedCall {
   oscar::PagedArgs args;
-  CUtensorMap kmap, vmap;
+  CUtensorMap qmap, kmap, vmap;
   const void* k_cache;
   int64_t kcb, kct, kch;
   int64_t n;
   cudaStream_t stream;
 };
 
+template <int D, typename T>
+int launch_mass_rows(const PagedCall& c, int num_req, const int* req_id, const int* q_start, const int* q_len,
+                     const int* seq) {
+  oscar::PagedPlan keys;
+  keys.num_req = num_req;
+  int64_t tiles = 0;
+  for (int i = 0; i < num_req; ++i) {
+    keys.req_id[i] = req_id[i];
+    keys.q_start[i] = q_start[i];
+    keys.q_len[i] = q_len[i];
+    keys.seq[i] = seq[i];
+    keys.tile_begin[i] = tiles;
+    tiles += ((int64_t)seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys;
+  }
+  keys.tile_begin[num_req] = tiles;
+  if (tiles == 0) return OSCAR_OK;
+  launch_pdl(oscar::paged_mass_rows_kernel<D, T>, dim3((unsigned)tiles, (unsigned)c.args.hk), dim3(32 * oscar::kPgWarps),
+             (size_t)oscar::kPgKeys * D * 2, c.stream, c.args, keys, reinterpret_cast<const T*>(c.k_cache), c.kcb, c.kct,
+             c.kch);
+  return cuda_status("paged_mass_rows_kernel");
+}
+
 template <int D, typename T, int NRT>
-int launch_split(const PagedCall& c, const PagedBatch& b, bool few) {
+int launch_split(const PagedCall& c, const PagedBatch& b) {
   const oscar::PagedArgs& a = c.args;
   const oscar::PagedPlan& p = b.plan;
   constexpr size_t smem = sizeof(oscar::PagedSmem<D, NRT>);
@@ -273,33 +369,44 @@ int launch_split(const PagedCall& c, const PagedBatch& b, bool few) {
     if (st) return st;
   }
   if (a.weights == nullptr) return OSCAR_OK;
-  if (few) {
+  if (b.cls == kFew) {
     launch_pdl(oscar::paged_mass_kernel<16 * NRT>, dim3((unsigned)p.total_tiles), dim3(oscar::kPgKeys), 0, c.stream, a, p);
     return cuda_status("paged_mass_kernel");
   }
-  oscar::PagedPlan keys = p;
-  int64_t tiles = 0;
-  for (int i = 0; i < p.num_req; ++i) {
-    keys.tile_begin[i] = tiles;
-    tiles += ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys;
-  }
-  keys.tile_begin[p.num_req] = tiles;
-  if (tiles == 0) return OSCAR_OK;
-  launch_pdl(oscar::paged_mass_rows_kernel<D, T>, dim3((unsigned)tiles, (unsigned)a.hk), dim3(32 * oscar::kPgWarps),
-             (size_t)oscar::kPgKeys * D * 2, c.stream, a, keys, reinterpret_cast<const T*>(c.k_cache), c.kcb, c.kct, c.kch);
-  return cuda_status("paged_mass_rows_kernel");
+  return launch_mass_rows<D, T>(c, p.num_req, p.req_id, p.q_start, p.q_len, p.seq);
 }
 
 template <int D, typename T>
-int launch_paged(const PagedCall& c, const PagedBatch& b, bool few) {
-  return b.rows <= 16 ? launch_split<D, T, 1>(c, b, few) : launch_split<D, T, 2>(c, b, few);
+int launch_chunk(const PagedCall& c, const PagedBatch& b) {
+  const oscar::PagedArgs& a = c.args;
+  const oscar::PcPlan& p = b.chunk;
+  constexpr size_t smem = sizeof(oscar::PcSmem<D>);
+  static_assert(smem <= 227 * 1024, "PcSmem exceeds the shared memory of a CTA");
+  allow_smem<oscar::paged_chunk_kernel<D, T>>(smem);
+  launch_pdl(oscar::paged_chunk_kernel<D, T>, dim3(p.ctas), dim3(oscar::PcShape<D>::kThreads), smem, c.stream, a, p,
+             c.qmap, c.kmap, c.vmap);
+  int st = cuda_status("paged_chunk_kernel");
+  if (st) return st;
+  if (b.splits.n > 0) {
+    launch_pdl(oscar::paged_chunk_combine_kernel<D, T>, dim3((unsigned)(b.splits.n * oscar::PcShape<D>::kM * oscar::kPcRows / 4)),
+               dim3(128), 0, c.stream, a, p, b.splits);
+    st = cuda_status("paged_chunk_combine_kernel");
+    if (st) return st;
+  }
+  return a.weights == nullptr ? OSCAR_OK : launch_mass_rows<D, T>(c, p.num_req, p.req_id, p.q_start, p.q_len, p.seq);
+}
+
+template <int D, typename T>
+int launch_paged(const PagedCall& c, const PagedBatch& b) {
+  if (b.cls == kChunk) return launch_chunk<D, T>(c, b);
+  return b.rows <= 16 ? launch_split<D, T, 1>(c, b) : launch_split<D, T, 2>(c, b);
 }
 
 template <typename T>
-int launch_paged_d(int d, const PagedCall& c, const PagedBatch& b, bool few) {
-  if (d == 256) return launch_paged<256, T>(c, b, few);
-  if (d == 128) return launch_paged<128, T>(c, b, few);
-  return launch_paged<64, T>(c, b, few);
+int launch_paged_d(int d, const PagedCall& c, const PagedBatch& b) {
+  if (d == 256) return launch_paged<256, T>(c, b);
+  if (d == 128) return launch_paged<128, T>(c, b);
+  return launch_paged<64, T>(c, b);
 }
 
 }  // namespace
@@ -314,11 +421,12 @@ int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs,
     return -1;
   int64_t need = 0;
   PagedBatch b;
-  for (int few = 0; few < 2; ++few)
+  for (int cls = 0; cls < kClasses; ++cls)
     for (int r = 0; r < num_requests;) {
-      r = paged_batch(b, r, few, qsl, seqs, num_requests, num_q_heads / num_kv_heads, num_kv_heads, device_info().sms);
-      if (b.plan.num_req > 0)
-        need = std::max(need, paged_space(b, few, qsl[num_requests], num_q_heads, head_dim, weighted != 0).total());
+      r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
+                      device_info().sms);
+      if (b.num() > 0)
+        need = std::max(need, paged_space(b, qsl[num_requests], num_q_heads, head_dim, weighted != 0).total());
     }
   return need;
 }
@@ -382,11 +490,14 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
       !paged_map(&c.vmap, vb, dtype, nb, block_size, num_kv_heads, head_dim, v_stride_block, v_stride_token, v_stride_head, a.box))
     return fail(OSCAR_ERR_INVALID, "paged_attention: the caches' strides do not fit a tensor map");
   PagedBatch b;
-  for (int few = 0; few < 2; ++few)
+  for (int cls = 0; cls < kClasses; ++cls)
     for (int r = 0; r < num_requests;) {
-      r = paged_batch(b, r, few, qsl, seqs, num_requests, a.group, num_kv_heads, device_info().sms);
-      if (b.plan.num_req == 0) continue;
-      const PagedSpace space = paged_space(b, few, n_tokens, num_q_heads, head_dim, weights != nullptr);
+      r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, a.group, num_kv_heads, head_dim, device_info().sms);
+      if (b.num() == 0) continue;
+      if (cls == kChunk && !query_map(&c.qmap, q, dtype, n_tokens, num_q_heads, head_dim, q_token_stride, q_head_stride,
+                                      a.group, b.chunk.tokens))
+        return fail(OSCAR_ERR_INVALID, "paged_attention: the queries' strides do not fit a tensor map");
+      const PagedSpace space = paged_space(b, n_tokens, num_q_heads, head_dim, weights != nullptr);
       if (workspace_bytes < space.total() || !workspace)
         return fail(OSCAR_ERR_INVALID, "paged_attention: workspace of %lld bytes, %lld needed", (long long)workspace_bytes,
                     (long long)space.total());
@@ -395,8 +506,8 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
       a.part_ml = reinterpret_cast<float2*>(at + space.stats);
       a.part_o = reinterpret_cast<float*>(at + space.stats + space.part_ml);
       a.scores = space.scores ? reinterpret_cast<float*>(at + space.stats + space.part_ml + space.part_o) : nullptr;
-      st = dtype == OSCAR_DTYPE_BF16 ? launch_paged_d<__nv_bfloat16>(head_dim, c, b, few)
-                                     : launch_paged_d<__half>(head_dim, c, b, few);
+      st = dtype == OSCAR_DTYPE_BF16 ? launch_paged_d<__nv_bfloat16>(head_dim, c, b)
+                                     : launch_paged_d<__half>(head_dim, c, b);
       if (st) return st;
     }
   return OSCAR_OK;
