@@ -48,6 +48,15 @@ struct PagedPlan {
   int64_t tile_begin[kPgReqs + 1];
 };
 
+// Division by the page size without a divide (it sits in the producers' serial path, where
+// one costs 150 cycles): q = (mulhi(mul, n) + n) >> shift for n < 2^31, with
+// shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  OSCAR_DEVINL uint32_t div(uint32_t n) const { return (__umulhi(mul, n) + n) >> shift; }
+  OSCAR_DEVINL uint32_t mod(uint32_t n) const { return n - div(n) * d; }
+};
+
 struct PagedArgs {
   const void* q;
   int64_t q_tok, q_head;  // strides in elements
@@ -57,6 +66,7 @@ struct PagedArgs {
   int hq, hk, group;
   int64_t num_blocks;
   int bs;
+  FastDiv page;           // by bs
   int box;                // tokens per TMA box: a power of two that divides the page, at most 64
   const int32_t* table;
   int64_t table_stride;
@@ -149,7 +159,8 @@ OSCAR_DEVINL bool pg_wait(int& abort, uint32_t bar, uint32_t parity) {
 }
 
 // Producer: one warp.  Lane i holds the block of box (base + i) of the unit, the
-// next 32 boxes' blocks are fetched one group ahead; lane 0 issues.
+// next 32 boxes' blocks are fetched one group ahead; one elected lane issues (lanes
+// with operands of their own would be serialised).
 template <int D, int ROWS, typename Smem>
 OSCAR_DEVINL void pg_produce(Smem& sm, const PagedArgs& a, const PagedPlan& p, const CUtensorMap* kmap,
                              const CUtensorMap* vmap, int64_t g0, int64_t g1, int lane) {
@@ -162,17 +173,15 @@ OSCAR_DEVINL void pg_produce(Smem& sm, const PagedArgs& a, const PagedPlan& p, c
     const int64_t stop = u.end < g1 ? u.end : g1;
     const int32_t* row = a.table + (int64_t)p.req_id[u.r] * a.table_stride;
     const int boxes = (u.seq + a.box - 1) / a.box;  // of the whole request
-    auto fetch = [&](int64_t b) -> int {
-      if (b >= boxes) return -1;
-      return row[(b * a.box) / a.bs];
-    };
-    int64_t base = (g - u.begin) * per;
+    const uint32_t box = (uint32_t)a.box;
+    auto fetch = [&](int b) -> int { return b < boxes ? row[a.page.div((uint32_t)b * box)] : -1; };
+    int base = (int)(g - u.begin) * per;
     int cur = fetch(base + lane), nxt = fetch(base + 32 + lane);
     for (; g < stop; ++g, ++it) {
       const int st = it % kSt;
       const uint32_t phase = (it / kSt) & 1;
-      const int64_t first = (g - u.begin) * per;  // first box of the tile
-      const int live = (int)max((int64_t)0, min((int64_t)per, boxes - first));
+      const int first = (int)(g - u.begin) * per;  // first box of the tile
+      const int live = max(0, min(per, boxes - first));
       const uint32_t bytes = (uint32_t)live * box_bytes * kPanels;
       const uint32_t fk = smem_u32(&sm.full_k[st]), fv = smem_u32(&sm.full_v[st]);
       if (it >= kSt) {
@@ -189,26 +198,26 @@ OSCAR_DEVINL void pg_produce(Smem& sm, const PagedArgs& a, const PagedPlan& p, c
       }
       __syncwarp();
       for (int j = 0; j < live; ++j) {
-        const int64_t b = first + j;
+        const int b = first + j;
         if (b - base >= 32) {
           base += 32;
           cur = nxt;
           nxt = fetch(base + 32 + lane);
         }
-        int blk = __shfl_sync(0xffffffffu, cur, (int)(b - base));
+        int blk = __shfl_sync(0xffffffffu, cur, b - base);
         if (blk < 0 || blk >= a.num_blocks) {
           if (lane == 0) flag_error(2u);
           blk = (int)a.num_blocks;  // outside the map: the box is filled with zeros
         }
-        const int off = (int)((b * a.box) % a.bs);
-        // lanes 0 .. 2 * panels - 1 issue one box each: K panels, then V panels
-        if (lane < 2 * kPanels) {
-          const int pn = lane % kPanels;
-          const uint32_t at = (uint32_t)pn * (kPgKeys * 128u) + (uint32_t)j * box_bytes;
-          if (lane < kPanels)
-            tma_load_4d(smem_u32(sm.k[st]) + at, kmap, pn * 64, u.h, off, blk, fk);
-          else
-            tma_load_4d(smem_u32(sm.v[st]) + at, vmap, pn * 64, u.h, off, blk, fv);
+        const int off = (int)a.page.mod((uint32_t)b * box);
+        if (tc::elect_one()) {
+          const uint32_t at = (uint32_t)j * box_bytes;
+#pragma unroll
+          for (int pn = 0; pn < kPanels; ++pn)
+            tma_load_4d(smem_u32(sm.k[st]) + pn * (kPgKeys * 128u) + at, kmap, pn * 64, u.h, off, blk, fk);
+#pragma unroll
+          for (int pn = 0; pn < kPanels; ++pn)
+            tma_load_4d(smem_u32(sm.v[st]) + pn * (kPgKeys * 128u) + at, vmap, pn * 64, u.h, off, blk, fv);
         }
       }
     }
@@ -577,9 +586,9 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
     const int key = i / (D / 8), c = i % (D / 8);
     uint4 v = make_uint4(0, 0, 0, 0);
     if (key0 + key < seq) {
-      const int64_t blk = row[(key0 + key) / a.bs];
+      const int64_t blk = row[a.page.div(key0 + key)];
       if (blk >= 0 && blk < a.num_blocks)
-        v = *reinterpret_cast<const uint4*>(k_cache + blk * kcb + (int64_t)((key0 + key) % a.bs) * kct + h * kch + 8 * c);
+        v = *reinterpret_cast<const uint4*>(k_cache + blk * kcb + (int64_t)a.page.mod(key0 + key) * kct + h * kch + 8 * c);
     }
     *reinterpret_cast<uint4*>(pg_raw + (c / 8) * (kPgKeys * 128) + pg_swz(key, c % 8)) = v;
   }
@@ -649,9 +658,9 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
   float total = 0.0f;
 #pragma unroll
   for (int w = 0; w < kPgWarps; ++w) total += part[w][tid];
-  const int64_t blk = row[key / a.bs];
+  const int64_t blk = row[a.page.div(key)];
   if (blk < 0 || blk >= a.num_blocks) return;  // flagged by the attention pass
-  float* w = a.weights + (blk * a.hk + h) * a.bs + key % a.bs;
+  float* w = a.weights + (blk * a.hk + h) * a.bs + a.page.mod(key);
   if (key < seq - q_len)
     atomicAdd(w, total);
   else
@@ -680,9 +689,9 @@ __global__ void __launch_bounds__(kPgKeys) paged_mass_kernel(const __grid_consta
   float sum = 0.0f;
   const float* s = a.scores + g * ROWS * kPgKeys + threadIdx.x;
   for (int i = first * a.group; i < u.nrows; ++i) sum = fmaf(pg_exp2(s[i * kPgKeys] - st[i].x), st[i].y, sum);
-  const int64_t blk = a.table[(int64_t)p.req_id[u.r] * a.table_stride + key / a.bs];
+  const int64_t blk = a.table[(int64_t)p.req_id[u.r] * a.table_stride + a.page.div(key)];
   if (blk < 0 || blk >= a.num_blocks) return;  // flagged by the attention pass
-  float* w = a.weights + (blk * a.hk + u.h) * a.bs + key % a.bs;
+  float* w = a.weights + (blk * a.hk + u.h) * a.bs + a.page.mod(key);
   if (key < u.seq - u.q_len)
     atomicAdd(w, sum);  // requests may share a page of history
   else

@@ -269,6 +269,12 @@ int check_paged(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, i
   return OSCAR_OK;
 }
 
+oscar::FastDiv fast_div(uint32_t d) {
+  uint32_t shift = 0;
+  while (((uint64_t)1 << shift) < d) ++shift;
+  return oscar::FastDiv{d, (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1), shift};
+}
+
 // The cache as a 4D map (dims, heads, tokens of a page, pages) in boxes of 64 dims x `box` tokens.
 bool paged_map(CUtensorMap* map, const void* base, int dtype, int64_t num_blocks, int bs, int hk, int d, int64_t sb,
                int64_t st, int64_t sh, int box) {
@@ -474,6 +480,7 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.out = out, a.lse = lse;
   a.hq = num_q_heads, a.hk = num_kv_heads, a.group = num_q_heads / num_kv_heads;
   a.num_blocks = num_blocks, a.bs = block_size;
+  a.page = fast_div((uint32_t)block_size);
   a.box = std::min(oscar::kPgKeys, block_size & -block_size);
   a.table = block_table, a.table_stride = bt_stride;
   a.scale_log2 = scale * 1.4426950408889634f;

@@ -24,8 +24,9 @@
 //   O += P V  : A = P in tensor memory, B = V, MN-major, 128-byte swizzle.
 // The running maximum moves only when a score exceeds it by kPgHeadroom (log2
 // units); then the thread rescales its row of O in tensor memory.
-// Warps: 4 kM softmax, one MMA issuer, one TMA producer (ring of slots in the
-// order the MMAs use them; boxes of 64 dims x a power-of-two of tokens).
+// Warps: 4 kM softmax, one MMA issuer, two TMA producers (K and Q; V) that fill one
+// ring of slots in the order the MMAs use them, in boxes of 64 dims x a power of
+// two of tokens.
 // Every wait is bounded; a time-out sets the CTA's abort flag and drains.
 #pragma once
 
@@ -64,7 +65,7 @@ struct PcShape {
   static constexpr int kSlot = kPcKeys * D * 2 / kHalves;
   static constexpr int kSlots = D == 64 ? 8 : 5;
   static constexpr int kSoftWarps = 4 * kM;
-  static constexpr int kThreads = 32 * (kSoftWarps + 2);
+  static constexpr int kThreads = 32 * (kSoftWarps + 3);
 };
 
 template <int D>
@@ -159,6 +160,12 @@ OSCAR_DEVINL uint64_t f2_add(uint64_t a, uint64_t b) {
 OSCAR_DEVINL float f2_lo(uint64_t a) { return __uint_as_float((uint32_t)a); }
 OSCAR_DEVINL float f2_hi(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
 
+OSCAR_DEVINL float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 template <typename T> OSCAR_DEVINL uint32_t pc_pack(float lo, float hi);
 template <> OSCAR_DEVINL uint32_t pc_pack<__nv_bfloat16>(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
@@ -239,22 +246,26 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const uint32_t s_col = tmem + lanes + 128 * b;
         if (!wait(smem_u32(&sm.s_full[b]), (job >> 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc::tmem_ld32(s_col + 32 * c, s + 32 * c);
-        tc::tmem_wait_ld();
+        // Two passes over the scores in chunks of 32 columns, each a short loop: unrolled over
+        // the row, the warps of the CTA run out of the instruction cache (see below)
         const int vis = lim - t * kPcKeys;  // keys c < vis are visible
-        if (__any_sync(0xffffffffu, vis < kPcKeys)) {
-#pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= vis) s[c] = 0xff800000u;
-        }
+        const bool masked = __any_sync(0xffffffffu, vis < kPcKeys);
+        uint32_t s[32];
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPcKeys; c0 += 32) {
+          tc::tmem_ld32(s_col + c0, s);
+          tc::tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-        for (int c = 0; c < 128; c += 8)
+            for (int c = 0; c < 32; ++c) s[c] = c0 + c < vis ? s[c] : 0xff800000u;
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            m4[i] = fmaxf(m4[i], fmaxf(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])));
+          for (int c = 0; c < 32; c += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
+        }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
         const bool grow = mx > m + kPgHeadroom;
         const bool rescale = grow && m != -INFINITY;
@@ -278,17 +289,24 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
         const float base = m == -INFINITY ? 0.0f : -m;
         const uint64_t scale2 = f2_pack(scale, scale), base2 = f2_pack(base, base);
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPcKeys; c0 += 32) {
+          // (the columns P overwrites, [c0 / 2, c0 / 2 + 16), have been read)
+          tc::tmem_ld32(s_col + c0, s);
+          tc::tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-        for (int c = 0; c < 128; c += 64) {
-          uint32_t pk[32];
+            for (int c = 0; c < 32; ++c) s[c] = c0 + c < vis ? s[c] : 0xff800000u;
+          }
+          uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, base2);
             const float e0 = pg_exp2(f2_lo(x)), e1 = pg_exp2(f2_hi(x));
             l2 = f2_add(l2, f2_pack(e0, e1));
             pk[i] = pc_pack<T>(e0, e1);
           }
-          tc::tmem_st32(s_col + c / 2, pk);
+          tc::tmem_st16(s_col + c0 / 2, pk);
         }
         const int have = seq - t * kPcKeys;
         if (have < kPcKeys) {
@@ -371,67 +389,19 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     const uint64_t dk = pc_desc(smem_u32(sm.ring), 16, 1024);
     const uint64_t dv = pc_desc(smem_u32(sm.ring), (kPcKeys / kHalves) * 128, 1024);
     constexpr uint64_t kSlotStep = Shape::kSlot >> 4;
-    bool ok = true;
-    int unit = 0;
-    // jobs [0, n) of the CTA; S runs two jobs ahead of O and may belong to the next unit
-    PcWalk<D> ws = w;                 // unit of the next S
-    int js = 0, jo = 0;               // next S and O jobs
-    int s_left = w.live() ? (w.t_end - w.t) * kM : 0;  // S jobs left in ws's unit
-    bool s_open = false;              // ws's Q has been waited for
-    auto issue_s = [&]() -> bool {
-      if (!ws.live()) return true;
-      if (!s_open) {
-        if (!wait(smem_u32(&sm.q_full), unit & 1)) return false;
-        s_open = true;
-      }
-      const int tile = kM == 2 ? js >> 1 : js;
-      const int mt = kM == 2 ? js & 1 : 0;
-      if (mt == 0) {
-#pragma unroll
-        for (int hf = 0; hf < kHalves; ++hf) {
-          const int at = pc_k_at<D>(tile, hf);
-          if (!wait(full(at % kSlots), (at / kSlots) & 1)) return false;
-        }
-      }
-      tc::tc_fence_after();
-      const bool last = --s_left == 0;
-      if (tc::elect_one()) {
-#pragma unroll
-        for (int pn = 0; pn < kPanels; ++pn) {
-          const int at = pc_k_at<D>(tile, pn * kHalves / kPanels);
-          const uint64_t qd = dq + (uint64_t)((mt * kPanels + pn) * (kPcRows * 128 >> 4));
-          const uint64_t kd = dk + (uint64_t)(at % kSlots) * kSlotStep +
-                              (uint64_t)((pn % (kPanels / kHalves)) * (kPcKeys * 128 >> 4));
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            tc::mma_ss(tmem + 128 * (js & 1), qd + 2 * ks, kd + 2 * ks, idesc_s, pn + ks > 0 ? 1u : 0u);
-        }
-        tc::mma_commit(smem_u32(&sm.s_full[js & 1]));
-        if (mt == kM - 1) {
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) tc::mma_commit(empty(pc_k_at<D>(tile, hf) % kSlots));
-        }
-        if (last) tc::mma_commit(smem_u32(&sm.q_empty));
-      }
-      __syncwarp();
-      ++js;
-      if (last) {
-        ws.next(a.hk);
-        ++unit;
-        s_open = false;
-        s_left = ws.live() ? (ws.t_end - ws.t) * kM : 0;
-      }
-      return true;
-    };
-    ok = issue_s();
-    ok = ok && issue_s();
-    for (; w.live() && ok; w.next(a.hk)) {
-      const int jobs = (w.t_end - w.t) * kM;
+    // S runs two jobs ahead of O and may belong to the next unit
+    PcWalk<D> ws = w;                            // unit of the next S
+    int unit = 0;                                // its number
+    int s_left = (ws.t_end - ws.t) * kM, o_left = s_left;  // jobs left in the units of the next S and O
+    bool s_open = false, o_open = false;         // the unit's Q has been waited for; O holds a product of the unit
+    const int jobs = n_tiles * kM;
 #pragma unroll 1
-      for (int i = 0; i < jobs; ++i, ++jo) {
+    for (int step = 0; step < jobs + 2; ++step) {
+      const int jo = step - 2, js = step;
+      if (jo >= 0) {
         const int tile = kM == 2 ? jo >> 1 : jo;
         const int mt = kM == 2 ? jo & 1 : 0;
-        if (!wait(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) { ok = false; break; }
+        if (!wait(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
         bool there = true;
         if (mt == 0) {
 #pragma unroll
@@ -440,7 +410,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
             there = there && wait(full(at % kSlots), (at / kSlots) & 1);
           }
         }
-        if (!there) { ok = false; break; }
+        if (!there) break;
         tc::tc_fence_after();
         if (tc::elect_one()) {
           constexpr int kStepsPerSlot = kPcKeys / kHalves / 16;
@@ -448,16 +418,58 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
           for (int ks = 0; ks < kPcKeys / 16; ++ks) {
             const int at = pc_v_at<D>(tile, ks / kStepsPerSlot, n_tiles);
             const uint64_t vd = dv + (uint64_t)(at % kSlots) * kSlotStep + (uint64_t)((ks % kStepsPerSlot) * (2048 >> 4));
-            tc::mma_ts(tmem + kColO + 128 * mt, tmem + 128 * (jo & 1) + 8 * ks, vd, idesc_o, (i >= kM || ks > 0) ? 1u : 0u);
-          }
-          if (mt == kM - 1) {
-#pragma unroll
-            for (int hf = 0; hf < kHalves; ++hf) tc::mma_commit(empty(pc_v_at<D>(tile, hf, n_tiles) % kSlots));
+            tc::mma_ts(tmem + kColO + 128 * mt, tmem + 128 * (jo & 1) + 8 * ks, vd, idesc_o, (o_open || ks > 0) ? 1u : 0u);
+            if (mt == kM - 1 && (ks + 1) % kStepsPerSlot == 0) tc::mma_commit(empty(at % kSlots));
           }
           tc::mma_commit(smem_u32(&sm.o_done[jo & 1]));
         }
         __syncwarp();
-        if (!issue_s()) { ok = false; break; }
+        if (mt == kM - 1) o_open = true;
+        if (--o_left == 0) {
+          w.next(a.hk);
+          o_open = false;
+          o_left = w.live() ? (w.t_end - w.t) * kM : 0;
+        }
+      }
+      if (js < jobs) {
+        if (!s_open && !wait(smem_u32(&sm.q_full), unit & 1)) break;
+        s_open = true;
+        const int tile = kM == 2 ? js >> 1 : js;
+        const int mt = kM == 2 ? js & 1 : 0;
+        bool there = true;
+        if (mt == 0) {
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf) {
+            const int at = pc_k_at<D>(tile, hf);
+            there = there && wait(full(at % kSlots), (at / kSlots) & 1);
+          }
+        }
+        if (!there) break;
+        tc::tc_fence_after();
+        const bool last = --s_left == 0;
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int pn = 0; pn < kPanels; ++pn) {
+            const int at = pc_k_at<D>(tile, pn * kHalves / kPanels);
+            const uint64_t qd = dq + (uint64_t)((mt * kPanels + pn) * (kPcRows * 128 >> 4));
+            const uint64_t kd = dk + (uint64_t)(at % kSlots) * kSlotStep +
+                                (uint64_t)((pn % (kPanels / kHalves)) * (kPcKeys * 128 >> 4));
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc::mma_ss(tmem + 128 * (js & 1), qd + 2 * ks, kd + 2 * ks, idesc_s, pn + ks > 0 ? 1u : 0u);
+            // a slot is released as soon as its last product is issued
+            if (mt == kM - 1 && (pn + 1) % (kPanels / kHalves) == 0) tc::mma_commit(empty(at % kSlots));
+          }
+          tc::mma_commit(smem_u32(&sm.s_full[js & 1]));
+          if (last) tc::mma_commit(smem_u32(&sm.q_empty));
+        }
+        __syncwarp();
+        if (last) {
+          ws.next(a.hk);
+          ++unit;
+          s_open = false;
+          s_left = ws.live() ? (ws.t_end - ws.t) * kM : 0;
+        }
       }
     }
     // no MMA may be in flight when the tensor memory is freed
@@ -465,104 +477,103 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     __syncwarp();
     if (!tc::mbar_wait(smem_u32(&sm.end), 0) && lane == 0) flag_error(16u);
   } else {
-    // ================= producer: slots in the order the MMAs use them
+    // ================= producers: one warp fetches K (and Q), one V, each in the order of use.
+    // Lane i holds the pages of boxes i, i + 32, .. of the next tile, looked up while the tile
+    // before it is issued; one elected lane issues (operands uniform over the warp)
+    const bool is_k = warp == kMma + 1;
+    const CUtensorMap* map = is_k ? &kmap : &vmap;
     const int per = kPcKeys / a.box;  // boxes per tile
-    const uint32_t box_bytes = (uint32_t)a.box * 128u;
-    int at = 0, unit = 0;  // next slot, next unit
-    bool ok = true;
-    // the K tile after the current one is fetched before the current V (D 256: S runs two tiles ahead of O)
-    PcWalk<D> wk = w, wv = w;
-    struct Stream {  // tiles of one of K / V over the CTA's pieces
-      int t;
-      bool open;
-    } sk{0, false}, sv{0, false};
-    const int32_t* krow = nullptr;
-    int kboxes = 0, vboxes = 0;
-    const int32_t* vrow = nullptr;
-    auto acquire = [&](int n) -> bool {
-      return n < kSlots || wait(empty(n % kSlots), ((n / kSlots) - 1) & 1);
+    const uint32_t box = (uint32_t)a.box, box_bytes = box * 128u;
+    const int32_t* row = nullptr;
+    int boxes = 0, unit = 0, t = 0, last_at = -1;
+    int blk[kPcKeys / 32];
+    auto look_up = [&] {
+#pragma unroll
+      for (int i = 0; i < kPcKeys / 32; ++i) {
+        if (32 * i >= per) break;
+        const int j = lane + 32 * i, b = t * per + j;
+        blk[i] = j < per && b < boxes ? row[a.page.div((uint32_t)b * box)] : 0;
+      }
     };
-    auto load = [&](bool is_k) -> bool {
-      PcWalk<D>& x = is_k ? wk : wv;
-      Stream& s = is_k ? sk : sv;
-      if (!x.live()) return true;
-      if (!s.open) {
-        s.open = true;
-        s.t = x.t;
-        (is_k ? krow : vrow) = a.table + (int64_t)p.req_id[x.r] * a.table_stride;
-        (is_k ? kboxes : vboxes) = (p.seq[x.r] + a.box - 1) / a.box;
+    bool ok = true, open = false;
+#pragma unroll 1
+    for (int tile = 0; tile < n_tiles && ok; ++tile) {
+      if (!open) {  // a new piece, with its queries
+        t = w.t;
+        row = a.table + (int64_t)p.req_id[w.r] * a.table_stride;
+        boxes = (p.seq[w.r] + a.box - 1) / a.box;
+        look_up();
+        open = true;
         if (is_k) {
-          if (unit > 0 && !wait(smem_u32(&sm.q_empty), (unit - 1) & 1)) return false;
-          if (lane == 0) {
+          if (unit > 0 && !wait(smem_u32(&sm.q_empty), (unit - 1) & 1)) break;
+          if (tc::elect_one()) {
             const uint32_t bar = smem_u32(&sm.q_full);
             tc::mbar_expect_tx(bar, (uint32_t)(kM * kPanels * p.tokens * a.group * 128));
-#pragma unroll
-            for (int mt = 0; mt < kM; ++mt)
-#pragma unroll
-              for (int pn = 0; pn < kPanels; ++pn)
-                tma_load_3d(smem_u32(sm.q[mt][pn]), &qmap, 64 * pn, x.h * a.group,
-                            p.q_start[x.r] + (x.qb * kM + mt) * p.tokens, bar);
+#pragma unroll 1
+            for (int i = 0; i < kM * kPanels; ++i)
+              tma_load_3d(smem_u32(sm.q) + i * kPcRows * 128, &qmap, 64 * (i % kPanels), w.h * a.group,
+                          p.q_start[w.r] + (w.qb * kM + i / kPanels) * p.tokens, bar);
           }
           __syncwarp();
           ++unit;
         }
       }
-      const int first = s.t * per, boxes = is_k ? kboxes : vboxes;
-      const int32_t* trow = is_k ? krow : vrow;
-      const CUtensorMap* map = is_k ? &kmap : &vmap;
-      // a lane looks up the pages of boxes lane, lane + 32, ... of the tile
-      int blk[4];
+      const int first = t * per, h = w.h, here = min(per, max(0, boxes - first));
+      int cur[kPcKeys / 32];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = lane + 32 * i;
-        blk[i] = 0;
-        if (j < per && first + j < boxes) {
-          blk[i] = trow[((int64_t)(first + j) * a.box) / a.bs];
-          if (blk[i] < 0 || blk[i] >= a.num_blocks) {
-            flag_error(2u);
-            blk[i] = (int)a.num_blocks;  // outside the map: zeros
-          }
+      for (int i = 0; i < kPcKeys / 32; ++i) {
+        cur[i] = blk[i];
+        if (lane + 32 * i < here && (cur[i] < 0 || cur[i] >= a.num_blocks)) {
+          flag_error(2u);
+          cur[i] = (int)a.num_blocks;  // outside the map: zeros
         }
       }
-#pragma unroll
-      for (int hf = 0; hf < kHalves; ++hf, ++at) {
-        if (!acquire(at)) return false;
-        const int slot = at % kSlots;
+      if (++t < w.t_end) {
+        look_up();
+      } else {
+        w.next(a.hk);
+        open = false;
+      }
+#pragma unroll 1
+      for (int hf = 0; hf < kHalves; ++hf) {
+        const int at = is_k ? pc_k_at<D>(tile, hf) : pc_v_at<D>(tile, hf, n_tiles), slot = at % kSlots;
         // K: panels [hf * kPanels / kHalves, ..), all boxes; V: all panels, boxes of this key half
         const int pan0 = is_k ? hf * (kPanels / kHalves) : 0, pans = is_k ? kPanels / kHalves : kPanels;
         const int box0 = is_k ? 0 : hf * (per / kHalves), nbox = is_k ? per : per / kHalves;
-        const int live = max(0, min(nbox, boxes - first - box0));
-        if (lane == 0) tc::mbar_expect_tx(full(slot), (uint32_t)(live * pans) * box_bytes);
-        __syncwarp();
+        const int live = max(0, min(nbox, here - box0));
         const uint32_t panel = (uint32_t)nbox * box_bytes;  // bytes of a panel of the slot
-        for (int i = 0; i < live * pans; i += 32) {
-          const int id = i + lane, j = box0 + (id % max(live, 1)), pn = id / max(live, 1);
+        if (at >= kSlots && !wait(empty(slot), ((at / kSlots) - 1) & 1)) { ok = false; break; }
+        last_at = at;
+        if (tc::elect_one()) tc::mbar_expect_tx(full(slot), (uint32_t)(live * pans) * box_bytes);
+        __syncwarp();
+        const uint32_t dst = smem_u32(sm.ring[slot]);
+#pragma unroll 1
+        for (int i = 0; i < live; ++i) {
+          const int j = box0 + i;
           int b = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int v = __shfl_sync(0xffffffffu, blk[k], j & 31);
+          for (int k = 0; k < kPcKeys / 32; ++k) {
+            if (32 * k >= per) break;
+            const int v = __shfl_sync(0xffffffffu, cur[k], j & 31);
             if (j >> 5 == k) b = v;
           }
-          if (id < live * pans)
-            tma_load_4d(smem_u32(sm.ring[slot]) + pn * panel + (uint32_t)(j - box0) * box_bytes, map, 64 * (pan0 + pn), x.h,
-                        (int)(((int64_t)(first + j) * a.box) % a.bs), b, full(slot));
+          const int off = (int)a.page.mod((uint32_t)(first + j) * box);
+          if (tc::elect_one()) {
+#pragma unroll
+            for (int pn = 0; pn < kPanels; ++pn)
+              if (pn < pans)
+                tma_load_4d(dst + pn * panel + (uint32_t)i * box_bytes, map, 64 * (pan0 + pn), h, off, b, full(slot));
+          }
         }
+        __syncwarp();
       }
-      if (++s.t == x.t_end) {
-        x.next(a.hk);
-        s.open = false;
-      }
-      return true;
-    };
-    ok = load(true);
-    if (kM == 1) ok = ok && load(true);
-    while (wv.live() && ok) {
-      ok = load(false);
-      ok = ok && load(true);
     }
-    // no copy may still be writing shared memory when the CTA ends
-    for (int i = max(0, at - kSlots); i < at; ++i) tc::mbar_wait(full(i % kSlots), (i / kSlots) & 1);
-    if (unit > 0) tc::mbar_wait(smem_u32(&sm.q_full), (unit - 1) & 1);
+    // no copy may still be writing shared memory when the CTA ends.  The MMA warp has waited for
+    // all of them unless a wait timed out
+    if (*reinterpret_cast<volatile int*>(&sm.abort) != 0) {
+      for (int n = max(0, last_at - kSlots + 1); n <= last_at; ++n) tc::mbar_wait(full(n % kSlots), (n / kSlots) & 1);
+      if (is_k && unit > 0) tc::mbar_wait(smem_u32(&sm.q_full), (unit - 1) & 1);
+    }
   }
 
   tc::tc_fence_before();
