@@ -30,6 +30,7 @@ using oscar_host::device_info;
 using oscar_host::encode_tiled;
 using oscar_host::fail;
 using oscar_host::launch_pdl;
+using oscar_host::launch_pdl_cluster;
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -181,12 +182,13 @@ struct PagedBatch {
 template <int D>
 void plan_chunk(PagedBatch& b, int hk, int sms) {
   oscar::PcPlan& p = b.chunk;
-  const int per = p.tokens * oscar::PcShape<D>::kM;
+  const int per = p.tokens * oscar::kPcUnit;
   int64_t total = 0;
   for (int i = 0; i < p.num_req; ++i)
     for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb)
-      total += (int64_t)hk * oscar::pc_tiles<D>(p.q_len[i], p.seq[i], p.tokens, qb);
-  p.ctas = (int)std::min<int64_t>(std::min(std::max(sms, 1), oscar::kPcCtas), total);
+      total += (int64_t)hk * oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb);
+  const int workers = oscar::PcShape<D>::kPair ? sms / 2 : sms;
+  p.ctas = (int)std::min<int64_t>(std::min(std::max(workers, 1), oscar::kPcCtas), total);
   b.splits.n = 0;
   int64_t at = 0;  // tiles before the unit
   int c = 0;       // CTAs begun
@@ -194,7 +196,7 @@ void plan_chunk(PagedBatch& b, int hk, int sms) {
   for (int i = 0; i < p.num_req; ++i)
     for (int h = 0; h < hk; ++h)
       for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb) {
-        const int nt = oscar::pc_tiles<D>(p.q_len[i], p.seq[i], p.tokens, qb);
+        const int nt = oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb);
         const bool at_start = c < p.ctas && start_of(c) == at;
         const int first = at_start ? c : c - 1;  // the CTA that holds the unit's first tile
         while (c < p.ctas && start_of(c) < at + nt) {
@@ -251,7 +253,7 @@ int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const
 PagedSpace paged_space(const PagedBatch& b, int64_t n, int hq, int d, bool weighted) {
   PagedSpace s{};
   if (weighted) s.stats = round256(n * hq * (int64_t)sizeof(float2));
-  const int64_t pieces = b.cls == kChunk ? (int64_t)2 * b.chunk.ctas * oscar::kPcRows * (d == 256 ? 1 : 2)
+  const int64_t pieces = b.cls == kChunk ? (int64_t)2 * b.chunk.ctas * oscar::kPcRows * oscar::kPcUnit
                                          : (int64_t)2 * b.plan.ctas * b.rows;
   s.part_ml = round256(pieces * (int64_t)sizeof(float2));
   s.part_o = round256(pieces * d * (int64_t)sizeof(float));
@@ -389,12 +391,13 @@ int launch_chunk(const PagedCall& c, const PagedBatch& b) {
   constexpr size_t smem = sizeof(oscar::PcSmem<D>);
   static_assert(smem <= 227 * 1024, "PcSmem exceeds the shared memory of a CTA");
   allow_smem<oscar::paged_chunk_kernel<D, T>>(smem);
-  launch_pdl(oscar::paged_chunk_kernel<D, T>, dim3(p.ctas), dim3(oscar::PcShape<D>::kThreads), smem, c.stream, a, p,
-             c.qmap, c.kmap, c.vmap);
+  constexpr bool pair = oscar::PcShape<D>::kPair;
+  launch_pdl_cluster(pair ? 2 : 1, oscar::paged_chunk_kernel<D, T>, dim3(pair ? 2 * p.ctas : p.ctas),
+                     dim3(oscar::PcShape<D>::kThreads), smem, c.stream, a, p, c.qmap, c.kmap, c.vmap);
   int st = cuda_status("paged_chunk_kernel");
   if (st) return st;
   if (b.splits.n > 0) {
-    launch_pdl(oscar::paged_chunk_combine_kernel<D, T>, dim3((unsigned)(b.splits.n * oscar::PcShape<D>::kM * oscar::kPcRows / 4)),
+    launch_pdl(oscar::paged_chunk_combine_kernel<D, T>, dim3((unsigned)(b.splits.n * oscar::kPcUnit * oscar::kPcRows / 4)),
                dim3(128), 0, c.stream, a, p, b.splits);
     st = cuda_status("paged_chunk_combine_kernel");
     if (st) return st;

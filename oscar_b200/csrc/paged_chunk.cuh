@@ -1,21 +1,26 @@
 // Attention of long chunks over a paged 16-bit cache on the 5th-generation
 // tensor cores (same function as paged.cuh; requests with many query rows).
 //
-// Work.  A unit is (request, kv head, q-block); a q-block is kM = 1 (D 256) or 2
-// (D 64, 128) tiles of 128 query rows, each holding floor(128 / group) tokens x
-// group heads.  Its visible keys are cut into 128-key tiles, and the tiles of
-// all units, in order, are divided evenly over the CTAs (one per SM) by the
-// host, so a CTA streams whole units except at its two ends; the pieces of a
-// divided unit are written unnormalised in fp32 and combined by a dependent
-// launch in CTA order.
+// Work.  A unit is (request, kv head, q-block); a q-block is two tiles of 128
+// query rows, each holding floor(128 / group) tokens x group heads.  Its visible
+// keys are cut into 128-key tiles, and the tiles of all units, in order, are
+// divided evenly over the workers by the host, so a worker streams whole units
+// except at its two ends; the pieces of a divided unit are written unnormalised
+// in fp32 and combined by a dependent launch in worker order.
 //
-// Tile.  Bound by the tensor pipe at D 256 (per 128 keys 16 + 8 MMAs of N 128
-// and N 256) and by the exponentials at D <= 128 (128 x 128 of them per MMA
-// tile at 16 per cycle and SM).  Jobs alternate between two score buffers:
-// D 256: job j is key tile j of the one row tile; D <= 128: key tile j / 2 of
-// row tile j % 2.  The MMA warp issues S(0), S(1), then per job O += P(j) V as
-// soon as P(j) is written and S(j + 2), so while the softmax of one job runs the
-// tensor pipe has the other job's products.
+// A worker is one CTA that holds both row tiles (D 64, 128), or a pair of CTAs
+// with one row tile each (D 256): the pair's products are issued once for 256
+// rows (cta_group::2), and each CTA fetches half of every K and V tile.  One CTA
+// alone would need 63 bytes per cycle of K and V to keep its tensor pipe busy,
+// and TMA brings an SM at most 46 (measured on resident data); it also leaves
+// room for 2.5 tiles of K and V instead of 1.25 beside the queries.
+//
+// Tile.  Bound by the tensor pipe at D 256 and by the exponentials at D <= 128
+// (128 x 128 per row tile at 16 per cycle and SM).  Jobs alternate between two
+// score buffers: D 256: job j is key tile j; D <= 128: key tile j / 2 of row tile
+// j % 2.  The MMA warp issues S(0), S(1), then per job O += P(j) V as soon as
+// P(j) is written and S(j + 2), so while the softmax of one job runs the tensor
+// pipe has the other job's products.
 //   TMEM columns: S[0] [0, 128), S[1] [128, 256), O [256, 512) (D 256) or
 //   O[0] [256, 256 + D), O[1] [384, 384 + D).  P(j) (16 bit) replaces the first
 //   64 columns of S(j) and is the A operand of P V; rows lie on lanes, one
@@ -24,10 +29,13 @@
 //   O += P V  : A = P in tensor memory, B = V, MN-major, 128-byte swizzle.
 // The running maximum moves only when a score exceeds it by kPgHeadroom (log2
 // units); then the thread rescales its row of O in tensor memory.
-// Warps: 4 kM softmax, one MMA issuer, two TMA producers (K and Q; V) that fill one
-// ring of slots in the order the MMAs use them, in boxes of 64 dims x a power of
-// two of tokens.
-// Every wait is bounded; a time-out sets the CTA's abort flag and drains.
+//
+// Warps: 4 or 8 softmax, one MMA issuer, two TMA producers (K and Q; V) that
+// fill one ring of slots in the order the MMAs use them, in boxes of 64 dims x a
+// power of two of tokens.  Each role is a short loop: unrolled over a row or a
+// tile they overran the instruction cache (4.0 against 2.85 ms for 8192 queries
+// on 17448 keys).  Every wait is bounded; a time-out sets the CTA's abort flag
+// and drains.
 #pragma once
 
 #include <climits>
@@ -38,19 +46,20 @@ namespace oscar {
 
 constexpr int kPcRows = 128;
 constexpr int kPcKeys = 128;
-constexpr int kPcCtas = 192;  // CTAs of a plan
+constexpr int kPcCtas = 192;   // workers of a plan
+constexpr int kPcUnit = 2;     // row tiles of a unit
 
 struct PcStart {
   int r, h, qb, t;  // plan index, kv head, q-block, first key tile
 };
 struct PcPlan {
-  int num_req, ctas, tokens;  // tokens per row tile
+  int num_req, ctas, tokens;  // workers; tokens per row tile
   int req_id[kPgReqs], q_start[kPgReqs], q_len[kPgReqs], seq[kPgReqs];
   PcStart start[kPcCtas];
-  int tiles[kPcCtas];  // key tiles of each CTA
+  int tiles[kPcCtas];  // key tiles of each worker
 };
 struct PcSplit {
-  int r, h, qb, c0, c1;  // a divided unit and its CTAs
+  int r, h, qb, c0, c1;  // a divided unit and its workers
 };
 struct PcSplits {
   int n;
@@ -59,10 +68,12 @@ struct PcSplits {
 
 template <int D>
 struct PcShape {
-  static constexpr int kM = D == 256 ? 1 : 2;           // row tiles per unit
-  static constexpr int kPanels = D / 64;
-  static constexpr int kHalves = D == 256 ? 2 : 1;      // slots per K or V tile
-  static constexpr int kSlot = kPcKeys * D * 2 / kHalves;
+  static constexpr bool kPair = D == 256;               // a worker is a pair of CTAs
+  static constexpr int kM = kPair ? 1 : 2;              // row tiles per CTA
+  static constexpr int kPanels = D / 64;                // 64-dim panels
+  static constexpr int kKeys = kPair ? 64 : kPcKeys;    // keys of a K tile in this CTA
+  static constexpr int kVPanels = kPair ? 2 : kPanels;  // panels of a V tile in this CTA
+  static constexpr int kSlot = kKeys * D * 2;           // a K tile or a V tile
   static constexpr int kSlots = D == 64 ? 8 : 5;
   static constexpr int kSoftWarps = 4 * kM;
   static constexpr int kThreads = 32 * (kSoftWarps + 3);
@@ -71,12 +82,11 @@ struct PcShape {
 template <int D>
 struct PcSmem {
   using S = PcShape<D>;
-  uint8_t q[S::kM][S::kPanels][kPcRows * 128];  // [row tile][64-dim panel][row][128 bytes], swizzled
-  // K tile: [panel][128 keys][128 bytes]; a slot holds half of the panels at D 256.
-  // V tile: the same; at D 256 a slot holds 64 keys: [panel][64 keys][128 bytes]
-  uint8_t ring[S::kSlots][S::kSlot];
+  uint8_t q[S::kM][S::kPanels][kPcRows * 128];  // [row tile][panel][row][128 bytes], swizzled
+  uint8_t ring[S::kSlots][S::kSlot];            // K: [panel][key][128 bytes]; V: [panel][128 keys][128 bytes]
+  // full, q_full, p_full: of a pair, the first CTA's are used by both
   unsigned long long full[S::kSlots], empty[S::kSlots];
-  unsigned long long q_full, q_empty, s_full[2], p_full[2], o_done[2], end;
+  unsigned long long q_full, q_empty, s_full[2], p_full[2], o_done[2], tail, end;
   uint32_t tmem;
   int abort;
 };
@@ -94,26 +104,115 @@ OSCAR_DEVINL void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y
 }
 
 // key tiles that q-block qb of a request sees (at least 1, so that empty rows are written)
-template <int D>
 __host__ __device__ inline int pc_tiles(int q_len, int seq, int tokens, int qb) {
-  const int last = (qb + 1) * tokens * PcShape<D>::kM;
+  const int last = (qb + 1) * tokens * kPcUnit;
   const int visible = seq - q_len + (last < q_len ? last : q_len);
   return visible > kPcKeys ? (visible + kPcKeys - 1) / kPcKeys : 1;
 }
 
-// Ring position of half hf of key tile t's K and V (n tiles in the CTA's stream).
-// D <= 128: K0 V0 K1 V1 ..; D 256: K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1), two slots each.
+// Ring position of key tile t's K and V (n tiles in the worker's stream).
+// D <= 128: K0 V0 K1 V1 ..; D 256 (S runs two tiles ahead of O): K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1).
 template <int D>
-OSCAR_DEVINL int pc_k_at(int t, int hf) {
-  return D == 256 ? 2 * (t == 0 ? 0 : 2 * t - 1) + hf : 2 * t;
+OSCAR_DEVINL int pc_k_at(int t) {
+  return D == 256 ? (t == 0 ? 0 : 2 * t - 1) : 2 * t;
 }
 template <int D>
-OSCAR_DEVINL int pc_v_at(int t, int hf, int n) {
-  return D == 256 ? 2 * (t == n - 1 ? 2 * n - 1 : 2 * t + 2) + hf : 2 * t + 1;
+OSCAR_DEVINL int pc_v_at(int t, int n) {
+  return D == 256 ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1;
 }
 
-// The pieces of units of one CTA, walked alike by every role.
-template <int D>
+// The two CTAs of a pair
+OSCAR_DEVINL uint32_t pc_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
+  return r;
+}
+OSCAR_DEVINL uint32_t pc_map(uint32_t addr, uint32_t rank) {  // the same shared address in CTA `rank` of the cluster
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+OSCAR_DEVINL void pc_cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+OSCAR_DEVINL void pc_arrive(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+}
+OSCAR_DEVINL void pc_expect(uint32_t cluster_addr, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;\n" ::"r"(cluster_addr),
+               "r"(bytes)
+               : "memory");
+}
+OSCAR_DEVINL bool pc_try_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
+      "p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+template <bool kPair>
+OSCAR_DEVINL void pc_commit(uint32_t bar) {  // pair: the barrier of both CTAs
+  if constexpr (kPair) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+  } else {
+    tc::mma_commit(bar);
+  }
+}
+template <bool kPair>
+OSCAR_DEVINL void pc_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  } else {
+    tc::mma_ss(d, a, b, idesc, acc);
+  }
+}
+template <bool kPair>
+OSCAR_DEVINL void pc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  if constexpr (kPair) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+  } else {
+    tc::mma_ts(d, a, b, idesc, acc);
+  }
+}
+// TMA loads into this CTA that count on a barrier of either CTA of the pair
+template <bool kPair>
+OSCAR_DEVINL void pc_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint32_t bar) {
+  if constexpr (kPair) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, "
+        "%5}], [%6];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+  } else {
+    tma_load_4d(dst, map, x, y, z, w, bar);
+  }
+}
+template <bool kPair>
+OSCAR_DEVINL void pc_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+  if constexpr (kPair) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+        "%4}], [%5];\n" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  } else {
+    tma_load_3d(dst, map, x, y, z, bar);
+  }
+}
+
+// The pieces of units of one worker, walked alike by every role.
 struct PcWalk {
   const PcPlan& p;
   int r, h, qb, t, left;
@@ -124,7 +223,7 @@ struct PcWalk {
   }
   OSCAR_DEVINL void open() {
     if (left <= 0) return;
-    nt = pc_tiles<D>(p.q_len[r], p.seq[r], p.tokens, qb);
+    nt = pc_tiles(p.q_len[r], p.seq[r], p.tokens, qb);
     t_end = min(nt, t + left);
   }
   OSCAR_DEVINL bool live() const { return left > 0; }
@@ -132,7 +231,7 @@ struct PcWalk {
     left -= t_end - t;
     t = 0;
     ++piece;
-    const int per = p.tokens * PcShape<D>::kM;
+    const int per = p.tokens * kPcUnit;
     if (++qb >= (p.q_len[r] + per - 1) / per) {
       qb = 0;
       if (++h >= hk) {
@@ -182,50 +281,64 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
                    const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
   using Shape = PcShape<D>;
-  constexpr int kM = Shape::kM, kPanels = Shape::kPanels, kHalves = Shape::kHalves, kSlots = Shape::kSlots;
+  constexpr bool kPair = Shape::kPair;
+  constexpr int kM = Shape::kM, kPanels = Shape::kPanels, kSlots = Shape::kSlots;
   constexpr int kMma = Shape::kSoftWarps;
   constexpr int kColO = 256;
   extern __shared__ __align__(1024) uint8_t pc_raw[];
   PcSmem<D>& sm = *reinterpret_cast<PcSmem<D>*>(pc_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t rank = kPair ? pc_rank() : 0u;
+  const int worker = kPair ? (int)blockIdx.x / 2 : (int)blockIdx.x;
   pdl_release();
   auto full = [&](int i) { return smem_u32(&sm.full[i]); };
   auto empty = [&](int i) { return smem_u32(&sm.empty[i]); };
+  // a barrier that the pair's first CTA owns, for arrivals and loads
+  auto lead = [&](uint32_t bar) { return kPair ? pc_map(bar, 0) : bar; };
   if (warp == kMma) {
     if (lane == 0) {
+      constexpr int kCtas = kPair ? 2 : 1;
       for (int i = 0; i < kSlots; ++i) {
-        tc::mbar_init(full(i), 1);
+        tc::mbar_init(full(i), kCtas);  // each CTA's producer announces its own bytes
         tc::mbar_init(empty(i), 1);
       }
       for (int i = 0; i < 2; ++i) {
         tc::mbar_init(smem_u32(&sm.s_full[i]), 1);
-        tc::mbar_init(smem_u32(&sm.p_full[i]), kPcRows);
+        tc::mbar_init(smem_u32(&sm.p_full[i]), 4 * kCtas);  // a warp's rows each
         tc::mbar_init(smem_u32(&sm.o_done[i]), 1);
       }
-      tc::mbar_init(smem_u32(&sm.q_full), 1);
+      tc::mbar_init(smem_u32(&sm.q_full), kCtas);
       tc::mbar_init(smem_u32(&sm.q_empty), 1);
+      tc::mbar_init(smem_u32(&sm.tail), 1);
       tc::mbar_init(smem_u32(&sm.end), 1);
       sm.abort = 0;
       tc::mbar_fence_init();
     }
     __syncwarp();
-    tc::tmem_alloc(smem_u32(&sm.tmem), 512);
-    tc::tmem_relinquish();
+    if constexpr (kPair) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&sm.tmem)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::);
+    } else {
+      tc::tmem_alloc(smem_u32(&sm.tmem), 512);
+      tc::tmem_relinquish();
+    }
   }
   tc::tc_fence_before();
-  __syncthreads();
+  if constexpr (kPair) pc_cluster_sync();  // the other CTA's barriers are initialised
+  else __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = sm.tmem;
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {  // warp-uniform
     return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
   };
   pdl_wait();
-  PcWalk<D> w(p, blockIdx.x);
+  PcWalk w(p, worker);
   const int n_tiles = w.left;
 
   if (warp < kMma) {
     // ================= softmax: thread = query row of row tile `wg`
     const int wg = warp / 4, row = tid & 127;
+    const int rt = kPair ? (int)rank : wg;  // row tile of the unit
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const int rows = p.tokens * a.group;  // live rows of a row tile
     int job = kM == 2 ? wg : 0;           // jobs are numbered over the whole CTA
@@ -233,7 +346,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     bool ok = true;
     for (; w.live() && ok; w.next(a.hk)) {
       const int q_len = p.q_len[w.r], seq = p.seq[w.r];
-      const int tok = (w.qb * kM + wg) * p.tokens + row / a.group;
+      const int tok = (w.qb * kPcUnit + rt) * p.tokens + row / a.group;
       const bool live = row < rows && tok < q_len;
       // visible keys; rows that hold no query are computed as they come and not written
       const int lim = live ? max(0, seq - q_len + tok + 1) : INT_MAX;
@@ -308,33 +421,13 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
           }
           tc::tmem_st16(s_col + c0 / 2, pk);
         }
-        const int have = seq - t * kPcKeys;
-        if (have < kPcKeys) {
-          // the last tile: what lies past the sequence may be anything (0 * NaN).  The V slots of
-          // the tile have landed before their rows are cleared
-          const int first = max(have, 0);
-          const int order = kM == 2 ? job >> 1 : job;  // key tile in the CTA's stream
-          // (D 256: the product before it is complete, so the slot's earlier use has landed too and
-          // the parity below can only mean this one)
-          bool there = kM == 2 || job == 0 || wait(smem_u32(&sm.o_done[b ^ 1]), ((job - 1) >> 1) & 1);
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) {
-            const int at = pc_v_at<D>(order, hf, n_tiles);
-            there = there && wait(full(at % kSlots), (at / kSlots) & 1);
-            constexpr int kRowsHere = kPcKeys / kHalves;
-            uint8_t* v = sm.ring[at % kSlots];
-            for (int i = row; i < kRowsHere * (D / 8); i += kPcRows) {
-              const int key = i / (D / 8), ch = i % (D / 8);
-              if (hf * kRowsHere + key >= first)
-                *reinterpret_cast<uint4*>(v + (ch / 8) * (kRowsHere * 128) + key * 128 + (ch % 8) * 16) = make_uint4(0, 0, 0, 0);
-            }
-          }
-          if (!there) { ok = false; break; }
-          tc::fence_async_smem();
-        }
         tc::tmem_wait_st();
         tc::tc_fence_before();
-        tc::mbar_arrive(smem_u32(&sm.p_full[b]));
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) pc_arrive(lead(smem_u32(&sm.p_full[b])));
+          else tc::mbar_arrive(smem_u32(&sm.p_full[b]));
+        }
       }
       if (!ok) break;
       // ---- O of this piece
@@ -347,7 +440,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       const float inv = none ? 0.0f : 1.0f / total;
       const int head = w.h * a.group + row % a.group;
       const int64_t orow = (int64_t)(p.q_start[w.r] + tok) * a.hq + head;
-      const int64_t prow = ((int64_t)(2 * blockIdx.x + (w.piece == 0 ? 0 : 1)) * kM + wg) * kPcRows + row;
+      const int64_t prow = ((int64_t)(2 * worker + (w.piece == 0 ? 0 : 1)) * kPcUnit + rt) * kPcRows + row;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -381,47 +474,55 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       tc::tc_fence_before();  // the next unit's first product overwrites O after this thread's next P
     }
   } else if (warp == kMma) {
-    // ================= MMA issuer
+    // ================= MMA issuer (of a pair: the first CTA's)
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    constexpr uint32_t idesc_s = tc::instr_desc(fmt, 0, 0, kPcRows, kPcKeys);
-    constexpr uint32_t idesc_o = tc::instr_desc(fmt, 0, 1, kPcRows, D);
+    constexpr int kRows = kPair ? 2 * kPcRows : kPcRows;
+    constexpr uint32_t idesc_s = tc::instr_desc(fmt, 0, 0, kRows, kPcKeys);
+    constexpr uint32_t idesc_o = tc::instr_desc(fmt, 0, 1, kRows, D);
     const uint64_t dq = pc_desc(smem_u32(sm.q), 16, 1024);
     const uint64_t dk = pc_desc(smem_u32(sm.ring), 16, 1024);
-    const uint64_t dv = pc_desc(smem_u32(sm.ring), (kPcKeys / kHalves) * 128, 1024);
+    const uint64_t dv = pc_desc(smem_u32(sm.ring), kPcKeys * 128, 1024);
     constexpr uint64_t kSlotStep = Shape::kSlot >> 4;
+    auto wait_pair = [&](uint32_t bar, uint32_t parity) -> bool {
+      if constexpr (kPair) {
+        bool got = false;
+        for (uint32_t i = 0; i < tc::kSpinLimit && !got; ++i) {
+          got = pc_try_cluster(bar, parity);
+          if (!got && *reinterpret_cast<volatile int*>(&sm.abort) != 0) break;
+        }
+        if (!got) {
+          *reinterpret_cast<volatile int*>(&sm.abort) = 1;
+          flag_error(16u);
+        }
+        return __all_sync(0xffffffffu, got);
+      } else {
+        return wait(bar, parity);
+      }
+    };
     // S runs two jobs ahead of O and may belong to the next unit
-    PcWalk<D> ws = w;                            // unit of the next S
+    PcWalk ws = w;                               // unit of the next S
     int unit = 0;                                // its number
     int s_left = (ws.t_end - ws.t) * kM, o_left = s_left;  // jobs left in the units of the next S and O
     bool s_open = false, o_open = false;         // the unit's Q has been waited for; O holds a product of the unit
-    const int jobs = n_tiles * kM;
+    const int jobs = rank == 0 ? n_tiles * kM : -2;
 #pragma unroll 1
     for (int step = 0; step < jobs + 2; ++step) {
       const int jo = step - 2, js = step;
       if (jo >= 0) {
         const int tile = kM == 2 ? jo >> 1 : jo;
         const int mt = kM == 2 ? jo & 1 : 0;
-        if (!wait(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
-        bool there = true;
-        if (mt == 0) {
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) {
-            const int at = pc_v_at<D>(tile, hf, n_tiles);
-            there = there && wait(full(at % kSlots), (at / kSlots) & 1);
-          }
-        }
-        if (!there) break;
+        const int at = pc_v_at<D>(tile, n_tiles), slot = at % kSlots;
+        if (!wait_pair(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
+        if (mt == 0 && !wait_pair(full(slot), (at / kSlots) & 1)) break;
         tc::tc_fence_after();
         if (tc::elect_one()) {
-          constexpr int kStepsPerSlot = kPcKeys / kHalves / 16;
+          const uint64_t vd = dv + (uint64_t)slot * kSlotStep;
 #pragma unroll
-          for (int ks = 0; ks < kPcKeys / 16; ++ks) {
-            const int at = pc_v_at<D>(tile, ks / kStepsPerSlot, n_tiles);
-            const uint64_t vd = dv + (uint64_t)(at % kSlots) * kSlotStep + (uint64_t)((ks % kStepsPerSlot) * (2048 >> 4));
-            tc::mma_ts(tmem + kColO + 128 * mt, tmem + 128 * (jo & 1) + 8 * ks, vd, idesc_o, (o_open || ks > 0) ? 1u : 0u);
-            if (mt == kM - 1 && (ks + 1) % kStepsPerSlot == 0) tc::mma_commit(empty(at % kSlots));
-          }
-          tc::mma_commit(smem_u32(&sm.o_done[jo & 1]));
+          for (int ks = 0; ks < kPcKeys / 16; ++ks)
+            pc_mma_ts<kPair>(tmem + kColO + 128 * mt, tmem + 128 * (jo & 1) + 8 * ks, vd + ks * (2048 >> 4), idesc_o,
+                             (o_open || ks > 0) ? 1u : 0u);
+          if (mt == kM - 1) pc_commit<kPair>(empty(slot));
+          pc_commit<kPair>(smem_u32(&sm.o_done[jo & 1]));
         }
         __syncwarp();
         if (mt == kM - 1) o_open = true;
@@ -432,36 +533,26 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
       }
       if (js < jobs) {
-        if (!s_open && !wait(smem_u32(&sm.q_full), unit & 1)) break;
+        if (!s_open && !wait_pair(smem_u32(&sm.q_full), unit & 1)) break;
         s_open = true;
         const int tile = kM == 2 ? js >> 1 : js;
         const int mt = kM == 2 ? js & 1 : 0;
-        bool there = true;
-        if (mt == 0) {
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf) {
-            const int at = pc_k_at<D>(tile, hf);
-            there = there && wait(full(at % kSlots), (at / kSlots) & 1);
-          }
-        }
-        if (!there) break;
+        const int at = pc_k_at<D>(tile), slot = at % kSlots;
+        if (mt == 0 && !wait_pair(full(slot), (at / kSlots) & 1)) break;
         tc::tc_fence_after();
         const bool last = --s_left == 0;
         if (tc::elect_one()) {
 #pragma unroll
           for (int pn = 0; pn < kPanels; ++pn) {
-            const int at = pc_k_at<D>(tile, pn * kHalves / kPanels);
             const uint64_t qd = dq + (uint64_t)((mt * kPanels + pn) * (kPcRows * 128 >> 4));
-            const uint64_t kd = dk + (uint64_t)(at % kSlots) * kSlotStep +
-                                (uint64_t)((pn % (kPanels / kHalves)) * (kPcKeys * 128 >> 4));
+            const uint64_t kd = dk + (uint64_t)slot * kSlotStep + (uint64_t)(pn * (Shape::kKeys * 128 >> 4));
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
-              tc::mma_ss(tmem + 128 * (js & 1), qd + 2 * ks, kd + 2 * ks, idesc_s, pn + ks > 0 ? 1u : 0u);
-            // a slot is released as soon as its last product is issued
-            if (mt == kM - 1 && (pn + 1) % (kPanels / kHalves) == 0) tc::mma_commit(empty(at % kSlots));
+              pc_mma_ss<kPair>(tmem + 128 * (js & 1), qd + 2 * ks, kd + 2 * ks, idesc_s, pn + ks > 0 ? 1u : 0u);
           }
-          tc::mma_commit(smem_u32(&sm.s_full[js & 1]));
-          if (last) tc::mma_commit(smem_u32(&sm.q_empty));
+          if (mt == kM - 1) pc_commit<kPair>(empty(slot));
+          pc_commit<kPair>(smem_u32(&sm.s_full[js & 1]));
+          if (last) pc_commit<kPair>(smem_u32(&sm.q_empty));
         }
         __syncwarp();
         if (last) {
@@ -473,9 +564,11 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       }
     }
     // no MMA may be in flight when the tensor memory is freed
-    if (tc::elect_one()) tc::mma_commit(smem_u32(&sm.end));
-    __syncwarp();
-    if (!tc::mbar_wait(smem_u32(&sm.end), 0) && lane == 0) flag_error(16u);
+    if (rank == 0) {
+      if (tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
+      __syncwarp();
+      if (!tc::mbar_wait(smem_u32(&sm.end), 0) && lane == 0) flag_error(16u);
+    }
   } else {
     // ================= producers: one warp fetches K (and Q), one V, each in the order of use.
     // Lane i holds the pages of boxes i, i + 32, .. of the next tile, looked up while the tile
@@ -484,8 +577,12 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     const CUtensorMap* map = is_k ? &kmap : &vmap;
     const int per = kPcKeys / a.box;  // boxes per tile
     const uint32_t box = (uint32_t)a.box, box_bytes = box * 128u;
+    // of a pair's tile: K half of the keys, V half of the dims
+    const int box0 = kPair && is_k ? (int)rank * (per / 2) : 0, nbox = kPair && is_k ? per / 2 : per;
+    const int pan0 = kPair && !is_k ? (int)rank * Shape::kVPanels : 0, pans = is_k ? kPanels : Shape::kVPanels;
+    const uint32_t panel = (uint32_t)nbox * box_bytes;  // bytes of a panel of the slot
     const int32_t* row = nullptr;
-    int boxes = 0, unit = 0, t = 0, last_at = -1;
+    int boxes = 0, unit = 0, t = 0, last_at = -1, tails = 0;
     int blk[kPcKeys / 32];
     auto look_up = [&] {
 #pragma unroll
@@ -495,9 +592,9 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         blk[i] = j < per && b < boxes ? row[a.page.div((uint32_t)b * box)] : 0;
       }
     };
-    bool ok = true, open = false;
+    bool open = false;
 #pragma unroll 1
-    for (int tile = 0; tile < n_tiles && ok; ++tile) {
+    for (int tile = 0; tile < n_tiles; ++tile) {
       if (!open) {  // a new piece, with its queries
         t = w.t;
         row = a.table + (int64_t)p.req_id[w.r] * a.table_stride;
@@ -507,18 +604,21 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         if (is_k) {
           if (unit > 0 && !wait(smem_u32(&sm.q_empty), (unit - 1) & 1)) break;
           if (tc::elect_one()) {
-            const uint32_t bar = smem_u32(&sm.q_full);
-            tc::mbar_expect_tx(bar, (uint32_t)(kM * kPanels * p.tokens * a.group * 128));
+            const uint32_t bar = lead(smem_u32(&sm.q_full));
+            const uint32_t bytes = (uint32_t)(kM * kPanels * p.tokens * a.group * 128);
+            if constexpr (kPair) pc_expect(bar, bytes);
+            else tc::mbar_expect_tx(bar, bytes);
 #pragma unroll 1
             for (int i = 0; i < kM * kPanels; ++i)
-              tma_load_3d(smem_u32(sm.q) + i * kPcRows * 128, &qmap, 64 * (i % kPanels), w.h * a.group,
-                          p.q_start[w.r] + (w.qb * kM + i / kPanels) * p.tokens, bar);
+              pc_load_3d<kPair>(smem_u32(sm.q) + i * kPcRows * 128, &qmap, 64 * (i % kPanels), w.h * a.group,
+                                p.q_start[w.r] + (w.qb * kPcUnit + (kPair ? (int)rank : i / kPanels)) * p.tokens, bar);
           }
           __syncwarp();
           ++unit;
         }
       }
       const int first = t * per, h = w.h, here = min(per, max(0, boxes - first));
+      const int have = p.seq[w.r] - t * kPcKeys;  // keys of the request from the tile's first on
       int cur[kPcKeys / 32];
 #pragma unroll
       for (int i = 0; i < kPcKeys / 32; ++i) {
@@ -534,38 +634,53 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         w.next(a.hk);
         open = false;
       }
+      const int at = is_k ? pc_k_at<D>(tile) : pc_v_at<D>(tile, n_tiles), slot = at % kSlots;
+      const int live = max(0, min(nbox, here - box0));
+      if (at >= kSlots && !wait(empty(slot), ((at / kSlots) - 1) & 1)) break;
+      last_at = at;
+      // a V tile past whose end anything may stand (0 * NaN) is completed here before it is announced
+      const bool tail = !is_k && have < kPcKeys;
+      const uint32_t bar = tail ? smem_u32(&sm.tail) : lead(full(slot));
+      const uint32_t bytes = (uint32_t)(live * pans) * box_bytes;
+      if (tc::elect_one()) {
+        if (kPair && !tail) pc_expect(bar, bytes);
+        else tc::mbar_expect_tx(bar, bytes);
+      }
+      __syncwarp();
+      const uint32_t dst = smem_u32(sm.ring[slot]);
 #pragma unroll 1
-      for (int hf = 0; hf < kHalves; ++hf) {
-        const int at = is_k ? pc_k_at<D>(tile, hf) : pc_v_at<D>(tile, hf, n_tiles), slot = at % kSlots;
-        // K: panels [hf * kPanels / kHalves, ..), all boxes; V: all panels, boxes of this key half
-        const int pan0 = is_k ? hf * (kPanels / kHalves) : 0, pans = is_k ? kPanels / kHalves : kPanels;
-        const int box0 = is_k ? 0 : hf * (per / kHalves), nbox = is_k ? per : per / kHalves;
-        const int live = max(0, min(nbox, here - box0));
-        const uint32_t panel = (uint32_t)nbox * box_bytes;  // bytes of a panel of the slot
-        if (at >= kSlots && !wait(empty(slot), ((at / kSlots) - 1) & 1)) { ok = false; break; }
-        last_at = at;
-        if (tc::elect_one()) tc::mbar_expect_tx(full(slot), (uint32_t)(live * pans) * box_bytes);
-        __syncwarp();
-        const uint32_t dst = smem_u32(sm.ring[slot]);
-#pragma unroll 1
-        for (int i = 0; i < live; ++i) {
-          const int j = box0 + i;
-          int b = 0;
+      for (int i = 0; i < live; ++i) {
+        const int j = box0 + i;
+        int b = 0;
 #pragma unroll
-          for (int k = 0; k < kPcKeys / 32; ++k) {
-            if (32 * k >= per) break;
-            const int v = __shfl_sync(0xffffffffu, cur[k], j & 31);
-            if (j >> 5 == k) b = v;
-          }
-          const int off = (int)a.page.mod((uint32_t)(first + j) * box);
-          if (tc::elect_one()) {
-#pragma unroll
-            for (int pn = 0; pn < kPanels; ++pn)
-              if (pn < pans)
-                tma_load_4d(dst + pn * panel + (uint32_t)i * box_bytes, map, 64 * (pan0 + pn), h, off, b, full(slot));
-          }
+        for (int k = 0; k < kPcKeys / 32; ++k) {
+          if (32 * k >= per) break;
+          const int v = __shfl_sync(0xffffffffu, cur[k], j & 31);
+          if (j >> 5 == k) b = v;
         }
+        const int off = (int)a.page.mod((uint32_t)(first + j) * box);
+        if (tc::elect_one()) {
+#pragma unroll
+          for (int pn = 0; pn < kPanels; ++pn)
+            if (pn < pans)
+              pc_load_4d<kPair>(dst + pn * panel + (uint32_t)i * box_bytes, map, 64 * (pan0 + pn), h, off, b, bar);
+        }
+      }
+      __syncwarp();
+      if (tail) {
+        if (!wait(bar, tails & 1)) break;
+        ++tails;
+        const int clear = max(have, 0);
+        for (int i = lane; i < (kPcKeys - clear) * 8 * pans; i += 32) {
+          const int key = clear + i / (8 * pans), c = i % (8 * pans);
+          *reinterpret_cast<uint4*>(sm.ring[slot] + (c / 8) * panel + key * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        tc::fence_async_smem();
         __syncwarp();
+        if (lane == 0) {
+          if constexpr (kPair) pc_arrive(lead(full(slot)));
+          else tc::mbar_arrive(full(slot));
+        }
       }
     }
     // no copy may still be writing shared memory when the CTA ends.  The MMA warp has waited for
@@ -576,11 +691,14 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     }
   }
 
+  __syncwarp();
   tc::tc_fence_before();
-  __syncthreads();
+  if constexpr (kPair) pc_cluster_sync();  // neither CTA's barriers, tensor or shared memory are used from here on
+  else __syncthreads();
   if (warp == kMma) {
     tc::tc_fence_after();
-    tc::tmem_dealloc(tmem, 512);
+    if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");
+    else tc::tmem_dealloc(tmem, 512);
   }
 }
 
@@ -589,7 +707,7 @@ template <int D, typename T>
 __global__ void __launch_bounds__(128) paged_chunk_combine_kernel(const __grid_constant__ PagedArgs a,
                                                                   const __grid_constant__ PcPlan p,
                                                                   const __grid_constant__ PcSplits splits) {
-  constexpr int kM = PcShape<D>::kM, E = D / 32;
+  constexpr int kM = kPcUnit, E = D / 32;
   pdl_release();
   const int lane = threadIdx.x & 31;
   const int idx = blockIdx.x * 4 + (threadIdx.x >> 5);
