@@ -135,23 +135,20 @@ OSCAR_DEVINL uint32_t pc_map(uint32_t addr, uint32_t rank) {  // the same shared
 OSCAR_DEVINL void pc_cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// (kWrites: the arrival publishes this thread's shared-memory writes to the other CTA.  Arrivals for
+// tensor memory that tcgen05.wait has completed need no release beyond the CTA, and one at cluster
+// scope takes 800 cycles)
+template <bool kWrites>
 OSCAR_DEVINL void pc_arrive(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+  if constexpr (kWrites)
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+  else
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
 }
 OSCAR_DEVINL void pc_expect(uint32_t cluster_addr, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;\n" ::"r"(cluster_addr),
+  asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;\n" ::"r"(cluster_addr),
                "r"(bytes)
                : "memory");
-}
-OSCAR_DEVINL bool pc_try_cluster(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
-      "p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
 }
 template <bool kPair>
 OSCAR_DEVINL void pc_commit(uint32_t bar) {  // pair: the barrier of both CTAs
@@ -275,6 +272,32 @@ template <> OSCAR_DEVINL uint32_t pc_pack<__half>(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
+// x[k] of lane 8 g + i <-> x[i] of lane 8 g + k (16-byte pieces), in three exchanges
+OSCAR_DEVINL void pc_transpose8(uint32_t (&x)[8][4], int lane) {
+#pragma unroll
+  for (int bit = 1; bit < 8; bit <<= 1) {
+    const bool up = lane & bit;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k & bit) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        // the lane keeps the piece whose index has its own bit and sends the other one
+        const uint32_t give = up ? x[k][i] : x[k | bit][i];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, give, bit);
+        if (up) x[k][i] = got;
+        else x[k | bit][i] = got;
+      }
+    }
+  }
+}
+// 32 bytes (a whole sector) to a 32-byte aligned address
+OSCAR_DEVINL void pc_store32(void* dst, const uint32_t* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]),
+               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
+               : "memory");
+}
+
 template <int D, typename T>
 __global__ void __launch_bounds__(PcShape<D>::kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PcPlan p,
@@ -359,26 +382,22 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const uint32_t s_col = tmem + lanes + 128 * b;
         if (!wait(smem_u32(&sm.s_full[b]), (job >> 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        // Two passes over the scores in chunks of 32 columns, each a short loop: unrolled over
-        // the row, the warps of the CTA run out of the instruction cache (see below)
+        // the row's scores stay in registers over both passes
         const int vis = lim - t * kPcKeys;  // keys c < vis are visible
-        const bool masked = __any_sync(0xffffffffu, vis < kPcKeys);
-        uint32_t s[32];
-        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll 1
-        for (int c0 = 0; c0 < kPcKeys; c0 += 32) {
-          tc::tmem_ld32(s_col + c0, s);
-          tc::tmem_wait_ld();
-          if (masked) {
+        uint32_t s[kPcKeys];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] = c0 + c < vis ? s[c] : 0xff800000u;
-          }
+        for (int c = 0; c < kPcKeys; c += 32) tc::tmem_ld32(s_col + c, s + c);
+        tc::tmem_wait_ld();
+        if (__any_sync(0xffffffffu, vis < kPcKeys)) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 8)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
+          for (int c = 0; c < kPcKeys; ++c) s[c] = c < vis ? s[c] : 0xff800000u;
         }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kPcKeys; c += 8)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
         const bool grow = mx > m + kPgHeadroom;
         const bool rescale = grow && m != -INFINITY;
@@ -402,36 +421,31 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
         const float base = m == -INFINITY ? 0.0f : -m;
         const uint64_t scale2 = f2_pack(scale, scale), base2 = f2_pack(base, base);
-#pragma unroll 1
-        for (int c0 = 0; c0 < kPcKeys; c0 += 32) {
-          // (the columns P overwrites, [c0 / 2, c0 / 2 + 16), have been read)
-          tc::tmem_ld32(s_col + c0, s);
-          tc::tmem_wait_ld();
-          if (masked) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) s[c] = c0 + c < vis ? s[c] : 0xff800000u;
-          }
+        for (int c = 0; c < kPcKeys; c += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, base2);
+            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
             const float e0 = pg_exp2(f2_lo(x)), e1 = pg_exp2(f2_hi(x));
             l2 = f2_add(l2, f2_pack(e0, e1));
             pk[i] = pc_pack<T>(e0, e1);
           }
-          tc::tmem_st16(s_col + c0 / 2, pk);
+          tc::tmem_st16(s_col + c / 2, pk);
         }
         tc::tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (kPair) pc_arrive(lead(smem_u32(&sm.p_full[b])));
+          if constexpr (kPair) pc_arrive<false>(lead(smem_u32(&sm.p_full[b])));
           else tc::mbar_arrive(smem_u32(&sm.p_full[b]));
         }
       }
       if (!ok) break;
       // ---- O of this piece
+      // (D 256: the product before the last one first, whose arrival nothing else waits for)
       const int last = job - kM;
+      if (kM == 1 && last > 0 && !wait(smem_u32(&sm.o_done[(last - 1) & 1]), ((last - 1) >> 1) & 1)) { ok = false; break; }
       if (!wait(smem_u32(&sm.o_done[last & 1]), (last >> 1) & 1)) { ok = false; break; }
       tc::tc_fence_after();
       const float total = f2_lo(l2) + f2_hi(l2);
@@ -441,26 +455,42 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       const int head = w.h * a.group + row % a.group;
       const int64_t orow = (int64_t)(p.q_start[w.r] + tok) * a.hq + head;
       const int64_t prow = ((int64_t)(2 * worker + (w.piece == 0 ? 0 : 1)) * kPcUnit + rt) * kPcRows + row;
+      if (whole) {
+        // 64 columns at a time: a row's 128 bytes lie in one lane, and 8 lanes exchange 16-byte pieces
+        // so that a store instruction writes whole lines of 4 rows (32 lines of one sector each took
+        // 9400 cycles a unit)
+        const int64_t my_row = live ? orow : -1;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        tc::tmem_ld32(o_col + c, o);
-        tc::tmem_wait_ld();
-        if (!live) continue;
-        if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + orow * D + c);
+        for (int c = 0; c < D; c += 64) {
+          uint32_t o[32], x[8][4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t x[4];
+          for (int hf = 0; hf < 2; ++hf) {
+            tc::tmem_ld32(o_col + c + 32 * hf, o);
+            tc::tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              x[k] = pc_pack<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-            dst[i] = make_uint4(x[0], x[1], x[2], x[3]);
+            for (int i = 0; i < 16; ++i)
+              x[4 * hf + i / 4][i % 4] = pc_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
           }
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(a.part_o + prow * D + c);
+          pc_transpose8(x, lane);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int k = 0; k < 8; ++k) {
+            const int64_t to = __shfl_sync(0xffffffffu, my_row, (lane & 24) + k);
+            if (to >= 0)
+              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + to * D + c + 8 * (lane & 7)) =
+                  make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tc::tmem_ld32(o_col + c, o);
+          tc::tmem_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pc_store32(a.part_o + prow * D + c + 8 * i, o + 8 * i);
+          }
+          __syncwarp();
         }
       }
       if (live) {
@@ -483,21 +513,13 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     const uint64_t dk = pc_desc(smem_u32(sm.ring), 16, 1024);
     const uint64_t dv = pc_desc(smem_u32(sm.ring), kPcKeys * 128, 1024);
     constexpr uint64_t kSlotStep = Shape::kSlot >> 4;
-    auto wait_pair = [&](uint32_t bar, uint32_t parity) -> bool {
-      if constexpr (kPair) {
-        bool got = false;
-        for (uint32_t i = 0; i < tc::kSpinLimit && !got; ++i) {
-          got = pc_try_cluster(bar, parity);
-          if (!got && *reinterpret_cast<volatile int*>(&sm.abort) != 0) break;
-        }
-        if (!got) {
-          *reinterpret_cast<volatile int*>(&sm.abort) = 1;
-          flag_error(16u);
-        }
-        return __all_sync(0xffffffffu, got);
-      } else {
-        return wait(bar, parity);
-      }
+    // The warp runs the role converged and elects a lane for each batch of products (run by one
+    // thread of a diverged warp the products issue slower: 2580 against 2430 us).  What a step
+    // needs beside P is waited for before P where its slot was released by earlier steps, so that
+    // both products go out back to back; a new unit's queries come only once the S before it is
+    // complete and are waited for after the PV
+    auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
+      return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
     };
     // S runs two jobs ahead of O and may belong to the next unit
     PcWalk ws = w;                               // unit of the next S
@@ -508,24 +530,28 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
 #pragma unroll 1
     for (int step = 0; step < jobs + 2; ++step) {
       const int jo = step - 2, js = step;
+      const int o_mt = kM == 2 ? jo & 1 : 0, s_mt = kM == 2 ? js & 1 : 0;
+      const int v_at = pc_v_at<D>(kM == 2 ? jo >> 1 : jo, n_tiles), v_slot = v_at % kSlots;
+      const int k_at = pc_k_at<D>(kM == 2 ? js >> 1 : js), k_slot = k_at % kSlots;
+      if (jo >= 0 && o_mt == 0 && !wait_all(full(v_slot), (v_at / kSlots) & 1)) break;
+      if (js < jobs && s_open && s_mt == 0) {
+        if (!wait_all(full(k_slot), (k_at / kSlots) & 1)) break;
+        tc::tc_fence_after();
+      }
       if (jo >= 0) {
-        const int tile = kM == 2 ? jo >> 1 : jo;
-        const int mt = kM == 2 ? jo & 1 : 0;
-        const int at = pc_v_at<D>(tile, n_tiles), slot = at % kSlots;
-        if (!wait_pair(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
-        if (mt == 0 && !wait_pair(full(slot), (at / kSlots) & 1)) break;
+        if (!wait_all(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
         tc::tc_fence_after();
         if (tc::elect_one()) {
-          const uint64_t vd = dv + (uint64_t)slot * kSlotStep;
+          const uint64_t vd = dv + (uint64_t)v_slot * kSlotStep;
 #pragma unroll
           for (int ks = 0; ks < kPcKeys / 16; ++ks)
-            pc_mma_ts<kPair>(tmem + kColO + 128 * mt, tmem + 128 * (jo & 1) + 8 * ks, vd + ks * (2048 >> 4), idesc_o,
+            pc_mma_ts<kPair>(tmem + kColO + 128 * o_mt, tmem + 128 * (jo & 1) + 8 * ks, vd + ks * (2048 >> 4), idesc_o,
                              (o_open || ks > 0) ? 1u : 0u);
-          if (mt == kM - 1) pc_commit<kPair>(empty(slot));
+          if (o_mt == kM - 1) pc_commit<kPair>(empty(v_slot));
           pc_commit<kPair>(smem_u32(&sm.o_done[jo & 1]));
         }
         __syncwarp();
-        if (mt == kM - 1) o_open = true;
+        if (o_mt == kM - 1) o_open = true;
         if (--o_left == 0) {
           w.next(a.hk);
           o_open = false;
@@ -533,24 +559,22 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
       }
       if (js < jobs) {
-        if (!s_open && !wait_pair(smem_u32(&sm.q_full), unit & 1)) break;
-        s_open = true;
-        const int tile = kM == 2 ? js >> 1 : js;
-        const int mt = kM == 2 ? js & 1 : 0;
-        const int at = pc_k_at<D>(tile), slot = at % kSlots;
-        if (mt == 0 && !wait_pair(full(slot), (at / kSlots) & 1)) break;
-        tc::tc_fence_after();
+        if (!s_open) {
+          if (!wait_all(smem_u32(&sm.q_full), unit & 1) || !wait_all(full(k_slot), (k_at / kSlots) & 1)) break;
+          tc::tc_fence_after();
+          s_open = true;
+        }
         const bool last = --s_left == 0;
         if (tc::elect_one()) {
 #pragma unroll
           for (int pn = 0; pn < kPanels; ++pn) {
-            const uint64_t qd = dq + (uint64_t)((mt * kPanels + pn) * (kPcRows * 128 >> 4));
-            const uint64_t kd = dk + (uint64_t)slot * kSlotStep + (uint64_t)(pn * (Shape::kKeys * 128 >> 4));
+            const uint64_t qd = dq + (uint64_t)((s_mt * kPanels + pn) * (kPcRows * 128 >> 4));
+            const uint64_t kd = dk + (uint64_t)k_slot * kSlotStep + (uint64_t)(pn * (Shape::kKeys * 128 >> 4));
 #pragma unroll
             for (int ks = 0; ks < 4; ++ks)
               pc_mma_ss<kPair>(tmem + 128 * (js & 1), qd + 2 * ks, kd + 2 * ks, idesc_s, pn + ks > 0 ? 1u : 0u);
           }
-          if (mt == kM - 1) pc_commit<kPair>(empty(slot));
+          if (s_mt == kM - 1) pc_commit<kPair>(empty(k_slot));
           pc_commit<kPair>(smem_u32(&sm.s_full[js & 1]));
           if (last) pc_commit<kPair>(smem_u32(&sm.q_empty));
         }
@@ -563,12 +587,11 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
       }
     }
-    // no MMA may be in flight when the tensor memory is freed
-    if (rank == 0) {
-      if (tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
-      __syncwarp();
-      if (!tc::mbar_wait(smem_u32(&sm.end), 0) && lane == 0) flag_error(16u);
-    }
+    // no MMA may be in flight when the tensor memory is freed (of a pair, the arrival at the second
+    // CTA has come before that CTA ends)
+    if (rank == 0 && tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
+    __syncwarp();
+    wait_all(smem_u32(&sm.end), 0);
   } else {
     // ================= producers: one warp fetches K (and Q), one V, each in the order of use.
     // Lane i holds the pages of boxes i, i + 32, .. of the next tile, looked up while the tile
@@ -678,10 +701,18 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         tc::fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (kPair) pc_arrive(lead(full(slot)));
+          if constexpr (kPair) pc_arrive<true>(lead(full(slot)));
           else tc::mbar_arrive(full(slot));
         }
       }
+    }
+    // the releases of the last slots come to both CTAs of a pair: none may come to a CTA that ended
+    if constexpr (kPair) {
+      for (int i = max(0, n_tiles - 3); i < n_tiles; ++i) {
+        const int n = is_k ? pc_k_at<D>(i) : pc_v_at<D>(i, n_tiles);
+        if (n + kSlots >= 2 * n_tiles && n <= last_at && !wait(empty(n % kSlots), (n / kSlots) & 1)) break;
+      }
+      if (is_k && unit > 0) wait(smem_u32(&sm.q_empty), (unit - 1) & 1);
     }
     // no copy may still be writing shared memory when the CTA ends.  The MMA warp has waited for
     // all of them unless a wait timed out

@@ -182,6 +182,22 @@ def test_paged_attention_many_requests():
     check_attention(q, out, lse, attention64(q, kc, vc, table, lens, seqs, scale), seqs)
 
 
+@pytest.mark.parametrize("d,dtype,hq,hk", [(256, torch.bfloat16, 24, 4), (128, torch.float16, 16, 4), (64, torch.bfloat16, 16, 4)])
+def test_paged_attention_long_streams(d, dtype, hq, hk):
+    """Chunks long enough that every SM streams many tiles of several units, again and again."""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    lens, seqs = [1500, 700], [5000, 700]
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict(d=d, dtype=dtype, hq=hq, hk=hk))
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    check_attention(q, out, lse, attention64(q, kc, vc, table, lens, seqs, scale), seqs)
+    for _ in range(20):
+        again, lse2 = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert kernels.device_error(dev) == 0
+
+
 def test_paged_attention_large_scores():
     """Scores that grow along the keys move the running maximum again and again."""
     from oscar_b200 import kernels
