@@ -8,12 +8,14 @@
 // never overwrites a slot that is still to be read.
 //
 // evict_select_kernel (a CTA per request and head) finds the weight of the last
-// key that stays by a radix descent over order-preserving 32-bit keys (three
-// digits of 11, 11 and 10 bits, counted in shared memory), then walks the
-// positions in order, 1024 at a time, numbers the kept ones with a block-wide
-// prefix sum, writes their list and moves their weights.  Weights are held in
-// shared memory while the request has at most kEvCached keys, else read again
-// on each pass (they are then larger than the SM's share of L1 but in L2).
+// key that stays by histograms over order-preserving 32-bit keys: each round
+// spreads the range that still holds it, [lo, hi], over 2048 bins (the keys'
+// own minimum and maximum first, so that neighbouring threads rarely count in
+// the same bin) and narrows it to one bin, three rounds at most.  Then each warp
+// walks its own stretch of the positions twice: it counts its kept keys, and
+// after one prefix sum over the warps numbers them, writes their list and moves
+// their weights.  A stretch of kEvCached weights is held in shared memory; a
+// longer request is read again for each round and walked stretch by stretch.
 //
 // evict_move_kernel moves the rows.  Bound by bytes.  To other pages every row
 // is independent.  In place a CTA owns a 128-byte slice of one head's K or V
@@ -22,13 +24,13 @@
 // reads are already in flight.
 #pragma once
 
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace oscar {
 
 constexpr int kEvReqs = 256;
 constexpr int kEvThreads = 1024;
-constexpr int kEvCached = 49152;
+constexpr int kEvCached = 49152;  // weights in shared memory
 constexpr int kEvBins = 2048;
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvWaves = 8;  // rows per thread and step of the in-place move
@@ -45,6 +47,7 @@ struct EvictArgs {
   float* weights;                  // [num_blocks, hk, bs]
   int64_t num_blocks;
   int bs, hk;
+  FastDiv page;                    // by bs
   int row_bytes;                   // D * 2
   const int32_t *table, *dst;      // dst == table: in place
   int64_t table_stride, dst_stride;
@@ -61,20 +64,21 @@ OSCAR_DEVINL uint32_t ev_key(float w) {
 }
 
 OSCAR_DEVINL float* ev_weight(const EvictArgs& a, const int32_t* row, int h, int pos) {
-  const int64_t blk = row[pos / a.bs];
+  const int page = (int)a.page.div(pos);
+  const int64_t blk = row[page];
   if (blk < 0 || blk >= a.num_blocks) {
     flag_error(2u);
     return nullptr;
   }
-  return a.weights + (blk * a.hk + h) * a.bs + pos % a.bs;
+  return a.weights + (blk * a.hk + h) * a.bs + (pos - page * a.bs);
 }
 
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_constant__ EvictArgs a,
                                                                   const __grid_constant__ EvictPlan p) {
   extern __shared__ __align__(16) float ev_w[];
   __shared__ uint32_t bins[kEvBins];
-  __shared__ uint32_t warp_sum[32];
-  __shared__ uint32_t pick[2];
+  __shared__ uint32_t warp_sum[2][32];
+  __shared__ uint32_t range[2], pick[2];
   pdl_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x, h = blockIdx.y;
@@ -84,42 +88,61 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
   int32_t* kept = a.kept + ((int64_t)p.req_id[r] * a.hk + h) * a.kept_stride;
   const int n = min(seq, a.keep);
   const bool all = seq <= a.keep;
-  const bool cached = seq <= kEvCached;
+  if (tid == 0) range[0] = 0xffffffffu, range[1] = 0u;
   pdl_wait();
   for (int j = n + tid; j < a.kept_stride; j += kEvThreads) kept[j] = -1;
-  auto global_weight = [&](int pos) -> float {
-    const float* w = ev_weight(a, src_row, h, pos);
-    return w == nullptr ? 0.0f : *w;
-  };
-  if (cached) {
-#pragma unroll 4
-    for (int i = tid; i < seq; i += kEvThreads) ev_w[i] = global_weight(i);
+  // the weights of positions [first, first + kEvCached) to shared memory
+  auto load = [&](int first) {
+    const int end = min(seq, first + kEvCached);
+#pragma unroll 8
+    for (int i = first + tid; i < end; i += kEvThreads) {
+      const float* w = ev_weight(a, src_row, h, i);
+      ev_w[i - first] = w == nullptr ? 0.0f : *w;
+    }
     __syncthreads();
-  }
-  auto weight = [&](int pos) -> float { return cached ? ev_w[pos] : global_weight(pos); };
+  };
+  load(0);
 
   // the key value at which the list is full, and how many of the keys that equal it stay
-  const int lo = a.sink, hi = seq - a.recent;
+  const int lo_pos = a.sink, hi_pos = seq - a.recent;
   uint32_t threshold = 0, need = (uint32_t)max(0, a.keep - a.sink - a.recent);
+  // calls f(key) for the keys between sink and recent, in any order
+  auto each = [&](auto&& f) {
+    for (int first = 0; first < seq; first += kEvCached) {
+      if (seq > kEvCached) {
+        __syncthreads();
+        load(first);
+      }
+      const int from = max(lo_pos, first), to = min(hi_pos, min(seq, first + kEvCached));
+#pragma unroll 4
+      for (int i = from + tid; i < to; i += kEvThreads) f(ev_key(ev_w[i - first]));
+    }
+  };
   if (!all && need > 0) {
+    uint32_t least = 0xffffffffu, most = 0u;
+    each([&](uint32_t key) {
+      least = min(least, key);
+      most = max(most, key);
+    });
+    least = __reduce_min_sync(0xffffffffu, least);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) {
+      atomicMin(&range[0], least);
+      atomicMax(&range[1], most);
+    }
+    __syncthreads();
+    uint32_t lo = range[0], hi = range[1];
 #pragma unroll 1
-    for (int digit = 0; digit < 3; ++digit) {
-      const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-      const int width = digit == 2 ? 10 : 11;
-      const uint32_t above = digit == 0 ? 0u : 0xffffffffu << (shift + width);
+    while (lo < hi) {
+      // bins of 2^shift keys, at most 2048 of them
+      const int shift = max(0, 32 - __clz(hi - lo) - 11);
       for (int i = tid; i < kEvBins; i += kEvThreads) bins[i] = 0;
       __syncthreads();
-      for (int i0 = lo; i0 < hi; i0 += kEvThreads) {
-        const int i = i0 + tid;
-        const uint32_t key = i < hi ? ev_key(weight(i)) : 0u;
-        const bool in = i < hi && (key & above) == (threshold & above);
-        const uint32_t bin = (key >> shift) & ((1u << width) - 1);
-        // weights share few exponents: one add per distinct bin of the warp
-        const uint32_t who = __match_any_sync(0xffffffffu, in ? bin : 0xffffffffu);
-        if (in && (int)(__ffs(who) - 1) == lane) atomicAdd(&bins[bin], (uint32_t)__popc(who));
-      }
+      each([&](uint32_t key) {
+        if (key >= lo && key <= hi) atomicAdd(&bins[(key - lo) >> shift], 1u);
+      });
       __syncthreads();
-      // count from the top: thread t holds bins 2 t' and 2 t' + 1 in descending order
+      // count from the top: thread t holds bins 2 t' + 1 and 2 t' in descending order
       const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
       const uint32_t c1 = bins[b1], c0 = bins[b0];
       uint32_t sum = c1 + c0;
@@ -128,65 +151,79 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
         const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += x;
       }
-      if (lane == 31) warp_sum[warp] = sum;
+      if (lane == 31) warp_sum[0][warp] = sum;
       __syncthreads();
       uint32_t before = sum - (c1 + c0);
-      for (int w = 0; w < warp; ++w) before += warp_sum[w];
+      for (int w = 0; w < warp; ++w) before += warp_sum[0][w];
       if (before < need && before + c1 >= need) pick[0] = b1, pick[1] = need - before;
       else if (before + c1 < need && before + c1 + c0 >= need) pick[0] = b0, pick[1] = need - before - c1;
       __syncthreads();
-      threshold |= pick[0] << shift;
+      lo += pick[0] << shift;
+      hi = min(hi, lo + ((1u << shift) - 1u));
       need = pick[1];
       __syncthreads();
     }
+    threshold = lo;
   }
 
-  // ordered walk
-  uint32_t equal_seen = 0, out = 0;
-  for (int i0 = 0; i0 < seq; i0 += kEvThreads) {
-    const int i = i0 + tid;
-    const float w = i < seq ? weight(i) : 0.0f;
-    const bool fixed = i < seq && (all || i < lo || i >= hi);
-    const bool middle = i < seq && !fixed && a.keep > a.sink + a.recent;
-    const uint32_t key = ev_key(w);
-    const bool above = middle && key > threshold, equal = middle && key == threshold;
-    // prefix of equal keys, then of kept keys: both counts in one 32-bit word (16 bits each)
-    auto prefix = [&](uint32_t mine, uint32_t& total) -> uint32_t {
-      uint32_t sum = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += x;
-      }
-      if (lane == 31) warp_sum[warp] = sum;
+  // ordered walk: the kept keys are the fixed ones, those above the threshold and the first `need`
+  // that equal it
+  uint32_t out = 0, equal = 0;  // kept keys and equal keys of the stretches before
+  const bool chooses = !all && a.keep > a.sink + a.recent;
+  for (int first = 0; first < seq; first += kEvCached) {
+    if (seq > kEvCached) {
       __syncthreads();
-      const uint32_t v = warp_sum[lane];
-      uint32_t scan = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += x;
-      }
-      total = __shfl_sync(0xffffffffu, scan, 31);
-      const uint32_t base = warp == 0 ? 0u : __shfl_sync(0xffffffffu, scan, (warp + 31) & 31);
-      __syncthreads();
-      return base + sum - mine;
-    };
-    // low half: keys above or fixed; high half: equal ones (at most 1024 of each)
-    uint32_t total;
-    const uint32_t at = prefix((fixed || above ? 1u : 0u) | (equal ? 0x10000u : 0u), total);
-    const uint32_t eq_before = equal_seen + (at >> 16);
-    const bool stays = fixed || above || (equal && eq_before < need);
-    // kept keys before this one: all fixed / above ones and the equal ones that stay
-    const uint32_t j = out + (at & 0xffffu) + (min(eq_before, need) - min(equal_seen, need));
-    if (stays && (int)j < n) {
-      kept[j] = i;
-      float* dst = ev_weight(a, dst_row, h, (int)j);
-      if (dst != nullptr) *dst = w;
+      load(first);
     }
-    const uint32_t eq_after = equal_seen + (total >> 16);
-    out += (total & 0xffffu) + (min(eq_after, need) - min(equal_seen, need));
-    equal_seen = eq_after;
+    const int end = min(seq, first + kEvCached);
+    const int per = ((end - first + 31) / 32 + 31) / 32 * 32;  // positions of a warp
+    const int from = first + warp * per, to = min(end, from + per);
+    auto classify = [&](int i, bool& sure, bool& same) {
+      sure = same = false;
+      if (i >= to) return;
+      const bool fixed = all || i < lo_pos || i >= hi_pos;
+      const uint32_t key = ev_key(ev_w[i - first]);
+      sure = fixed || (chooses && key > threshold);
+      same = !fixed && chooses && key == threshold;
+    };
+    uint32_t sures = 0, sames = 0;
+    for (int i0 = from; i0 < to; i0 += 32) {
+      bool sure, same;
+      classify(i0 + lane, sure, same);
+      sures += __popc(__ballot_sync(0xffffffffu, sure));
+      sames += __popc(__ballot_sync(0xffffffffu, same));
+    }
+    if (lane == 0) warp_sum[0][warp] = sures, warp_sum[1][warp] = sames;
+    __syncthreads();
+    // before this warp: kept keys that do not depend on the rank of equal ones, and equal keys
+    uint32_t a_cnt = warp_sum[0][lane], e_cnt = warp_sum[1][lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t x = __shfl_up_sync(0xffffffffu, a_cnt, o), y = __shfl_up_sync(0xffffffffu, e_cnt, o);
+      if (lane >= o) a_cnt += x, e_cnt += y;
+    }
+    const uint32_t a_all = __shfl_sync(0xffffffffu, a_cnt, 31), e_all = __shfl_sync(0xffffffffu, e_cnt, 31);
+    uint32_t eq = equal + __shfl_sync(0xffffffffu, e_cnt, warp) - sames;
+    uint32_t j0 = out + __shfl_sync(0xffffffffu, a_cnt, warp) - sures + (min(eq, need) - min(equal, need));
+    for (int i0 = from; i0 < to; i0 += 32) {
+      const int i = i0 + lane;
+      bool sure, same;
+      classify(i, sure, same);
+      const uint32_t sb = __ballot_sync(0xffffffffu, sure), eb = __ballot_sync(0xffffffffu, same);
+      const uint32_t below = (1u << lane) - 1u;
+      const uint32_t rank = eq + __popc(eb & below);  // of an equal key
+      const uint32_t j = j0 + __popc(sb & below) + (min(rank, need) - min(eq, need));
+      if ((sure || (same && rank < need)) && (int)j < n) {
+        kept[j] = i;
+        float* dst = ev_weight(a, dst_row, h, (int)j);
+        if (dst != nullptr) *dst = ev_w[i - first];
+      }
+      const uint32_t eq_next = eq + __popc(eb);
+      j0 += __popc(sb) + (min(eq_next, need) - min(eq, need));
+      eq = eq_next;
+    }
+    out += a_all + (min(equal + e_all, need) - min(equal, need));
+    equal += e_all;
   }
 }
 
@@ -213,13 +250,13 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_copy_kernel(const __grid
       to_blk[i] = -1;
       if (j >= n) continue;
       const int s = kept[j];
-      const int64_t sb = src_row[s / a.bs], db = dst_row[j / a.bs];
+      const int64_t sb = src_row[a.page.div(s)], db = dst_row[a.page.div(j)];
       if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;  // flagged by the selection
-      const int so = s % a.bs;
+      const int so = (int)a.page.mod(s);
       kv[i] = *reinterpret_cast<const uint4*>(a.k + sb * a.kb + so * a.kt + h * a.kh + 16 * c);
       vv[i] = *reinterpret_cast<const uint4*>(a.v + sb * a.vb + so * a.vt + h * a.vh + 16 * c);
       to_blk[i] = db;
-      to_off[i] = j % a.bs;
+      to_off[i] = (int)a.page.mod(j);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -249,8 +286,8 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const __grid
   const int32_t* kept = a.kept + ((int64_t)p.req_id[r] * a.hk + h) * a.kept_stride;
   pdl_wait();
   auto slot = [&](int pos) -> uint8_t* {
-    const int64_t blk = row[pos / a.bs];
-    return blk < 0 || blk >= a.num_blocks ? nullptr : base + blk * sb + (int64_t)(pos % a.bs) * stt;
+    const int64_t blk = row[a.page.div(pos)];
+    return blk < 0 || blk >= a.num_blocks ? nullptr : base + blk * sb + (int64_t)a.page.mod(pos) * stt;
   };
   uint4 x[2][kEvWaves];
   auto read = [&](int j0, uint4 (&y)[kEvWaves]) {

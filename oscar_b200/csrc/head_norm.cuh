@@ -9,9 +9,10 @@
 // 16 bytes each, so the mean is a butterfly over those lanes and a pair's
 // partner is in the same lane (neighbours) or rot / 16 lanes away at the same
 // position (halves): nothing goes through shared memory.  Bound by bytes: each
-// vector is read and written once.  A warp handles kHnHeads heads of one (or
-// of 256 / D) tokens with all their loads in flight; the token's cos / sin
-// stay in registers over the heads.
+// vector is read and written once.  A warp walks the heads of one token (of
+// 256 / D tokens), kHnHeads at a time with the next ones' loads in flight; the
+// token's cos / sin and the weights stay in registers.  With few tokens the
+// heads of a token are split over several warps (`splits`).
 #pragma once
 
 #include "common.cuh"
@@ -91,7 +92,7 @@ OSCAR_DEVINL void hn_load(const void* base, int64_t at, int f32, float (&x)[N]) 
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kHnThreads) head_norm_kernel(const HeadNormArgs a) {
+__global__ void __launch_bounds__(kHnThreads) head_norm_kernel(const __grid_constant__ HeadNormArgs a, const int splits) {
   constexpr int L = D / 8;     // lanes per vector
   constexpr int V = 32 / L;    // tokens per warp
   pdl_release();
@@ -100,25 +101,38 @@ __global__ void __launch_bounds__(kHnThreads) head_norm_kernel(const HeadNormArg
   const int heads = a.hq + a.hk + (a.v_cache != nullptr ? a.hk : 0);
   const int groups = (heads + kHnHeads - 1) / kHnHeads;
   const int64_t item = (int64_t)blockIdx.x * (kHnThreads / 32) + (threadIdx.x >> 5);
-  const int64_t tok = (item / groups) * V + lane / L;
-  const int h0 = (int)(item % groups) * kHnHeads;
+  const int64_t tok = (item / splits) * V + lane / L;
   const bool live = tok < a.n;
   const bool rotates = d0 < a.rot;
   pdl_wait();
   int64_t pos = live ? a.positions[tok] : 0;
   int64_t slot = live && a.slots != nullptr ? a.slots[tok] : -1;
-  uint4 raw[kHnHeads];
-#pragma unroll
-  for (int i = 0; i < kHnHeads; ++i) {
-    const int h = h0 + i;
-    raw[i] = make_uint4(0, 0, 0, 0);
-    if (live && h < heads) {
-      const T* src = h < a.hq ? reinterpret_cast<const T*>(a.q) + tok * a.q_tok + h * a.q_head
-                   : h < a.hq + a.hk ? reinterpret_cast<const T*>(a.k) + tok * a.k_tok + (h - a.hq) * a.k_head
-                                     : reinterpret_cast<const T*>(a.v) + tok * a.v_tok + (h - a.hq - a.hk) * a.v_head;
-      raw[i] = *reinterpret_cast<const uint4*>(src + d0);
-    }
+  const T *q = nullptr, *k = nullptr, *v = nullptr;
+  if (live) {
+    q = reinterpret_cast<const T*>(a.q) + tok * a.q_tok + d0;
+    k = reinterpret_cast<const T*>(a.k) + tok * a.k_tok + d0;
+    if (a.v_cache != nullptr) v = reinterpret_cast<const T*>(a.v) + tok * a.v_tok + d0;
   }
+  auto fetch = [&](int g, uint4 (&raw)[kHnHeads]) {
+#pragma unroll
+    for (int i = 0; i < kHnHeads; ++i) {
+      const int h = g * kHnHeads + i;
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if (live && h < heads) {
+        const T* src = h < a.hq ? q + h * a.q_head : h < a.hq + a.hk ? k + (h - a.hq) * a.k_head : v + (h - a.hq - a.hk) * a.v_head;
+        raw[i] = __ldcs(reinterpret_cast<const uint4*>(src));
+      }
+    }
+  };
+  int g = (int)(item % splits);
+  uint4 raw[kHnHeads];
+  fetch(g, raw);
+  // the weights of the lane's dims, with the offset
+  float wq[8], wk[8];
+  hn_load<T, 8>(a.wq, d0, a.w_f32, wq);
+  hn_load<T, 8>(a.wk, d0, a.w_f32, wk);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) wq[j] += a.offset, wk[j] += a.offset;
   const bool known = pos >= 0 && pos < a.max_pos;
   if (!known) {
     if (sub == 0 && live) flag_error(64u);
@@ -129,9 +143,7 @@ __global__ void __launch_bounds__(kHnThreads) head_norm_kernel(const HeadNormArg
     if (sub == 0) flag_error(1u);
     slot = -1;
   }
-  const int64_t blk = slot < 0 ? 0 : slot / a.bs;
-  const int64_t off = slot < 0 ? 0 : slot - blk * a.bs;
-  // cos / sin of the lane's dims: 8 pairs (halves; the lane holds one side) or 4 (neighbours)
+  // cos / sin of the lane's dims: 8 pairs (halves; the lane holds one side) or 4 (neighbours).
   float c[8], s[8];
   const int half = a.rot >> 1;
   const bool upper = !a.interleaved && d0 >= half;  // the lane holds the second member of its pairs
@@ -146,57 +158,69 @@ __global__ void __launch_bounds__(kHnThreads) head_norm_kernel(const HeadNormArg
     } else {
       hn_load<T, 8>(a.cos_sin, row + (upper ? d0 - half : d0), a.cs_f32, c);
       hn_load<T, 8>(a.cos_sin, row + half + (upper ? d0 - half : d0), a.cs_f32, s);
+      if (!upper) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = -s[j];
+      }
     }
   }
-  const int partner = upper ? lane - a.rot / 16 : lane + a.rot / 16;
+  const int partner = (upper ? lane - a.rot / 16 : lane + a.rot / 16) & 31;
+  T *ck = nullptr, *cv = nullptr;  // the token's cache rows
+  if (slot >= 0) {
+    const int64_t blk = slot <= 0x7fffffff ? (int64_t)((uint32_t)slot / (uint32_t)a.bs) : slot / a.bs;
+    const int64_t off = slot - blk * a.bs;
+    ck = reinterpret_cast<T*>(a.k_cache) + blk * a.kcb + off * a.kct + d0;
+    cv = reinterpret_cast<T*>(a.v_cache) + blk * a.vcb + off * a.vct + d0;
+  }
+  T* oq = reinterpret_cast<T*>(a.out_q) + tok * a.oq_tok + d0;
+  T* ok = a.out_k == nullptr ? nullptr : reinterpret_cast<T*>(a.out_k) + tok * a.ok_tok + d0;
+  const bool writes = live && known;
+#pragma unroll 1
+  for (; g < groups; g += splits) {
+    uint4 next[kHnHeads];
+    fetch(g + splits, next);  // (past the heads: nothing is loaded)
 #pragma unroll
-  for (int i = 0; i < kHnHeads; ++i) {
-    const int h = h0 + i;
-    if (h >= heads) break;  // uniform over the warp
-    const int kv = h - a.hq;
-    if (kv >= a.hk) {  // a value head: straight to the cache
-      if (slot >= 0)
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.v_cache) + blk * a.vcb + off * a.vct + (kv - a.hk) * a.vch + d0) =
-            raw[i];
-      continue;
-    }
-    float x[8], w[8];
-    hn_unpack<T>(raw[i], x);
-    float ss = 0.0f;
+    for (int i = 0; i < kHnHeads; ++i) {
+      const int h = g * kHnHeads + i;
+      if (h >= heads) break;  // uniform over the warp
+      const int kv = h - a.hq;
+      if (kv >= a.hk) {  // a value head: straight to the cache
+        if (cv != nullptr) *reinterpret_cast<uint4*>(cv + (kv - a.hk) * a.vch) = raw[i];
+        continue;
+      }
+      float x[8];
+      hn_unpack<T>(raw[i], x);
+      float ss = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+      for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-    hn_load<T, 8>(kv < 0 ? a.wq : a.wk, d0, a.w_f32, w);
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss * (1.0f / D) + a.eps);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (w[j] + a.offset);
-    if (a.interleaved) {
-      if (rotates) {
+      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * (kv < 0 ? wq[j] : wk[j]);
+      if (a.interleaved) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float u = x[2 * j], v = x[2 * j + 1];
-          x[2 * j] = u * c[j] - v * s[j];
-          x[2 * j + 1] = v * c[j] + u * s[j];
+          const float u = x[2 * j], w = x[2 * j + 1];
+          if (rotates) x[2 * j] = u * c[j] - w * s[j], x[2 * j + 1] = w * c[j] + u * s[j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float other = __shfl_sync(0xffffffffu, x[j], partner);
+          if (rotates) x[j] = x[j] * c[j] + other * s[j];
         }
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float other = __shfl_sync(0xffffffffu, x[j], partner & 31);
-        if (rotates) x[j] = upper ? x[j] * c[j] + other * s[j] : x[j] * c[j] - other * s[j];
+      const uint4 y = hn_pack<T>(x);
+      if (kv < 0) {
+        if (writes) *reinterpret_cast<uint4*>(oq + h * a.oq_head) = y;
+      } else {
+        if (writes && ok != nullptr) *reinterpret_cast<uint4*>(ok + kv * a.ok_head) = y;
+        if (ck != nullptr) *reinterpret_cast<uint4*>(ck + kv * a.kch) = y;
       }
     }
-    if (!live || !known) continue;
-    const uint4 y = hn_pack<T>(x);
-    if (kv < 0) {
-      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out_q) + tok * a.oq_tok + h * a.oq_head + d0) = y;
-    } else {
-      if (a.out_k != nullptr)
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out_k) + tok * a.ok_tok + kv * a.ok_head + d0) = y;
-      if (slot >= 0)
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.k_cache) + blk * a.kcb + off * a.kct + kv * a.kch + d0) = y;
-    }
+#pragma unroll
+    for (int i = 0; i < kHnHeads; ++i) raw[i] = next[i];
   }
 }
 

@@ -35,6 +35,8 @@ constexpr int kPgKeys = 64;       // keys per tile
 constexpr int kPgReqs = 256;      // requests per launch (the plan travels by value)
 constexpr int kPgWarps = 8;       // compute warps
 constexpr int kPgThreads = 32 * (kPgWarps + 1);
+constexpr int kPgCtas = 192;      // CTAs of a plan
+constexpr int kPgMerge = 4;       // warps that combine one row
 constexpr float kPgHeadroom = 8.0f;
 
 struct PagedPlan {
@@ -46,6 +48,7 @@ struct PagedPlan {
   int q_len[kPgReqs];
   int seq[kPgReqs];
   int64_t tile_begin[kPgReqs + 1];
+  int64_t cta_begin[kPgCtas + 1];  // first tile of each CTA: total_tiles * c / ctas
 };
 
 // Division by the page size without a divide (it sits in the producers' serial path, where
@@ -86,10 +89,6 @@ OSCAR_DEVINL int pg_find(const int64_t* begin, int n, int64_t x) {
   }
   return lo;
 }
-OSCAR_DEVINL int64_t pg_start(const PagedPlan& p, int64_t c) { return p.total_tiles * c / p.ctas; }
-// the CTA whose range holds tile g (every CTA has at least one tile)
-OSCAR_DEVINL int pg_cta(const PagedPlan& p, int64_t g) { return (int)(((g + 1) * p.ctas - 1) / p.total_tiles); }
-
 OSCAR_DEVINL float pg_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
@@ -278,7 +277,7 @@ paged_split_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     tc::mbar_fence_init();
   }
   __syncthreads();
-  const int64_t g0 = pg_start(p, blockIdx.x), g1 = pg_start(p, blockIdx.x + 1);
+  const int64_t g0 = p.cta_begin[blockIdx.x], g1 = p.cta_begin[blockIdx.x + 1];
   pdl_wait();
   if (warp == kPgWarps) {
     pg_produce<D, ROWS>(sm, a, p, &kmap, &vmap, g0, g1, lane);
@@ -380,7 +379,7 @@ paged_split_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
         mw[hf] = best;
         grow = grow || best > own_max(hf) + kPgHeadroom;
-        if (a.scores != nullptr) {
+        if (a.scores != nullptr && 16 * my_rt + 8 * hf + qr < u.nrows) {
           float* dst = a.scores + (g * ROWS + 16 * my_rt + 8 * hf + qr) * kPgKeys + my_key + 2 * qc;
 #pragma unroll
           for (int e = 0; e < kOwn; e += 2) *reinterpret_cast<float2*>(dst + 4 * e) = make_float2(s[hf][e], s[hf][e + 1]);
@@ -521,51 +520,50 @@ paged_split_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
   }
 }
 
-// Combine of the divided units: a warp per (query token, head) row; lane i holds
-// dims 8 i' .. of the row (D / 32 each).  O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c
-// in CTA order.  Rows of undivided units are done already.
+// Combine of the divided units: a CTA of kPgMerge warps per (query token, head)
+// row.  O = sum 2^(m_c - M) O_c / sum 2^(m_c - M) l_c; warp w takes pieces w, w + 4, ..
+// of the row in CTA order (a lane D / 32 dims), then the warps' sums are added in
+// warp order.  Rows of undivided units are done already.
 template <int D, typename T, int ROWS>
-__global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constant__ PagedArgs a,
-                                                            const __grid_constant__ PagedPlan p, int64_t rows) {
+__global__ void __launch_bounds__(32 * kPgMerge) paged_combine_kernel(const __grid_constant__ PagedArgs a,
+                                                                      const __grid_constant__ PagedPlan p) {
   constexpr int E = D / 32;
+  __shared__ float part[kPgMerge][D], part_l[kPgMerge];
   pdl_release();
-  const int lane = threadIdx.x & 31;
-  const int64_t idx = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  pdl_wait();
-  if (idx >= rows) return;
-  // rows are numbered over the plan's requests: (request, token, head)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int head = blockIdx.y, h = head / a.group;
+  // tokens are numbered from the plan's first one
+  const int tok_all = blockIdx.x + p.q_start[0];
   int lo = 0, hi = p.num_req;
-  const int64_t tok_all = idx / a.hq + p.q_start[0];
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (p.q_start[mid] <= tok_all) lo = mid; else hi = mid;
   }
   const int r = lo;
-  const int tok = (int)(tok_all - p.q_start[r]);
-  if (tok >= p.q_len[r]) return;  // a token of a request that another launch holds
-  const int head = (int)(idx % a.hq), h = head / a.group;
-  const int rr = tok * a.group + head - h * a.group;
+  const int tok = tok_all - p.q_start[r];
+  const int rr = tok * a.group + head - h * a.group, row = rr % ROWS;
   const int nt = max(1, (p.seq[r] + kPgKeys - 1) / kPgKeys);
-  const int row = rr % ROWS;
   const int64_t ub = p.tile_begin[r] + ((int64_t)(rr / ROWS) * a.hk + h) * nt;
-  const int c0 = pg_cta(p, ub), c1 = pg_cta(p, ub + nt - 1);
-  if (c0 == c1) return;
+  const int c0 = pg_find(p.cta_begin, p.ctas, ub), c1 = pg_find(p.cta_begin, p.ctas, ub + nt - 1);
+  pdl_wait();
+  // (a token of a request that another launch holds, or a row that one CTA finished)
+  if (tok >= p.q_len[r] || c0 == c1) return;
+  // the unit is the first piece of every CTA that begins inside it, else the last one
+  const bool inside = p.cta_begin[c0] >= ub;
+  auto piece = [&](int c) -> int64_t { return (int64_t)(2 * c + (c > c0 || inside ? 0 : 1)) * ROWS + row; };
   float M = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const int slot = 2 * c + (pg_start(p, c) >= ub ? 0 : 1);
-    M = fmaxf(M, a.part_ml[(int64_t)slot * ROWS + row].x);
-  }
+  for (int c = c0 + lane; c <= c1; c += 32) M = fmaxf(M, a.part_ml[piece(c)].x);
   M = warp_max(M);
   const float base = M == -INFINITY ? 0.0f : M;
   float total = 0.0f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.0f;
 #pragma unroll 4
-  for (int c = c0; c <= c1; ++c) {
-    const int slot = 2 * c + (pg_start(p, c) >= ub ? 0 : 1);
-    const float2 ml = a.part_ml[(int64_t)slot * ROWS + row];
+  for (int c = c0 + warp; c <= c1; c += kPgMerge) {
+    const int64_t at = piece(c);
+    const float2 ml = a.part_ml[at];
     const float f = pg_exp2(ml.x - base);  // a piece without visible keys: 2^-inf = 0
-    const float* src = a.part_o + ((int64_t)slot * ROWS + row) * D + E * lane;
+    const float* src = a.part_o + at * D + E * lane;
     total = fmaf(f, ml.y, total);
 #pragma unroll
     for (int i = 0; i < E; i += 2) {
@@ -574,14 +572,26 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const __grid_constan
       acc[i + 1] = fmaf(f, v.y, acc[i + 1]);
     }
   }
+#pragma unroll
+  for (int i = 0; i < E; ++i) part[warp][E * lane + i] = acc[i];
+  if (lane == 0) part_l[warp] = total;
+  __syncthreads();
+  total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kPgMerge; ++w) total += part_l[w];
   const bool empty = M == -INFINITY && total == 0.0f;
   const float inv = empty ? 0.0f : 1.0f / total;
-  const int64_t orow = tok_all * a.hq + head;
-  T* dst = reinterpret_cast<T*>(a.out) + orow * D + E * lane;
+  const int64_t orow = (int64_t)tok_all * a.hq + head;
+  if (2 * threadIdx.x < D) {
+    float2 v = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int i = 0; i < E; i += 2)
-    *reinterpret_cast<uint32_t*>(dst + i) = pack2_f32<T>(acc[i] * inv, acc[i + 1] * inv);
-  if (lane == 0) {
+    for (int w = 0; w < kPgMerge; ++w) {
+      v.x += part[w][2 * threadIdx.x];
+      v.y += part[w][2 * threadIdx.x + 1];
+    }
+    reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(a.out) + orow * D)[threadIdx.x] = pack2_f32<T>(v.x * inv, v.y * inv);
+  }
+  if (threadIdx.x == 0) {
     a.lse[orow] = empty ? -INFINITY : base * 0.69314718055994531f + logf(total);
     if (a.stats != nullptr) a.stats[orow] = make_float2(base, inv);
   }
@@ -693,7 +703,8 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
 
 // The keys' attention weights from stored scores (few query rows): a thread per
 // (key, kv head) sums exp2(s - m) / l over the observed rows.  A key of the
-// chunk itself starts from zero, an older one adds to what it has.
+// chunk itself starts from zero, an older one adds to what it has.  Bound by
+// reading the scores, 8 rows in flight per thread.
 template <int ROWS>
 __global__ void __launch_bounds__(kPgKeys) paged_mass_kernel(const __grid_constant__ PagedArgs a,
                                                              const __grid_constant__ PagedPlan p) {
@@ -702,20 +713,21 @@ __global__ void __launch_bounds__(kPgKeys) paged_mass_kernel(const __grid_consta
   const int64_t g = blockIdx.x;
   const PagedUnit u = pg_unit<ROWS>(p, a, g);
   const int key = (int)(g - u.begin) * kPgKeys + threadIdx.x;
+  const int page = key < u.seq ? (int)a.page.div(key) : 0;
   pdl_wait();
-  const int first = max(0, u.q_len - a.observe);  // first observed token
+  const int64_t blk = key < u.seq ? a.table[(int64_t)p.req_id[u.r] * a.table_stride + page] : -1;
+  const int first = max(0, u.q_len - a.observe) * a.group;  // first observed row
   for (int i = threadIdx.x; i < u.nrows; i += kPgKeys) {
     const int tok = i / a.group;
     st[i] = a.stats[(int64_t)(u.q_start + tok) * a.hq + u.h * a.group + i - tok * a.group];
   }
   __syncthreads();
-  if (key >= u.seq) return;
+  if (blk < 0 || blk >= a.num_blocks) return;  // past the request, or flagged by the attention pass
   float sum = 0.0f;
   const float* s = a.scores + g * ROWS * kPgKeys + threadIdx.x;
-  for (int i = first * a.group; i < u.nrows; ++i) sum = fmaf(pg_exp2(s[i * kPgKeys] - st[i].x), st[i].y, sum);
-  const int64_t blk = a.table[(int64_t)p.req_id[u.r] * a.table_stride + a.page.div(key)];
-  if (blk < 0 || blk >= a.num_blocks) return;  // flagged by the attention pass
-  float* w = a.weights + (blk * a.hk + u.h) * a.bs + a.page.mod(key);
+#pragma unroll 8
+  for (int i = first; i < u.nrows; ++i) sum = fmaf(pg_exp2(s[i * kPgKeys] - st[i].x), st[i].y, sum);
+  float* w = a.weights + (blk * a.hk + u.h) * a.bs + (key - page * a.bs);
   if (key < u.seq - u.q_len)
     atomicAdd(w, sum);  // requests may share a page of history
   else

@@ -60,13 +60,16 @@ namespace {
 template <typename T>
 void launch_head_norm(const oscar::HeadNormArgs& a, int d, cudaStream_t s) {
   const int heads = a.hq + a.hk + (a.v_cache != nullptr ? a.hk : 0);
-  const int64_t per = 256 / d;  // tokens per warp
-  const int64_t items = (a.n + per - 1) / per * ((heads + oscar::kHnHeads - 1) / oscar::kHnHeads);
+  const int groups = (heads + oscar::kHnHeads - 1) / oscar::kHnHeads;
   constexpr int kWarps = oscar::kHnThreads / 32;
-  const dim3 grid((unsigned)((items + kWarps - 1) / kWarps)), block(oscar::kHnThreads);
-  if (d == 256) launch_pdl(oscar::head_norm_kernel<T, 256>, grid, block, 0, s, a);
-  else if (d == 128) launch_pdl(oscar::head_norm_kernel<T, 128>, grid, block, 0, s, a);
-  else launch_pdl(oscar::head_norm_kernel<T, 64>, grid, block, 0, s, a);
+  const int64_t tokens = (a.n + 256 / d - 1) / (256 / d);  // warps that hold whole tokens
+  // enough warps to fill the SMs (16 each), at most one per group of heads
+  const int64_t want = (int64_t)std::max(device_info().sms, 1) * 16;
+  const int splits = (int)std::min<int64_t>(groups, std::max<int64_t>(1, (want + tokens - 1) / tokens));
+  const dim3 grid((unsigned)((tokens * splits + kWarps - 1) / kWarps)), block(oscar::kHnThreads);
+  if (d == 256) launch_pdl(oscar::head_norm_kernel<T, 256>, grid, block, 0, s, a, splits);
+  else if (d == 128) launch_pdl(oscar::head_norm_kernel<T, 128>, grid, block, 0, s, a, splits);
+  else launch_pdl(oscar::head_norm_kernel<T, 64>, grid, block, 0, s, a, splits);
 }
 
 }  // namespace
@@ -246,7 +249,8 @@ int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const
   }
   p.tile_begin[p.num_req] = tiles;
   p.total_tiles = tiles;
-  p.ctas = (int)std::min<int64_t>(std::max(sms, 1), tiles);
+  p.ctas = (int)std::min<int64_t>(std::min(std::max(sms, 1), oscar::kPgCtas), tiles);
+  for (int c = 0; c <= p.ctas; ++c) p.cta_begin[c] = tiles * c / p.ctas;
   return r;
 }
 
@@ -361,18 +365,17 @@ int launch_split(const PagedCall& c, const PagedBatch& b) {
              c.vmap);
   int st = cuda_status("paged_split_kernel");
   if (st) return st;
-  bool divided = false;
-  for (int i = 0; i < p.num_req && !divided; ++i) {
-    // a unit of request i lies in one CTA's range unless a range begins inside it
+  bool divided = false;  // does a CTA begin inside a unit?
+  for (int i = 0, c = 0; i < p.num_req && !divided; ++i) {
     const int64_t nt = std::max<int64_t>(1, ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys);
-    for (int64_t u = p.tile_begin[i]; u < p.tile_begin[i + 1] && !divided; u += nt)
-      divided = ((u + 1) * p.ctas - 1) / p.total_tiles != ((u + nt) * p.ctas - 1) / p.total_tiles;
+    for (; c < p.ctas && p.cta_begin[c] < p.tile_begin[i + 1] && !divided; ++c)
+      divided = (p.cta_begin[c] - p.tile_begin[i]) % nt != 0;
   }
   if (divided) {
     const int last = p.num_req - 1;
-    const int64_t rows = ((int64_t)p.q_start[last] + p.q_len[last] - p.q_start[0]) * a.hq;
-    launch_pdl(oscar::paged_combine_kernel<D, T, 16 * NRT>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, c.stream, a,
-               p, rows);
+    const int tokens = p.q_start[last] + p.q_len[last] - p.q_start[0];
+    launch_pdl(oscar::paged_combine_kernel<D, T, 16 * NRT>, dim3((unsigned)tokens, (unsigned)a.hq),
+               dim3(32 * oscar::kPgMerge), 0, c.stream, a, p);
     st = cuda_status("paged_combine_kernel");
     if (st) return st;
   }
@@ -568,6 +571,7 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
   a.vb = 2 * v_stride_block, a.vt = 2 * v_stride_token, a.vh = 2 * v_stride_head;
   a.weights = weights;
   a.num_blocks = num_blocks, a.bs = block_size, a.hk = num_kv_heads;
+  a.page = fast_div((uint32_t)block_size);
   a.row_bytes = 2 * head_dim;
   a.table = block_table, a.table_stride = bt_stride;
   a.dst = in_place ? block_table : dst_table, a.dst_stride = in_place ? bt_stride : dst_stride;
@@ -580,7 +584,7 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
     for (; r < num_requests && p.num_req < oscar::kEvReqs; ++r) {
       p.req_id[p.num_req] = r;
       p.seq[p.num_req++] = seqs[r];
-      if (seqs[r] <= oscar::kEvCached) longest = std::max(longest, seqs[r]);
+      longest = std::max(longest, std::min(seqs[r], oscar::kEvCached));
       moved = std::max(moved, std::min(seqs[r], keep));
     }
     allow_smem<oscar::evict_select_kernel>(oscar::kEvCached * sizeof(float));
