@@ -478,8 +478,9 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
     return fail(OSCAR_ERR_INVALID, "paged_attention: a sequence needs caches and a block table");
   if (n_tokens == 0) return OSCAR_OK;
   if (!q || !out || !lse) return fail(OSCAR_ERR_INVALID, "paged_attention: null pointer");
-  if (!aligned16(q) || !aligned16(out) || !aligned16(workspace) || (q_token_stride | q_head_stride) % 8)
-    return fail(OSCAR_ERR_INVALID, "paged_attention: query rows, output and workspace must be 16-byte aligned");
+  if (!aligned16(q) || (reinterpret_cast<uintptr_t>(out) & 31) || (reinterpret_cast<uintptr_t>(workspace) & 31) ||
+      (q_token_stride | q_head_stride) % 8)
+    return fail(OSCAR_ERR_INVALID, "paged_attention: query rows must be 16-byte, output and workspace 32-byte aligned");
   PagedCall c{};
   oscar::PagedArgs& a = c.args;
   a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;

@@ -38,8 +38,13 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# the current stream's handle without a Stream object (0.1 instead of 2.3 us a call) where torch offers it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(torch.cuda.current_device() if device.index is None else device.index)
 
 
 def _require_cuda(*tensors: torch.Tensor | None) -> torch.device:
@@ -404,35 +409,57 @@ def merge_slab(output, lse, part, part_lse, start, ids) -> None:
 
 # ---------------------------------------------------------------------------
 # the 16-bit paged layer
-def _rows16(t: torch.Tensor) -> torch.Tensor:
+_HALF = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
+
+
+def _cuda_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The one CUDA device of the tensors (as _require_cuda, for calls whose host time counts)."""
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            _require_cuda(first, *others)
+    if index < 0:
+        _require_cuda(first)
+    return index
+
+
+def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
     """[n, heads, D] with contiguous, 16-byte aligned head vectors (a copy of t where its layout has none)."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    if stride[2] != 1 or (stride[0] | stride[1]) % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
-def _cache16(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, hk: int, d: int) -> None:
-    for t in (k_cache, v_cache):
-        if t.ndim != 4 or t.shape[2] != hk or t.shape[3] != d or t.shape != k_cache.shape:
-            raise ValueError(f"{name}: caches must be [blocks, tokens, {hk}, {d}] and alike")
-        if t.dtype != dtype:
-            raise ValueError(f"{name}: the caches must have the heads' type {dtype}, got {t.dtype}")
-        if t.stride(3) != 1:
-            raise ValueError(f"{name}: cache rows must be contiguous in the last dim")
+def _cache16(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, hk: int, d: int) -> tuple:
+    """Strides of the two caches, [blocks, tokens, hk, d] of `dtype` with contiguous rows."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or shape[2] != hk or shape[3] != d:
+        raise ValueError(f"{name}: caches must be [blocks, tokens, {hk}, {d}] and alike")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError(f"{name}: the caches must have the heads' type {dtype}, got {k_cache.dtype} and {v_cache.dtype}")
+    if ks[3] != 1 or vs[3] != 1:
+        raise ValueError(f"{name}: cache rows must be contiguous in the last dim")
+    return ks, vs
 
 
 def _host_ints(values) -> np.ndarray:
+    if type(values) is np.ndarray and values.dtype == np.int32 and values.flags.c_contiguous:
+        return values
     if isinstance(values, torch.Tensor):
         values = values.cpu().numpy()
     return np.ascontiguousarray(values, dtype=np.int32)
 
 
-def _table32(name: str, table: torch.Tensor, dev: torch.device) -> torch.Tensor:
+def _table32(name: str, table: torch.Tensor) -> torch.Tensor:
     if table.ndim != 2:
         raise ValueError(f"{name}: the block table must be [requests, pages]")
     if table.dtype != torch.int32:
         table = table.to(torch.int32)
     return table if table.stride(1) == 1 else table.contiguous()
+
+
+def _long(t: torch.Tensor) -> torch.Tensor:
+    return t if t.dtype == torch.int64 and t.is_contiguous() else t.to(torch.int64).contiguous()
 
 
 def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight_offset: float = 0.0,
@@ -449,57 +476,64 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
     back (v is not needed); with them k and v go to ``slot_mapping`` (slots
     < 0 are skipped) and the keys come back only into a given ``out_k``.
     Returns (out_q, out_k)."""
-    if q.ndim != 3 or k.ndim != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or k.dtype != q.dtype:
+    q_shape, k_shape, dtype = q.shape, k.shape, q.dtype
+    if len(q_shape) != 3 or len(k_shape) != 3 or k_shape[0] != q_shape[0] or k_shape[2] != q_shape[2] or k.dtype != dtype:
         raise ValueError("qk_norm_rope: q [n, Hq, D] and k [n, Hk, D] of one type are needed")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"qk_norm_rope: unsupported type {q.dtype}")
-    n, hq, d = q.shape
-    hk = k.shape[1]
+    code = _HALF.get(dtype)
+    if code is None:
+        raise ValueError(f"qk_norm_rope: unsupported type {dtype}")
+    n, hq, d = q_shape
+    hk = k_shape[1]
     write = k_cache is not None
     if write != (v_cache is not None) or write != (slot_mapping is not None) or (write and v is None):
         raise ValueError("qk_norm_rope: v, caches and slot_mapping come together")
-    dev = _require_cuda(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, slot_mapping, out_q, out_k)
-    if q_weight.shape != (d,) or k_weight.shape != (d,) or q_weight.dtype != k_weight.dtype:
+    index = _cuda_index(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, slot_mapping, out_q, out_k)
+    w_dtype, cs_dtype, cs_shape = q_weight.dtype, cos_sin.dtype, cos_sin.shape
+    if q_weight.shape != (d,) or k_weight.shape != (d,) or w_dtype != k_weight.dtype:
         raise ValueError(f"qk_norm_rope: the weights must be two [{d}] tensors of one type")
-    if cos_sin.ndim != 2 or positions.ndim != 1 or positions.shape[0] != n:
+    if len(cs_shape) != 2 or positions.shape != (n,):
         raise ValueError("qk_norm_rope: cos_sin [max_positions, rot] and positions [n] are needed")
-    for t in (q_weight, cos_sin):
-        if t.dtype not in (torch.float32, q.dtype):
-            raise ValueError("qk_norm_rope: weights and cos_sin must be fp32 or of the heads' type")
-    q, k = _rows16(q), _rows16(k)
-    q_weight, k_weight = q_weight.contiguous(), k_weight.contiguous()
-    cos_sin = cos_sin if cos_sin.stride(1) == 1 and cos_sin.stride(0) % 8 == 0 else cos_sin.contiguous()
-    positions = positions.to(torch.int64).contiguous()
+    if (w_dtype != torch.float32 and w_dtype != dtype) or (cs_dtype != torch.float32 and cs_dtype != dtype):
+        raise ValueError("qk_norm_rope: weights and cos_sin must be fp32 or of the heads' type")
+    qt, kt, ct = q.stride(), k.stride(), cos_sin.stride()
+    q, k = _rows16(q, qt), _rows16(k, kt)
+    qt, kt = q.stride(), k.stride()
+    q_weight, k_weight, positions = q_weight.contiguous(), k_weight.contiguous(), _long(positions)
+    if ct[1] != 1 or ct[0] % 8:
+        cos_sin = cos_sin.contiguous()
+        ct = cos_sin.stride()
     if out_q is None:
-        out_q = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
-    if out_k is None and not write:
-        out_k = torch.empty(n, hk, d, dtype=q.dtype, device=dev)
-    for t, heads in ((out_q, hq), (out_k, hk)):
-        if t is not None and (t.shape != (n, heads, d) or t.dtype != q.dtype or t.stride(2) != 1):
-            raise ValueError(f"qk_norm_rope: outputs must be [{n}, {heads}, {d}] rows of {q.dtype}")
+        out_q = torch.empty(q_shape, dtype=dtype, device=q.device)
+    elif out_q.shape != q_shape or out_q.dtype != dtype or out_q.stride(2) != 1:
+        raise ValueError(f"qk_norm_rope: out_q must be {list(q_shape)} rows of {dtype}")
+    if out_k is None:
+        if not write:
+            out_k = torch.empty(k_shape, dtype=dtype, device=q.device)
+    elif out_k.shape != k_shape or out_k.dtype != dtype or out_k.stride(2) != 1:
+        raise ValueError(f"qk_norm_rope: out_k must be {list(k_shape)} rows of {dtype}")
     nb = bs = 1
-    ks = vs = (d, d, d)
-    vt = (0, 0)
+    ks = vs = vt = (0, 0, 0)
+    kc_p = vc_p = v_p = slots_p = ok_p = None
     if write:
-        if v.shape != k.shape or v.dtype != q.dtype:
+        if v.shape != k_shape or v.dtype != dtype:
             raise ValueError("qk_norm_rope: v must match k")
-        v = _rows16(v)
+        v = _rows16(v, v.stride())
         vt = v.stride()
-        _cache16("qk_norm_rope", k_cache, v_cache, q.dtype, hk, d)
+        ks, vs = _cache16("qk_norm_rope", k_cache, v_cache, dtype, hk, d)
         nb, bs = k_cache.shape[:2]
-        ks, vs = k_cache.stride(), v_cache.stride()
-        slot_mapping = slot_mapping.to(torch.int64).contiguous()
+        slot_mapping = _long(slot_mapping)
         if slot_mapping.numel() < n:
             raise ValueError("slot_mapping shorter than the token count")
-    qt, kt, oq = q.stride(), k.stride(), out_q.stride()
-    ok = (0, 0) if out_k is None else out_k.stride()
+        kc_p, vc_p, v_p, slots_p = k_cache.data_ptr(), v_cache.data_ptr(), v.data_ptr(), slot_mapping.data_ptr()
+    oq, ok = out_q.stride(), (0, 0)
+    if out_k is not None:
+        ok, ok_p = out_k.stride(), out_k.data_ptr()
     check(_native.lib().oscar_qk_norm_rope(
-        q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], _ptr(v) if write else None, vt[0], vt[1],
-        _DTYPES[q.dtype], n, hq, hk, d, q_weight.data_ptr(), k_weight.data_ptr(), _DTYPES[q_weight.dtype], float(eps),
-        float(weight_offset), cos_sin.data_ptr(), _DTYPES[cos_sin.dtype], cos_sin.stride(0), cos_sin.shape[0],
-        cos_sin.shape[1], 1 if interleaved else 0, positions.data_ptr(), out_q.data_ptr(), oq[0], oq[1], _ptr(out_k),
-        ok[0], ok[1], _ptr(k_cache), _ptr(v_cache), nb, bs, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        _ptr(slot_mapping), _stream(dev)))
+        q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v_p, vt[0], vt[1], code, n, hq, hk, d,
+        q_weight.data_ptr(), k_weight.data_ptr(), _DTYPES[w_dtype], eps, weight_offset, cos_sin.data_ptr(),
+        _DTYPES[cs_dtype], ct[0], cs_shape[0], cs_shape[1], 1 if interleaved else 0, positions.data_ptr(),
+        out_q.data_ptr(), oq[0], oq[1], ok_p, ok[0], ok[1], kc_p, vc_p, nb, bs, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        slots_p, _raw_stream(index)))
     return out_q, out_k
 
 
@@ -517,41 +551,44 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
     every cached key, summed over the heads of its group and the last
     ``observe`` tokens of each request (None: all): keys older than the chunk
     add it to what they have, the chunk's own keys start from it."""
-    if q.ndim != 3 or k_cache.ndim != 4 or k_cache.shape[2] < 1 or q.shape[1] % k_cache.shape[2]:
+    q_shape, c_shape, dtype = q.shape, k_cache.shape, q.dtype
+    if len(q_shape) != 3 or len(c_shape) != 4 or c_shape[2] < 1 or q_shape[1] % c_shape[2]:
         raise ValueError("paged_attention: q [n, Hq, D] with Hq a multiple of the caches' heads is needed")
-    if q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"paged_attention: unsupported query type {q.dtype}")
-    n, hq, d = q.shape
-    nb, bs, hk = k_cache.shape[:3]
-    dev = _require_cuda(q, k_cache, v_cache, table, weights, out)
-    _cache16("paged_attention", k_cache, v_cache, q.dtype, hk, d)
+    code = _HALF.get(dtype)
+    if code is None:
+        raise ValueError(f"paged_attention: unsupported query type {dtype}")
+    n, hq, d = q_shape
+    nb, bs, hk = c_shape[:3]
+    index = _cuda_index(q, k_cache, v_cache, table, weights, out)
+    ks, vs = _cache16("paged_attention", k_cache, v_cache, dtype, hk, d)
     qsl_a, seqs_a = _host_ints(qsl), _host_ints(seqs)
     if qsl_a.ndim != 1 or seqs_a.ndim != 1 or qsl_a.size != seqs_a.size + 1 or qsl_a[0] != 0 or qsl_a[-1] != n:
         raise ValueError("paged_attention: invalid query layout")
-    table = _table32("paged_attention", table, dev)
+    table = _table32("paged_attention", table)
     if weights is not None and (weights.shape != (nb, hk, bs) or weights.dtype != torch.float32
                                 or not weights.is_contiguous()):
         raise ValueError(f"paged_attention: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")
     if observe is not None and (weights is None or int(observe) < 1):
         raise ValueError("paged_attention: observe needs weights and at least one token")
-    q = _rows16(q)
+    q = _rows16(q, q.stride())
+    dev = q.device
     if out is None:
-        out = torch.empty(n, hq, d, dtype=q.dtype, device=dev)
-    elif out.shape != (n, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError(f"paged_attention: out must be contiguous [{n}, {hq}, {d}] of {q.dtype}")
-    lse = torch.empty(n, hq, dtype=torch.float32, device=dev)
+        out = torch.empty(q_shape, dtype=dtype, device=dev)
+    elif out.shape != q_shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 32:
+        raise ValueError(f"paged_attention: out must be contiguous, 32-byte aligned {list(q_shape)} of {dtype}")
+    lse = torch.empty((n, hq), dtype=torch.float32, device=dev)
     lib = _native.lib()
     qsl_p, seqs_p, b = qsl_a.ctypes.data, seqs_a.ctypes.data, seqs_a.size
     need = lib.oscar_paged_attention_workspace(qsl_p, seqs_p, b, hq, hk, d, 0 if weights is None else 1)
     if need < 0:
         check(_native.ERR_INVALID)
     ws = torch.empty(max(need, 16), dtype=torch.uint8, device=dev)
-    ks, vs, qs = k_cache.stride(), v_cache.stride(), q.stride()
+    qs, (rows, cols), ts = q.stride(), table.shape, table.stride()
     check(lib.oscar_paged_attention(
-        q.data_ptr(), qs[0], qs[1], _DTYPES[q.dtype], n, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs,
-        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.data_ptr(), table.shape[0], table.shape[1], table.stride(0),
-        qsl_p, seqs_p, b, float(scale), _ptr(weights), 0x7FFFFFFF if observe is None else min(int(observe), 0x7FFFFFFF),
-        out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, _stream(dev)))
+        q.data_ptr(), qs[0], qs[1], code, n, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, ks[0], ks[1],
+        ks[2], vs[0], vs[1], vs[2], table.data_ptr(), rows, cols, ts[0], qsl_p, seqs_p, b, scale,
+        None if weights is None else weights.data_ptr(), 0x7FFFFFFF if observe is None else min(int(observe), 0x7FFFFFFF),
+        out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, _raw_stream(index)))
     return out, lse
 
 
@@ -564,28 +601,31 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     with other requests, which must not be overwritten).  ``seqs``: host list.
     Returns the kept positions [requests, Hk, min(keep, max(seqs))] int32 (-1
     past a request's list); the new lengths are min(seqs, keep)."""
-    if k_cache.ndim != 4:
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4:
         raise ValueError("evict_cache: caches must be [blocks, tokens, heads, D]")
-    nb, bs, hk, d = k_cache.shape
-    if k_cache.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"evict_cache: unsupported cache type {k_cache.dtype}")
-    dev = _require_cuda(k_cache, v_cache, weights, table, dst_table)
-    _cache16("evict_cache", k_cache, v_cache, k_cache.dtype, hk, d)
+    nb, bs, hk, d = shape
+    if dtype not in _HALF:
+        raise ValueError(f"evict_cache: unsupported cache type {dtype}")
+    index = _cuda_index(k_cache, v_cache, weights, table, dst_table)
+    ks, vs = _cache16("evict_cache", k_cache, v_cache, dtype, hk, d)
     if weights.shape != (nb, hk, bs) or weights.dtype != torch.float32 or not weights.is_contiguous():
         raise ValueError(f"evict_cache: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")
     seqs_a = _host_ints(seqs)
     if seqs_a.ndim != 1:
         raise ValueError("evict_cache: seqs must be a list of lengths")
-    table = _table32("evict_cache", table, dev)
-    dst = None if dst_table is None else _table32("evict_cache", dst_table, dev)
-    cols = max(0, min(int(keep), int(seqs_a.max(initial=0))))
-    kept = torch.empty(seqs_a.size, hk, cols, dtype=torch.int32, device=dev)
-    ks, vs = k_cache.stride(), v_cache.stride()
+    table = _table32("evict_cache", table)
+    rows, cols = table.shape
+    dst_p, dst_rows, dst_cols, dst_stride = None, 0, 0, 0
+    if dst_table is not None:
+        dst = _table32("evict_cache", dst_table)
+        dst_p, (dst_rows, dst_cols), dst_stride = dst.data_ptr(), dst.shape, dst.stride(0)
+    places = max(0, min(int(keep), int(seqs_a.max(initial=0))))
+    kept = torch.empty((seqs_a.size, hk, places), dtype=torch.int32, device=k_cache.device)
     check(_native.lib().oscar_evict_cache(
         k_cache.data_ptr(), v_cache.data_ptr(), d, nb, bs, hk, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        weights.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1], table.stride(0), _ptr(dst),
-        0 if dst is None else dst.shape[0], 0 if dst is None else dst.shape[1], 0 if dst is None else dst.stride(0),
-        seqs_a.ctypes.data, seqs_a.size, int(keep), int(sink), int(recent), kept.data_ptr(), cols, _stream(dev)))
+        weights.data_ptr(), table.data_ptr(), rows, cols, table.stride(0), dst_p, dst_rows, dst_cols, dst_stride,
+        seqs_a.ctypes.data, seqs_a.size, int(keep), int(sink), int(recent), kept.data_ptr(), places, _raw_stream(index)))
     return kept
 
 
