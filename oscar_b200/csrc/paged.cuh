@@ -152,28 +152,19 @@ OSCAR_DEVINL uint32_t pg_swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (
 // for up to a millisecond a try: polls take shared-memory cycles from the
 // tensor cores' operands (2570 against 2430 us on the longest chunk).
 constexpr uint32_t kPgTries = 4096;
-template <bool kCluster = false>
 OSCAR_DEVINL bool pg_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
-  if constexpr (kCluster)
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, "
-        "1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(1000000u)
-        : "memory");
-  else
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity), "r"(1000000u)
-        : "memory");
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity), "r"(1000000u)
+      : "memory");
   return ok != 0;
 }
-template <bool kCluster = false>
 OSCAR_DEVINL bool pg_wait(int& abort, uint32_t bar, uint32_t parity) {
+  if (tc::mbar_test(bar, parity)) return true;
   for (uint32_t i = 0; i < kPgTries; ++i) {
-    if (pg_try<kCluster>(bar, parity)) return true;
+    if (pg_try(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(&abort) != 0) return false;
   }
   *reinterpret_cast<volatile int*>(&abort) = 1;

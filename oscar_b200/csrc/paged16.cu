@@ -182,33 +182,48 @@ struct PagedBatch {
   int num() const { return cls == kChunk ? chunk.num_req : plan.num_req; }
 };
 
+// Divides the tiles of all units over the workers.  A unit costs its tiles and
+// kUnitCost more (queries, first products, epilogue: about 9000 cycles against
+// 4100 a tile at D 128 and 7000 against 2600 at D 256, from clock traces), so that
+// short units are not piled on one worker.
 template <int D>
 void plan_chunk(PagedBatch& b, int hk, int sms) {
+  constexpr int kUnitCost = 2;
   oscar::PcPlan& p = b.chunk;
   const int per = p.tokens * oscar::kPcUnit;
   int64_t total = 0;
   for (int i = 0; i < p.num_req; ++i)
     for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb)
-      total += (int64_t)hk * oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb);
-  const int workers = oscar::PcShape<D>::kPair ? sms / 2 : sms;
-  p.ctas = (int)std::min<int64_t>(std::min(std::max(workers, 1), oscar::kPcCtas), total);
+      total += (int64_t)hk * (kUnitCost + oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb));
+  const int workers = std::min(std::max(oscar::PcShape<D>::kPair ? sms / 2 : sms, 1), oscar::kPcCtas);
+  p.ctas = 0;
   b.splits.n = 0;
-  int64_t at = 0;  // tiles before the unit
-  int c = 0;       // CTAs begun
-  auto start_of = [&](int64_t i) { return total * i / p.ctas; };
+  int64_t cost = 0;  // of the units before
+  int next = 0;      // the next worker to begin, at cost total * next / workers
+  auto begin_of = [&](int w) { return total * w / workers; };
   for (int i = 0; i < p.num_req; ++i)
     for (int h = 0; h < hk; ++h)
       for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb) {
         const int nt = oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb);
-        const bool at_start = c < p.ctas && start_of(c) == at;
-        const int first = at_start ? c : c - 1;  // the CTA that holds the unit's first tile
-        while (c < p.ctas && start_of(c) < at + nt) {
-          p.start[c] = oscar::PcStart{i, h, qb, (int)(start_of(c) - at)};
-          p.tiles[c] = (int)(start_of(c + 1) - start_of(c));
-          ++c;
+        const int holder = p.ctas - 1;  // the worker that reaches the unit, if none begins with it
+        int done = 0;                   // tiles of the unit before the current worker
+        bool begun = false;             // does a worker begin with the unit's first tile?
+        while (next < workers && begin_of(next) < cost + kUnitCost + nt) {
+          // a share that begins in a unit's fixed cost begins with its first tile; two that begin
+          // at the same tile are one
+          const int t = (int)std::max<int64_t>(0, begin_of(next) - cost - kUnitCost);
+          ++next;
+          if (t < done || (t == done && (begun || (done > 0)))) continue;
+          if (p.ctas > 0) p.tiles[p.ctas - 1] += t - done;
+          begun = begun || t == 0;
+          done = t;
+          p.start[p.ctas] = oscar::PcStart{i, h, qb, t};
+          p.tiles[p.ctas++] = 0;
         }
-        if (c - 1 > first) b.splits.unit[b.splits.n++] = oscar::PcSplit{i, h, qb, first, c - 1};
-        at += nt;
+        p.tiles[p.ctas - 1] += nt - done;
+        const int first = begun ? holder + 1 : holder;
+        if (p.ctas - 1 > first) b.splits.unit[b.splits.n++] = oscar::PcSplit{i, h, qb, first, p.ctas - 1};
+        cost += kUnitCost + nt;
       }
 }
 

@@ -291,13 +291,6 @@ OSCAR_DEVINL void pc_transpose8(uint32_t (&x)[8][4], int lane) {
     }
   }
 }
-// 32 bytes (a whole sector) to a 32-byte aligned address
-OSCAR_DEVINL void pc_store32(void* dst, const uint32_t* x) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]),
-               "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7])
-               : "memory");
-}
-
 template <int D, typename T>
 __global__ void __launch_bounds__(PcShape<D>::kThreads, 1)
 paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PcPlan p,
@@ -382,22 +375,32 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const uint32_t s_col = tmem + lanes + 128 * b;
         if (!wait(smem_u32(&sm.s_full[b]), (job >> 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
-        // the row's scores stay in registers over both passes
+        // D 256: the row's scores stay in registers over both passes.  D <= 128 (eleven warps, 168
+        // registers): chunks of 32 columns, read twice (103 against 115 us on ragged chunks at D 128;
+        // at D 256 2140 against 2025 us on the longest one)
+        constexpr int kChunk = kPair ? kPcKeys : 32;
         const int vis = lim - t * kPcKeys;  // keys c < vis are visible
-        uint32_t s[kPcKeys];
+        const bool masked = __any_sync(0xffffffffu, vis < kPcKeys);
+        uint32_t s[kChunk];
+        auto load_scores = [&](int c0) {
 #pragma unroll
-        for (int c = 0; c < kPcKeys; c += 32) tc::tmem_ld32(s_col + c, s + c);
-        tc::tmem_wait_ld();
-        if (__any_sync(0xffffffffu, vis < kPcKeys)) {
+          for (int c = 0; c < kChunk; c += 32) tc::tmem_ld32(s_col + c0 + c, s + c);
+          tc::tmem_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int c = 0; c < kPcKeys; ++c) s[c] = c < vis ? s[c] : 0xff800000u;
-        }
+            for (int c = 0; c < kChunk; ++c) s[c] = c0 + c < vis ? s[c] : 0xff800000u;
+          }
+        };
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPcKeys; c0 += kChunk) {
+          load_scores(c0);
 #pragma unroll
-        for (int c = 0; c < kPcKeys; c += 8)
+          for (int c = 0; c < kChunk; c += 8)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
+            for (int i = 0; i < 4; ++i)
+              m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
+        }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
         const bool grow = mx > m + kPgHeadroom;
         const bool rescale = grow && m != -INFINITY;
@@ -421,17 +424,22 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         }
         const float base = m == -INFINITY ? 0.0f : -m;
         const uint64_t scale2 = f2_pack(scale, scale), base2 = f2_pack(base, base);
+#pragma unroll 1
+        for (int c0 = 0; c0 < kPcKeys; c0 += kChunk) {
+          // (the columns P overwrites, [c0 / 2, c0 / 2 + 16), have been read)
+          if (kChunk < kPcKeys) load_scores(c0);
 #pragma unroll
-        for (int c = 0; c < kPcKeys; c += 32) {
-          uint32_t pk[16];
+          for (int c = 0; c < kChunk; c += 32) {
+            uint32_t pk[16];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
-            const float e0 = pg_exp2(f2_lo(x)), e1 = pg_exp2(f2_hi(x));
-            l2 = f2_add(l2, f2_pack(e0, e1));
-            pk[i] = pc_pack<T>(e0, e1);
+            for (int i = 0; i < 16; ++i) {
+              const uint64_t x = f2_fma(f2_pack(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
+              const float e0 = pg_exp2(f2_lo(x)), e1 = pg_exp2(f2_hi(x));
+              l2 = f2_add(l2, f2_pack(e0, e1));
+              pk[i] = pc_pack<T>(e0, e1);
+            }
+            tc::tmem_st16(s_col + (c0 + c) / 2, pk);
           }
-          tc::tmem_st16(s_col + c / 2, pk);
         }
         tc::tmem_wait_st();
         tc::tc_fence_before();
@@ -455,42 +463,37 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       const int head = w.h * a.group + row % a.group;
       const int64_t orow = (int64_t)(p.q_start[w.r] + tok) * a.hq + head;
       const int64_t prow = ((int64_t)(2 * worker + (w.piece == 0 ? 0 : 1)) * kPcUnit + rt) * kPcRows + row;
-      if (whole) {
-        // 64 columns at a time: a row's 128 bytes lie in one lane, and 8 lanes exchange 16-byte pieces
-        // so that a store instruction writes whole lines of 4 rows (32 lines of one sector each took
-        // 9400 cycles a unit)
-        const int64_t my_row = live ? orow : -1;
+      // 128 bytes of a row at a time lie in one lane; 8 lanes exchange 16-byte pieces so that a store
+      // instruction writes whole lines of 4 rows (32 lines of one sector each took 9400 cycles a unit)
+      const int64_t my_row = !live ? -1 : whole ? orow : prow;
+      const int step = whole ? 64 : 32;  // columns per 128 bytes
 #pragma unroll 1
-        for (int c = 0; c < D; c += 64) {
-          uint32_t o[32], x[8][4];
+      for (int c = 0; c < D; c += step) {
+        uint32_t x[8][4];
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            tc::tmem_ld32(o_col + c + 32 * hf, o);
-            tc::tmem_wait_ld();
+        for (int hf = 0; hf < 2; ++hf) {
+          if (hf == 1 && !whole) break;
+          uint32_t o[32];
+          tc::tmem_ld32(o_col + c + 32 * hf, o);
+          tc::tmem_wait_ld();
+          if (whole) {
 #pragma unroll
             for (int i = 0; i < 16; ++i)
               x[4 * hf + i / 4][i % 4] = pc_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-          }
-          pc_transpose8(x, lane);
+          } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const int64_t to = __shfl_sync(0xffffffffu, my_row, (lane & 24) + k);
-            if (to >= 0)
-              *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.out) + to * D + c + 8 * (lane & 7)) =
-                  make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
+            for (int i = 0; i < 32; ++i) x[i / 4][i % 4] = o[i];
           }
         }
-      } else {
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tc::tmem_ld32(o_col + c, o);
-          tc::tmem_wait_ld();
-          if (live) {
+        pc_transpose8(x, lane);
+        uint8_t* dst = whole ? reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + c)
+                             : reinterpret_cast<uint8_t*>(a.part_o + c);
+        const int64_t row_bytes = D * (whole ? 2 : 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) pc_store32(a.part_o + prow * D + c + 8 * i, o + 8 * i);
-          }
-          __syncwarp();
+        for (int k = 0; k < 8; ++k) {
+          const int64_t to = __shfl_sync(0xffffffffu, my_row, (lane & 24) + k);
+          if (to >= 0)
+            *reinterpret_cast<uint4*>(dst + to * row_bytes + 16 * (lane & 7)) = make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
         }
       }
       if (live) {
