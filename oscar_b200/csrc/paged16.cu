@@ -10,7 +10,8 @@
 #include "head_norm.cuh"
 #include "host.h"
 #include "paged.cuh"
-#include "paged_chunk.cuh"
+#include "paged_attn.cuh"
+#include "paged_mma.cuh"
 
 namespace oscar_host {
 
@@ -153,16 +154,17 @@ extern "C" int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t
 // ---------------------------------------------------------------------------
 namespace {
 
-constexpr int kFewRows = 32;  // query rows of a (request, kv head) in one block of the split kernel
-
-// How a request's new tokens are attended: kFew in one block of the split
-// kernel, kChunk on the tensor-memory kernel, kWide (a group of more than 128
-// heads) in several blocks of the split kernel.
-enum PagedClass { kFew = 0, kChunk = 1, kWide = 2, kClasses = 3 };
+// How a request's new tokens are attended.  kFew: at most 32 query rows per kv
+// head, one row tile, scores stored where the keys are weighed.  kOne: one row
+// tile.  kChunk: q-blocks of two row tiles.
+enum PagedClass { kFew = 0, kOne = 1, kChunk = 2, kClasses = 3 };
 inline PagedClass paged_class(int64_t len, int group) {
-  if (len * group <= kFewRows) return kFew;
-  return group <= oscar::kPcRows ? kChunk : kWide;
+  if (len * group <= oscar::kPgFewRows) return kFew;
+  return len <= oscar::kPcRows / group ? kOne : kChunk;
 }
+
+// kFew runs on mma.sync up to this many 64-key tiles per SM (paged_mma.cuh has both sides)
+constexpr int64_t kMmaTiles = 32;
 
 // Workspace of one launch, in this order.
 struct PagedSpace {
@@ -175,36 +177,37 @@ inline int64_t round256(int64_t x) { return (x + 255) & ~(int64_t)255; }
 // class.  Returns the index after the last one looked at.
 struct PagedBatch {
   PagedClass cls;
-  oscar::PagedPlan plan;   // kFew, kWide
-  int rows;                // rows per block of the split kernel
-  oscar::PcPlan chunk;     // kChunk
+  int64_t tiles;
+  int pieces;              // most pieces of a divided unit
+  oscar::PcPlan plan;
   oscar::PcSplits splits;  // its divided units
-  int num() const { return cls == kChunk ? chunk.num_req : plan.num_req; }
 };
 
 // Divides the tiles of all units over the workers.  A unit costs its tiles and
 // kUnitCost more (queries, first products, epilogue: about 9000 cycles against
 // 4100 a tile at D 128 and 7000 against 2600 at D 256, from clock traces), so that
 // short units are not piled on one worker.
-template <int D>
-void plan_chunk(PagedBatch& b, int hk, int sms) {
+template <typename Shape>
+void plan_units(PagedBatch& b, int hk, int sms) {
   constexpr int kUnitCost = 2;
-  oscar::PcPlan& p = b.chunk;
-  const int per = p.tokens * oscar::kPcUnit;
+  oscar::PcPlan& p = b.plan;
+  const int64_t per = (int64_t)p.tokens * Shape::kUnit;
   int64_t total = 0;
   for (int i = 0; i < p.num_req; ++i)
-    for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb)
-      total += (int64_t)hk * (kUnitCost + oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb));
-  const int workers = std::min(std::max(oscar::PcShape<D>::kPair ? sms / 2 : sms, 1), oscar::kPcCtas);
+    for (int qb = 0; qb * per < p.q_len[i]; ++qb)
+      total += (int64_t)hk * (kUnitCost + oscar::pc_tiles<Shape>(p.q_len[i], p.seq[i], p.tokens, qb));
+  const int workers = std::min(std::max(Shape::kPair ? sms / 2 : sms, 1), oscar::kPcCtas);
   p.ctas = 0;
   b.splits.n = 0;
+  b.tiles = 0;
+  b.pieces = 1;
   int64_t cost = 0;  // of the units before
   int next = 0;      // the next worker to begin, at cost total * next / workers
   auto begin_of = [&](int w) { return total * w / workers; };
   for (int i = 0; i < p.num_req; ++i)
     for (int h = 0; h < hk; ++h)
-      for (int qb = 0; qb * (int64_t)per < p.q_len[i]; ++qb) {
-        const int nt = oscar::pc_tiles(p.q_len[i], p.seq[i], p.tokens, qb);
+      for (int qb = 0; qb * per < p.q_len[i]; ++qb) {
+        const int nt = oscar::pc_tiles<Shape>(p.q_len[i], p.seq[i], p.tokens, qb);
         const int holder = p.ctas - 1;  // the worker that reaches the unit, if none begins with it
         int done = 0;                   // tiles of the unit before the current worker
         bool begun = false;             // does a worker begin with the unit's first tile?
@@ -213,75 +216,63 @@ void plan_chunk(PagedBatch& b, int hk, int sms) {
           // at the same tile are one
           const int t = (int)std::max<int64_t>(0, begin_of(next) - cost - kUnitCost);
           ++next;
-          if (t < done || (t == done && (begun || (done > 0)))) continue;
+          if (t < done || (t == done && (begun || done > 0))) continue;
           if (p.ctas > 0) p.tiles[p.ctas - 1] += t - done;
           begun = begun || t == 0;
           done = t;
           p.start[p.ctas] = oscar::PcStart{i, h, qb, t};
+          p.first[p.ctas] = (int)(b.tiles + t);
           p.tiles[p.ctas++] = 0;
         }
         p.tiles[p.ctas - 1] += nt - done;
         const int first = begun ? holder + 1 : holder;
         if (p.ctas - 1 > first) b.splits.unit[b.splits.n++] = oscar::PcSplit{i, h, qb, first, p.ctas - 1};
+        b.pieces = std::max(b.pieces, p.ctas - first);
         cost += kUnitCost + nt;
+        b.tiles += nt;
       }
 }
 
 int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const int32_t* seqs, int num, int group,
                 int hk, int d, int sms) {
-  oscar::PagedPlan& p = b.plan;
-  oscar::PcPlan& pc = b.chunk;
+  oscar::PcPlan& p = b.plan;
   b.cls = cls;
-  p.num_req = pc.num_req = 0;
-  int64_t most = 0;
-  int r = r0, count = 0;
-  for (; r < num && count < oscar::kPgReqs; ++r) {
-    const int64_t len = qsl[r + 1] - qsl[r];
+  p.num_req = 0;
+  int r = r0;
+  for (; r < num && p.num_req < oscar::kPgReqs; ++r) {
+    const int len = qsl[r + 1] - qsl[r];
     if (len == 0 || paged_class(len, group) != cls) continue;
-    const int i = count++;
-    (cls == kChunk ? pc.req_id : p.req_id)[i] = r;
-    (cls == kChunk ? pc.q_start : p.q_start)[i] = qsl[r];
-    (cls == kChunk ? pc.q_len : p.q_len)[i] = (int)len;
-    (cls == kChunk ? pc.seq : p.seq)[i] = seqs[r];
-    most = std::max(most, len * group);
+    const int i = p.num_req++;
+    p.req_id[i] = r;
+    p.q_start[i] = qsl[r];
+    p.q_len[i] = len;
+    p.seq[i] = seqs[r];
   }
-  if (count == 0) return r;
-  if (cls == kChunk) {
-    pc.num_req = count;
-    pc.tokens = oscar::kPcRows / group;
-    if (d == 256) plan_chunk<256>(b, hk, sms);
-    else if (d == 128) plan_chunk<128>(b, hk, sms);
-    else plan_chunk<64>(b, hk, sms);
-    return r;
+  if (p.num_req == 0) return r;
+  p.tokens = p.box_tokens = oscar::kPcRows / group;
+  if (cls != kChunk) {
+    p.box_tokens = 1;
+    for (int i = 0; i < p.num_req; ++i) p.box_tokens = std::max(p.box_tokens, p.q_len[i]);
   }
-  p.num_req = count;
-  b.rows = most <= 16 ? 16 : kFewRows;
-  int64_t tiles = 0;
-  for (int i = 0; i < p.num_req; ++i) {
-    p.tile_begin[i] = tiles;
-    const int64_t blocks = ((int64_t)p.q_len[i] * group + b.rows - 1) / b.rows;
-    tiles += blocks * hk * std::max<int64_t>(1, ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys);
-  }
-  p.tile_begin[p.num_req] = tiles;
-  p.total_tiles = tiles;
-  p.ctas = (int)std::min<int64_t>(std::min(std::max(sms, 1), oscar::kPgCtas), tiles);
-  for (int c = 0; c <= p.ctas; ++c) p.cta_begin[c] = tiles * c / p.ctas;
+  if (cls != kChunk) plan_units<oscar::PcShape<256, true>>(b, hk, sms);  // (the plan does not depend on D)
+  else if (d == 256) plan_units<oscar::PcShape<256, false>>(b, hk, sms);
+  else plan_units<oscar::PcShape<128, false>>(b, hk, sms);  // (64 as 128)
   return r;
 }
 
 PagedSpace paged_space(const PagedBatch& b, int64_t n, int hq, int d, bool weighted) {
   PagedSpace s{};
   if (weighted) s.stats = round256(n * hq * (int64_t)sizeof(float2));
-  const int64_t pieces = b.cls == kChunk ? (int64_t)2 * b.chunk.ctas * oscar::kPcRows * oscar::kPcUnit
-                                         : (int64_t)2 * b.plan.ctas * b.rows;
+  const int64_t pieces = (int64_t)2 * b.plan.ctas * oscar::kPcRows * (b.cls == kChunk ? 2 : 1);
   s.part_ml = round256(pieces * (int64_t)sizeof(float2));
   s.part_o = round256(pieces * d * (int64_t)sizeof(float));
-  if (weighted && b.cls == kFew) s.scores = b.plan.total_tiles * b.rows * oscar::kPgKeys * (int64_t)sizeof(float);
+  if (weighted && b.cls == kFew) s.scores = b.tiles * oscar::kPgFewRows * oscar::kPgKeys * (int64_t)sizeof(float);
   return s;
 }
 
 int check_paged(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, int64_t n_tokens, int32_t hq, int32_t hk) {
   if (hq < 1 || hk < 1 || hq % hk || hq > 4096) return fail(OSCAR_ERR_INVALID, "paged_attention: Hq must be a multiple of Hk");
+  if (hq / hk > oscar::kPcRows) return fail(OSCAR_ERR_UNSUPPORTED, "paged_attention: GQA group %d > %d", hq / hk, oscar::kPcRows);
   if (num_requests < 0 || !qsl || (num_requests > 0 && !seqs) || qsl[0] != 0 || qsl[num_requests] != n_tokens)
     return fail(OSCAR_ERR_INVALID, "paged_attention: invalid query layout");
   for (int r = 0; r < num_requests; ++r)
@@ -348,22 +339,27 @@ struct PagedCall {
   cudaStream_t stream;
 };
 
+// The keys' weights of a launch's requests, from the scores or computed again
 template <int D, typename T>
-int launch_mass_rows(const PagedCall& c, int num_req, const int* req_id, const int* q_start, const int* q_len,
-                     const int* seq) {
-  oscar::PagedPlan keys;
-  keys.num_req = num_req;
+int launch_mass(const PagedCall& c, const PagedBatch& b) {
+  oscar::KeyPlan keys;
+  keys.num_req = b.plan.num_req;
   int64_t tiles = 0;
-  for (int i = 0; i < num_req; ++i) {
-    keys.req_id[i] = req_id[i];
-    keys.q_start[i] = q_start[i];
-    keys.q_len[i] = q_len[i];
-    keys.seq[i] = seq[i];
-    keys.tile_begin[i] = tiles;
-    tiles += ((int64_t)seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys;
+  for (int i = 0; i < b.plan.num_req; ++i) {
+    keys.req_id[i] = b.plan.req_id[i];
+    keys.q_start[i] = b.plan.q_start[i];
+    keys.q_len[i] = b.plan.q_len[i];
+    keys.seq[i] = b.plan.seq[i];
+    keys.tile_begin[i] = (int)tiles;
+    const int64_t nt = ((int64_t)b.plan.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys;
+    tiles += b.cls == kFew ? std::max<int64_t>(1, nt) * c.args.hk : nt;
   }
-  keys.tile_begin[num_req] = tiles;
+  keys.tile_begin[keys.num_req] = (int)tiles;
   if (tiles == 0) return OSCAR_OK;
+  if (b.cls == kFew) {
+    launch_pdl(oscar::paged_mass_kernel, dim3((unsigned)tiles), dim3(oscar::kPgKeys), 0, c.stream, c.args, keys);
+    return cuda_status("paged_mass_kernel");
+  }
   launch_pdl(oscar::paged_mass_rows_kernel<D, T>, dim3((unsigned)tiles, (unsigned)c.args.hk), dim3(32 * oscar::kPgWarps),
              (size_t)oscar::kPgKeys * D * 2, c.stream, c.args, keys, reinterpret_cast<const T*>(c.k_cache), c.kcb, c.kct,
              c.kch);
@@ -371,69 +367,67 @@ int launch_mass_rows(const PagedCall& c, int num_req, const int* req_id, const i
 }
 
 template <int D, typename T, int NRT>
-int launch_split(const PagedCall& c, const PagedBatch& b) {
-  const oscar::PagedArgs& a = c.args;
-  const oscar::PagedPlan& p = b.plan;
-  constexpr size_t smem = sizeof(oscar::PagedSmem<D, NRT>);
-  allow_smem<oscar::paged_split_kernel<D, T, NRT>>(smem);
-  launch_pdl(oscar::paged_split_kernel<D, T, NRT>, dim3(p.ctas), dim3(oscar::kPgThreads), smem, c.stream, a, p, c.kmap,
-             c.vmap);
-  int st = cuda_status("paged_split_kernel");
-  if (st) return st;
-  bool divided = false;  // does a CTA begin inside a unit?
-  for (int i = 0, c = 0; i < p.num_req && !divided; ++i) {
-    const int64_t nt = std::max<int64_t>(1, ((int64_t)p.seq[i] + oscar::kPgKeys - 1) / oscar::kPgKeys);
-    for (; c < p.ctas && p.cta_begin[c] < p.tile_begin[i + 1] && !divided; ++c)
-      divided = (p.cta_begin[c] - p.tile_begin[i]) % nt != 0;
-  }
-  if (divided) {
-    const int last = p.num_req - 1;
-    const int tokens = p.q_start[last] + p.q_len[last] - p.q_start[0];
-    launch_pdl(oscar::paged_combine_kernel<D, T, 16 * NRT>, dim3((unsigned)tokens, (unsigned)a.hq),
-               dim3(32 * oscar::kPgMerge), 0, c.stream, a, p);
-    st = cuda_status("paged_combine_kernel");
-    if (st) return st;
-  }
-  if (a.weights == nullptr) return OSCAR_OK;
-  if (b.cls == kFew) {
-    launch_pdl(oscar::paged_mass_kernel<16 * NRT>, dim3((unsigned)p.total_tiles), dim3(oscar::kPgKeys), 0, c.stream, a, p);
-    return cuda_status("paged_mass_kernel");
-  }
-  return launch_mass_rows<D, T>(c, p.num_req, p.req_id, p.q_start, p.q_len, p.seq);
+int launch_mma(const PagedCall& c, const PagedBatch& b) {
+  constexpr size_t smem = sizeof(oscar::PsSmem<D, NRT>);
+  static_assert(smem <= 227 * 1024, "PsSmem exceeds the shared memory of a CTA");
+  allow_smem<oscar::paged_attn_mma_kernel<D, T, NRT>>(smem);
+  launch_pdl(oscar::paged_attn_mma_kernel<D, T, NRT>, dim3(b.plan.ctas), dim3(oscar::kPgThreads), smem, c.stream, c.args,
+             b.plan, c.kmap, c.vmap);
+  return cuda_status("paged_attn_mma_kernel");
 }
 
-template <int D, typename T>
-int launch_chunk(const PagedCall& c, const PagedBatch& b) {
-  const oscar::PagedArgs& a = c.args;
-  const oscar::PcPlan& p = b.chunk;
-  constexpr size_t smem = sizeof(oscar::PcSmem<D>);
+template <int D, typename T, bool kFewRows>
+int launch_tc(const PagedCall& c, const PagedBatch& b) {
+  using Shape = oscar::PcShape<D, kFewRows>;
+  constexpr size_t smem = sizeof(oscar::PcSmem<D, kFewRows>);
   static_assert(smem <= 227 * 1024, "PcSmem exceeds the shared memory of a CTA");
-  allow_smem<oscar::paged_chunk_kernel<D, T>>(smem);
-  constexpr bool pair = oscar::PcShape<D>::kPair;
-  launch_pdl_cluster(pair ? 2 : 1, oscar::paged_chunk_kernel<D, T>, dim3(pair ? 2 * p.ctas : p.ctas),
-                     dim3(oscar::PcShape<D>::kThreads), smem, c.stream, a, p, c.qmap, c.kmap, c.vmap);
-  int st = cuda_status("paged_chunk_kernel");
+  allow_smem<oscar::paged_attn_tc_kernel<D, T, kFewRows>>(smem);
+  launch_pdl_cluster(Shape::kPair ? 2 : 1, oscar::paged_attn_tc_kernel<D, T, kFewRows>,
+                     dim3(Shape::kPair ? 2 * b.plan.ctas : b.plan.ctas), dim3(Shape::kThreads), smem, c.stream, c.args,
+                     b.plan, c.qmap, c.kmap, c.vmap);
+  return cuda_status("paged_attn_tc_kernel");
+}
+
+template <int D, typename T, bool kFewRows>
+int launch_paged(const PagedCall& c, const PagedBatch& b) {
+  using Shape = oscar::PcShape<D, kFewRows>;
+  const oscar::PagedArgs& a = c.args;
+  const oscar::PcPlan& p = b.plan;
+  int most = 0;  // tokens of a request
+  for (int i = 0; i < p.num_req; ++i) most = std::max(most, p.q_len[i]);
+  int st;
+  if (b.cls == kFew && b.tiles <= kMmaTiles * device_info().sms)
+    st = most * a.group <= 16 ? launch_mma<D, T, 1>(c, b) : launch_mma<D, T, 2>(c, b);
+  else
+    st = launch_tc<D, T, kFewRows>(c, b);
   if (st) return st;
   if (b.splits.n > 0) {
-    launch_pdl(oscar::paged_chunk_combine_kernel<D, T>, dim3((unsigned)(b.splits.n * oscar::kPcUnit * oscar::kPcRows / 4)),
-               dim3(128), 0, c.stream, a, p, b.splits);
-    st = cuda_status("paged_chunk_combine_kernel");
+    int rows = Shape::kUnit * oscar::kPcRows;  // of a unit
+    if (kFewRows) rows = most * a.group;
+    // four warps a row from nine pieces on: with one, a row's pieces come one after another (28
+    // against 10 us for one request's 24 rows in 37 pieces); below, they would mostly idle
+    if (b.pieces > 8)
+      launch_pdl(oscar::paged_merge_kernel<D, T, kFewRows, oscar::kPcMerge>, dim3((unsigned)rows, (unsigned)b.splits.n),
+                 dim3(128), 0, c.stream, a, p, b.splits);
+    else
+      launch_pdl(oscar::paged_merge_kernel<D, T, kFewRows, 1>, dim3((unsigned)(rows + 3) / 4, (unsigned)b.splits.n), dim3(128),
+                 0, c.stream, a, p, b.splits);
+    st = cuda_status("paged_merge_kernel");
     if (st) return st;
   }
-  return a.weights == nullptr ? OSCAR_OK : launch_mass_rows<D, T>(c, p.num_req, p.req_id, p.q_start, p.q_len, p.seq);
-}
-
-template <int D, typename T>
-int launch_paged(const PagedCall& c, const PagedBatch& b) {
-  if (b.cls == kChunk) return launch_chunk<D, T>(c, b);
-  return b.rows <= 16 ? launch_split<D, T, 1>(c, b) : launch_split<D, T, 2>(c, b);
+  return a.weights == nullptr ? OSCAR_OK : launch_mass<D, T>(c, b);
 }
 
 template <typename T>
 int launch_paged_d(int d, const PagedCall& c, const PagedBatch& b) {
-  if (d == 256) return launch_paged<256, T>(c, b);
-  if (d == 128) return launch_paged<128, T>(c, b);
-  return launch_paged<64, T>(c, b);
+  if (b.cls == kChunk) {
+    if (d == 256) return launch_paged<256, T, false>(c, b);
+    if (d == 128) return launch_paged<128, T, false>(c, b);
+    return launch_paged<64, T, false>(c, b);
+  }
+  if (d == 256) return launch_paged<256, T, true>(c, b);
+  if (d == 128) return launch_paged<128, T, true>(c, b);
+  return launch_paged<64, T, true>(c, b);
 }
 
 }  // namespace
@@ -452,7 +446,7 @@ int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs,
     for (int r = 0; r < num_requests;) {
       r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
                       device_info().sms);
-      if (b.num() > 0)
+      if (b.plan.num_req > 0)
         need = std::max(need, paged_space(b, qsl[num_requests], num_q_heads, head_dim, weighted != 0).total());
     }
   return need;
@@ -521,10 +515,11 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   PagedBatch b;
   for (int cls = 0; cls < kClasses; ++cls)
     for (int r = 0; r < num_requests;) {
-      r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, a.group, num_kv_heads, head_dim, device_info().sms);
-      if (b.num() == 0) continue;
-      if (cls == kChunk && !query_map(&c.qmap, q, dtype, n_tokens, num_q_heads, head_dim, q_token_stride, q_head_stride,
-                                      a.group, b.chunk.tokens))
+      r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, a.group, num_kv_heads, head_dim,
+                      device_info().sms);
+      if (b.plan.num_req == 0) continue;
+      if (!query_map(&c.qmap, q, dtype, n_tokens, num_q_heads, head_dim, q_token_stride, q_head_stride, a.group,
+                     b.plan.box_tokens))
         return fail(OSCAR_ERR_INVALID, "paged_attention: the queries' strides do not fit a tensor map");
       const PagedSpace space = paged_space(b, n_tokens, num_q_heads, head_dim, weights != nullptr);
       if (workspace_bytes < space.total() || !workspace)

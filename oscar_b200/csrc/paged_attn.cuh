@@ -1,41 +1,49 @@
-// Attention of long chunks over a paged 16-bit cache on the 5th-generation
-// tensor cores (same function as paged.cuh; requests with many query rows).
+// Attention of new tokens over a paged 16-bit cache on the 5th-generation tensor
+// cores (function and arguments: paged.cuh).
 //
-// Work.  A unit is (request, kv head, q-block); a q-block is two tiles of 128
-// query rows, each holding floor(128 / group) tokens x group heads.  Its visible
-// keys are cut into 128-key tiles, and the tiles of all units, in order, are
-// divided evenly over the workers by the host, so a worker streams whole units
-// except at its two ends; the pieces of a divided unit are written unnormalised
-// in fp32 and combined by a dependent launch in worker order.
+// Work.  A unit is (request, kv head, q-block); a q-block is one (kFew: requests
+// of at most 128 query rows) or two tiles of 128 query rows, each holding
+// floor(128 / group) tokens x group heads.  Its visible keys are cut into tiles,
+// and the tiles of all units, in order, are divided over the workers by the
+// host, so a worker streams whole units except at its two ends; the pieces of
+// a divided unit are written unnormalised in fp32 and combined by a dependent
+// launch in worker order (no atomics: the result does not depend on timing).
 //
-// A worker is one CTA that holds both row tiles (D 64, 128), or a pair of CTAs
-// with one row tile each (D 256): the pair's products are issued once for 256
-// rows (cta_group::2), and each CTA fetches half of every K and V tile.  One CTA
-// alone would need 63 bytes per cycle of K and V to keep its tensor pipe busy,
-// and TMA brings an SM at most 46 (measured on resident data); it also leaves
-// room for 2.5 tiles of K and V instead of 1.25 beside the queries.
+// A worker is one CTA, or (D 256, two row tiles) a pair of CTAs with one row tile
+// each: the pair's products are issued once for 256 rows (cta_group::2), and
+// each CTA fetches half of every K and V tile.  One CTA alone would need 63
+// bytes per cycle of K and V to keep its tensor pipe busy, and TMA brings an SM
+// at most 46 (measured on resident data); it also leaves room for 2.5 tiles of K
+// and V instead of 1.25 beside the queries.
 //
-// Tile.  Bound by the tensor pipe at D 256 and by the exponentials at D <= 128
-// (128 x 128 per row tile at 16 per cycle and SM).  Jobs alternate between two
-// score buffers: D 256: job j is key tile j; D <= 128: key tile j / 2 of row tile
-// j % 2.  The MMA warp issues S(0), S(1), then per job O += P(j) V as soon as
-// P(j) is written and S(j + 2), so while the softmax of one job runs the tensor
-// pipe has the other job's products.
-//   TMEM columns: S[0] [0, 128), S[1] [128, 256), O [256, 512) (D 256) or
+// Bounds.  kFew: HBM; the keys stream through shared memory once, 64-key tiles,
+// and the products of 128 padded rows take half of the time their bytes do
+// (mma.sync on the live rows took more: its operand reads alone filled the
+// shared-memory bandwidth that the copies leave).  Else D 256: the tensor pipe;
+// D <= 128: the exponentials (128 x 128 per row tile at 16 per cycle and SM).
+//
+// Tile.  Jobs alternate between two score buffers: with one row tile per CTA job j
+// is key tile j, with two it is key tile j / 2 of row tile j % 2.  The MMA warp
+// issues S(0), S(1), then per job O += P(j) V as soon as P(j) is written and
+// S(j + 2), so while the softmax of one job runs the tensor pipe has the other
+// job's products.
+//   TMEM columns: S[0] [0, 128), S[1] [128, 256), O [256, 512) (one row tile) or
 //   O[0] [256, 256 + D), O[1] [384, 384 + D).  P(j) (16 bit) replaces the first
-//   64 columns of S(j) and is the A operand of P V; rows lie on lanes, one
+//   half of S(j)'s columns and is the A operand of P V; rows lie on lanes, one
 //   query row per softmax thread, so row maxima and sums stay in a thread.
 //   S = Q K^T : A = Q, B = K, both shared memory, K-major, 128-byte swizzle.
 //   O += P V  : A = P in tensor memory, B = V, MN-major, 128-byte swizzle.
 // The running maximum moves only when a score exceeds it by kPgHeadroom (log2
-// units); then the thread rescales its row of O in tensor memory.
+// units); then the thread rescales its row of O in tensor memory.  P is rounded to
+// the values' type (the product takes one type): 2^-9 (bf16) or 2^-12 of each
+// probability, below the rounding of the result.
 //
-// Warps: 4 or 8 softmax, one MMA issuer, two TMA producers (K and Q; V) that
-// fill one ring of slots in the order the MMAs use them, in boxes of 64 dims x a
-// power of two of tokens.  Each role is a short loop: unrolled over a row or a
-// tile they overran the instruction cache (4.0 against 2.85 ms for 8192 queries
-// on 17448 keys).  Every wait is bounded; a time-out sets the CTA's abort flag
-// and drains.
+// Warps: 4 softmax per row tile, one MMA issuer, two TMA producers (K and Q; V)
+// that fill one ring of slots in the order the MMAs use them, in boxes of 64
+// dims x a power of two of tokens.  Each role is a short loop: unrolled over a
+// row or a tile they overran the instruction cache (4.0 against 2.85 ms for 8192
+// queries on 17448 keys).  Every wait is bounded; a time-out sets the CTA's abort
+// flag and drains.
 #pragma once
 
 #include <climits>
@@ -44,19 +52,20 @@
 
 namespace oscar {
 
-constexpr int kPcRows = 128;
-constexpr int kPcKeys = 128;
+constexpr int kPcRows = 128;   // rows of a row tile
 constexpr int kPcCtas = 192;   // workers of a plan
-constexpr int kPcUnit = 2;     // row tiles of a unit
+constexpr int kPcMerge = 4;    // warps that combine a row of many pieces
 
 struct PcStart {
   int r, h, qb, t;  // plan index, kv head, q-block, first key tile
 };
 struct PcPlan {
   int num_req, ctas, tokens;  // workers; tokens per row tile
+  int box_tokens;             // tokens per query load: kFew: the most that a request has, else `tokens`
   int req_id[kPgReqs], q_start[kPgReqs], q_len[kPgReqs], seq[kPgReqs];
   PcStart start[kPcCtas];
   int tiles[kPcCtas];  // key tiles of each worker
+  int first[kPcCtas];  // tiles before it
 };
 struct PcSplit {
   int r, h, qb, c0, c1;  // a divided unit and its workers
@@ -66,24 +75,26 @@ struct PcSplits {
   PcSplit unit[kPcCtas];
 };
 
-template <int D>
+template <int D, bool kFew>
 struct PcShape {
-  static constexpr bool kPair = D == 256;               // a worker is a pair of CTAs
-  static constexpr int kM = kPair ? 1 : 2;              // row tiles per CTA
+  static constexpr bool kPair = D == 256 && !kFew;      // a worker is a pair of CTAs
+  static constexpr int kUnit = kFew ? 1 : 2;            // row tiles of a unit
+  static constexpr int kM = kPair ? 1 : kUnit;          // row tiles per CTA
+  static constexpr int kTile = kFew ? kPgKeys : 128;    // keys per tile
   static constexpr int kPanels = D / 64;                // 64-dim panels
-  static constexpr int kKeys = kPair ? 64 : kPcKeys;    // keys of a K tile in this CTA
+  static constexpr int kKeys = kPair ? 64 : kTile;      // keys of a K tile in this CTA
   static constexpr int kVPanels = kPair ? 2 : kPanels;  // panels of a V tile in this CTA
   static constexpr int kSlot = kKeys * D * 2;           // a K tile or a V tile
-  static constexpr int kSlots = D == 64 ? 8 : 5;
+  static constexpr int kSlots = kFew ? (D == 256 ? 5 : D == 128 ? 12 : 16) : (D == 64 ? 8 : 5);
   static constexpr int kSoftWarps = 4 * kM;
   static constexpr int kThreads = 32 * (kSoftWarps + 3);
 };
 
-template <int D>
+template <int D, bool kFew>
 struct PcSmem {
-  using S = PcShape<D>;
+  using S = PcShape<D, kFew>;
   uint8_t q[S::kM][S::kPanels][kPcRows * 128];  // [row tile][panel][row][128 bytes], swizzled
-  uint8_t ring[S::kSlots][S::kSlot];            // K: [panel][key][128 bytes]; V: [panel][128 keys][128 bytes]
+  uint8_t ring[S::kSlots][S::kSlot];            // K: [panel][key][128 bytes]; V: [panel][key][128 bytes]
   // full, q_full, p_full: of a pair, the first CTA's are used by both
   unsigned long long full[S::kSlots], empty[S::kSlots];
   unsigned long long q_full, q_empty, s_full[2], p_full[2], o_done[2], tail, end;
@@ -95,6 +106,9 @@ OSCAR_DEVINL uint64_t pc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
   return tc::smem_desc(addr, lbo, sbo) | (2ull << 61);  // 128-byte swizzle
 }
 
+OSCAR_DEVINL void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];\n" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
 OSCAR_DEVINL void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
@@ -104,21 +118,22 @@ OSCAR_DEVINL void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y
 }
 
 // key tiles that q-block qb of a request sees (at least 1, so that empty rows are written)
+template <typename Shape>
 __host__ __device__ inline int pc_tiles(int q_len, int seq, int tokens, int qb) {
-  const int last = (qb + 1) * tokens * kPcUnit;
-  const int visible = seq - q_len + (last < q_len ? last : q_len);
-  return visible > kPcKeys ? (visible + kPcKeys - 1) / kPcKeys : 1;
+  const int64_t last = (int64_t)(qb + 1) * tokens * Shape::kUnit;
+  const int visible = seq - q_len + (int)(last < q_len ? last : q_len);
+  return visible > Shape::kTile ? (visible + Shape::kTile - 1) / Shape::kTile : 1;
 }
 
-// Ring position of key tile t's K and V (n tiles in the worker's stream).
-// D <= 128: K0 V0 K1 V1 ..; D 256 (S runs two tiles ahead of O): K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1).
-template <int D>
+// Ring position of key tile t's K and V (n tiles in the worker's stream).  S runs two jobs ahead of
+// O: with two row tiles K0 V0 K1 V1 .., with one K0 K1 V0 K2 V1 .. K(n-1) V(n-2) V(n-1).
+template <int kM>
 OSCAR_DEVINL int pc_k_at(int t) {
-  return D == 256 ? (t == 0 ? 0 : 2 * t - 1) : 2 * t;
+  return kM == 1 ? (t == 0 ? 0 : 2 * t - 1) : 2 * t;
 }
-template <int D>
+template <int kM>
 OSCAR_DEVINL int pc_v_at(int t, int n) {
-  return D == 256 ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1;
+  return kM == 1 ? (t == n - 1 ? 2 * n - 1 : 2 * t + 2) : 2 * t + 1;
 }
 
 // The two CTAs of a pair
@@ -210,6 +225,7 @@ OSCAR_DEVINL void pc_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
 }
 
 // The pieces of units of one worker, walked alike by every role.
+template <typename Shape>
 struct PcWalk {
   const PcPlan& p;
   int r, h, qb, t, left;
@@ -220,7 +236,7 @@ struct PcWalk {
   }
   OSCAR_DEVINL void open() {
     if (left <= 0) return;
-    nt = pc_tiles(p.q_len[r], p.seq[r], p.tokens, qb);
+    nt = pc_tiles<Shape>(p.q_len[r], p.seq[r], p.tokens, qb);
     t_end = min(nt, t + left);
   }
   OSCAR_DEVINL bool live() const { return left > 0; }
@@ -228,7 +244,7 @@ struct PcWalk {
     left -= t_end - t;
     t = 0;
     ++piece;
-    const int per = p.tokens * kPcUnit;
+    const int per = p.tokens * Shape::kUnit;
     if (++qb >= (p.q_len[r] + per - 1) / per) {
       qb = 0;
       if (++h >= hk) {
@@ -291,22 +307,23 @@ OSCAR_DEVINL void pc_transpose8(uint32_t (&x)[8][4], int lane) {
     }
   }
 }
-template <int D, typename T>
-__global__ void __launch_bounds__(PcShape<D>::kThreads, 1)
-paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PcPlan p,
+template <int D, typename T, bool kFew>
+__global__ void __launch_bounds__(PcShape<D, kFew>::kThreads, 1)
+paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ PcPlan p,
                    const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
                    const __grid_constant__ CUtensorMap vmap) {
-  using Shape = PcShape<D>;
+  using Shape = PcShape<D, kFew>;
   constexpr bool kPair = Shape::kPair;
-  constexpr int kM = Shape::kM, kPanels = Shape::kPanels, kSlots = Shape::kSlots;
+  constexpr int kM = Shape::kM, kPanels = Shape::kPanels, kSlots = Shape::kSlots, kTile = Shape::kTile;
   constexpr int kMma = Shape::kSoftWarps;
   constexpr int kColO = 256;
   extern __shared__ __align__(1024) uint8_t pc_raw[];
-  PcSmem<D>& sm = *reinterpret_cast<PcSmem<D>*>(pc_raw);
+  PcSmem<D, kFew>& sm = *reinterpret_cast<PcSmem<D, kFew>*>(pc_raw);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t rank = kPair ? pc_rank() : 0u;
   const int worker = kPair ? (int)blockIdx.x / 2 : (int)blockIdx.x;
   pdl_release();
+  if (tid < 3) prefetch_map(tid == 0 ? &qmap : tid == 1 ? &kmap : &vmap);
   auto full = [&](int i) { return smem_u32(&sm.full[i]); };
   auto empty = [&](int i) { return smem_u32(&sm.empty[i]); };
   // a barrier that the pair's first CTA owns, for arrivals and loads
@@ -339,6 +356,12 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       tc::tmem_relinquish();
     }
   }
+  if constexpr (kFew) {
+    // rows that no query load reaches are zero: their scores and probabilities then are too, and the
+    // padded products switch nothing (the copies alone draw 950 of the card's 1000 W)
+    for (int i = tid; i < (int)sizeof(sm.q) / 16; i += Shape::kThreads) reinterpret_cast<uint4*>(sm.q)[i] = make_uint4(0, 0, 0, 0);
+    tc::fence_async_smem();
+  }
   tc::tc_fence_before();
   if constexpr (kPair) pc_cluster_sync();  // the other CTA's barriers are initialised
   else __syncthreads();
@@ -347,9 +370,10 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {  // warp-uniform
     return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
   };
+  PcWalk<Shape> w(p, worker);  // (the plan is an argument)
+  const int n_tiles = w.left, tile0 = p.first[worker];
   pdl_wait();
-  PcWalk w(p, worker);
-  const int n_tiles = w.left;
+  (void)tile0;
 
   if (warp < kMma) {
     // ================= softmax: thread = query row of row tile `wg`
@@ -362,10 +386,11 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     bool ok = true;
     for (; w.live() && ok; w.next(a.hk)) {
       const int q_len = p.q_len[w.r], seq = p.seq[w.r];
-      const int tok = (w.qb * kPcUnit + rt) * p.tokens + row / a.group;
+      const int tok = (w.qb * Shape::kUnit + rt) * p.tokens + row / a.group;
       const bool live = row < rows && tok < q_len;
       // visible keys; rows that hold no query are computed as they come and not written
       const int lim = live ? max(0, seq - q_len + tok + 1) : INT_MAX;
+      const bool busy = __any_sync(0xffffffffu, live);
       float m = -INFINITY;
       uint64_t l2 = 0;  // two partial sums
       const uint32_t o_col = tmem + lanes + kColO + (kM == 2 ? 128 * wg : 0);
@@ -375,12 +400,16 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const uint32_t s_col = tmem + lanes + 128 * b;
         if (!wait(smem_u32(&sm.s_full[b]), (job >> 1) & 1)) { ok = false; break; }
         tc::tc_fence_after();
+        if (kFew && !busy) {  // no query in this warp's rows: whatever their P is, it stays in them
+          if (lane == 0) tc::mbar_arrive(smem_u32(&sm.p_full[b]));
+          continue;
+        }
         // D 256: the row's scores stay in registers over both passes.  D <= 128 (eleven warps, 168
         // registers): chunks of 32 columns, read twice (103 against 115 us on ragged chunks at D 128;
         // at D 256 2140 against 2025 us on the longest one)
-        constexpr int kChunk = kPair ? kPcKeys : 32;
-        const int vis = lim - t * kPcKeys;  // keys c < vis are visible
-        const bool masked = __any_sync(0xffffffffu, vis < kPcKeys);
+        constexpr int kChunk = kM == 1 ? kTile : 32;
+        const int vis = lim - t * kTile;  // keys c < vis are visible
+        const bool masked = __any_sync(0xffffffffu, vis < kTile);
         uint32_t s[kChunk];
         auto load_scores = [&](int c0) {
 #pragma unroll
@@ -393,13 +422,22 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         };
         float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
-        for (int c0 = 0; c0 < kPcKeys; c0 += kChunk) {
+        for (int c0 = 0; c0 < kTile; c0 += kChunk) {
           load_scores(c0);
 #pragma unroll
           for (int c = 0; c < kChunk; c += 8)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               m4[i] = max3(m4[i], __uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1]));
+        }
+        if constexpr (kFew) {
+          if (a.scores != nullptr && live) {
+            float4* dst = reinterpret_cast<float4*>(a.scores + ((int64_t)(tile0 + job) * kPgFewRows + row) * kPgKeys);
+#pragma unroll
+            for (int c = 0; c < kTile; c += 4)
+              dst[c / 4] = make_float4(__uint_as_float(s[c]) * scale, __uint_as_float(s[c + 1]) * scale,
+                                       __uint_as_float(s[c + 2]) * scale, __uint_as_float(s[c + 3]) * scale);
+          }
         }
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
         const bool grow = mx > m + kPgHeadroom;
@@ -425,9 +463,9 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const float base = m == -INFINITY ? 0.0f : -m;
         const uint64_t scale2 = f2_pack(scale, scale), base2 = f2_pack(base, base);
 #pragma unroll 1
-        for (int c0 = 0; c0 < kPcKeys; c0 += kChunk) {
+        for (int c0 = 0; c0 < kTile; c0 += kChunk) {
           // (the columns P overwrites, [c0 / 2, c0 / 2 + 16), have been read)
-          if (kChunk < kPcKeys) load_scores(c0);
+          if (kChunk < kTile) load_scores(c0);
 #pragma unroll
           for (int c = 0; c < kChunk; c += 32) {
             uint32_t pk[16];
@@ -462,38 +500,44 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       const float inv = none ? 0.0f : 1.0f / total;
       const int head = w.h * a.group + row % a.group;
       const int64_t orow = (int64_t)(p.q_start[w.r] + tok) * a.hq + head;
-      const int64_t prow = ((int64_t)(2 * worker + (w.piece == 0 ? 0 : 1)) * kPcUnit + rt) * kPcRows + row;
+      const int64_t prow = ((int64_t)(2 * worker + (w.piece == 0 ? 0 : 1)) * Shape::kUnit + rt) * kPcRows + row;
       // 128 bytes of a row at a time lie in one lane; 8 lanes exchange 16-byte pieces so that a store
       // instruction writes whole lines of 4 rows (32 lines of one sector each took 9400 cycles a unit)
-      const int64_t my_row = !live ? -1 : whole ? orow : prow;
-      const int step = whole ? 64 : 32;  // columns per 128 bytes
-#pragma unroll 1
-      for (int c = 0; c < D; c += step) {
-        uint32_t x[8][4];
+      const int64_t row_bytes = D * (whole ? 2 : 4);
+      const int64_t my_row = !live ? -1 : (whole ? orow : prow) * row_bytes;
+      int64_t to[8];
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          if (hf == 1 && !whole) break;
-          uint32_t o[32];
-          tc::tmem_ld32(o_col + c + 32 * hf, o);
+      for (int k = 0; k < 8; ++k) to[k] = __shfl_sync(0xffffffffu, my_row, (lane & 24) + k);
+      uint8_t* const base = (whole ? reinterpret_cast<uint8_t*>(a.out) : reinterpret_cast<uint8_t*>(a.part_o)) + 16 * (lane & 7);
+      auto store = [&](uint32_t (&x)[8][4], int line) {  // the rows' line-th 128 bytes
+        pc_transpose8(x, lane);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (to[k] >= 0)
+            *reinterpret_cast<uint4*>(base + to[k] + 128 * line) = make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
+      };
+      if (busy) {
+        uint32_t o[32], x[8][4];
+        tc::tmem_ld32(o_col, o);
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
           tc::tmem_wait_ld();
           if (whole) {
+            // 64 columns make 128 bytes: this half's 16-bit values beside the last one's
+            const bool second = c & 32;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              x[4 * hf + i / 4][i % 4] = pc_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+            for (int i = 0; i < 16; ++i) {
+              const uint32_t v = pc_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+              if (second) x[4 + i / 4][i % 4] = v;
+              else x[i / 4][i % 4] = v;
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) x[i / 4][i % 4] = o[i];
           }
-        }
-        pc_transpose8(x, lane);
-        uint8_t* dst = whole ? reinterpret_cast<uint8_t*>(reinterpret_cast<T*>(a.out) + c)
-                             : reinterpret_cast<uint8_t*>(a.part_o + c);
-        const int64_t row_bytes = D * (whole ? 2 : 4);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const int64_t to = __shfl_sync(0xffffffffu, my_row, (lane & 24) + k);
-          if (to >= 0)
-            *reinterpret_cast<uint4*>(dst + to * row_bytes + 16 * (lane & 7)) = make_uint4(x[k][0], x[k][1], x[k][2], x[k][3]);
+          if (c + 32 < D) tc::tmem_ld32(o_col + c + 32, o);  // the next columns, during the exchange and the stores
+          if (!whole) store(x, c / 32);
+          else if (c & 32) store(x, c / 64);
         }
       }
       if (live) {
@@ -510,11 +554,11 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     // ================= MMA issuer (of a pair: the first CTA's)
     constexpr uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr int kRows = kPair ? 2 * kPcRows : kPcRows;
-    constexpr uint32_t idesc_s = tc::instr_desc(fmt, 0, 0, kRows, kPcKeys);
+    constexpr uint32_t idesc_s = tc::instr_desc(fmt, 0, 0, kRows, kTile);
     constexpr uint32_t idesc_o = tc::instr_desc(fmt, 0, 1, kRows, D);
     const uint64_t dq = pc_desc(smem_u32(sm.q), 16, 1024);
     const uint64_t dk = pc_desc(smem_u32(sm.ring), 16, 1024);
-    const uint64_t dv = pc_desc(smem_u32(sm.ring), kPcKeys * 128, 1024);
+    const uint64_t dv = pc_desc(smem_u32(sm.ring), kTile * 128, 1024);
     constexpr uint64_t kSlotStep = Shape::kSlot >> 4;
     // The warp runs the role converged and elects a lane for each batch of products (run by one
     // thread of a diverged warp the products issue slower: 2580 against 2430 us).  What a step
@@ -525,7 +569,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
       return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
     };
     // S runs two jobs ahead of O and may belong to the next unit
-    PcWalk ws = w;                               // unit of the next S
+    PcWalk<Shape> ws = w;                               // unit of the next S
     int unit = 0;                                // its number
     int s_left = (ws.t_end - ws.t) * kM, o_left = s_left;  // jobs left in the units of the next S and O
     bool s_open = false, o_open = false;         // the unit's Q has been waited for; O holds a product of the unit
@@ -534,8 +578,8 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     for (int step = 0; step < jobs + 2; ++step) {
       const int jo = step - 2, js = step;
       const int o_mt = kM == 2 ? jo & 1 : 0, s_mt = kM == 2 ? js & 1 : 0;
-      const int v_at = pc_v_at<D>(kM == 2 ? jo >> 1 : jo, n_tiles), v_slot = v_at % kSlots;
-      const int k_at = pc_k_at<D>(kM == 2 ? js >> 1 : js), k_slot = k_at % kSlots;
+      const int v_at = pc_v_at<kM>(kM == 2 ? jo >> 1 : jo, n_tiles), v_slot = v_at % kSlots;
+      const int k_at = pc_k_at<kM>(kM == 2 ? js >> 1 : js), k_slot = k_at % kSlots;
       if (jo >= 0 && o_mt == 0 && !wait_all(full(v_slot), (v_at / kSlots) & 1)) break;
       if (js < jobs && s_open && s_mt == 0) {
         if (!wait_all(full(k_slot), (k_at / kSlots) & 1)) break;
@@ -547,7 +591,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         if (tc::elect_one()) {
           const uint64_t vd = dv + (uint64_t)v_slot * kSlotStep;
 #pragma unroll
-          for (int ks = 0; ks < kPcKeys / 16; ++ks)
+          for (int ks = 0; ks < kTile / 16; ++ks)
             pc_mma_ts<kPair>(tmem + kColO + 128 * o_mt, tmem + 128 * (jo & 1) + 8 * ks, vd + ks * (2048 >> 4), idesc_o,
                              (o_open || ks > 0) ? 1u : 0u);
           if (o_mt == kM - 1) pc_commit<kPair>(empty(v_slot));
@@ -601,7 +645,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     // before it is issued; one elected lane issues (operands uniform over the warp)
     const bool is_k = warp == kMma + 1;
     const CUtensorMap* map = is_k ? &kmap : &vmap;
-    const int per = kPcKeys / a.box;  // boxes per tile
+    const int per = kTile / a.box;  // boxes per tile
     const uint32_t box = (uint32_t)a.box, box_bytes = box * 128u;
     // of a pair's tile: K half of the keys, V half of the dims
     const int box0 = kPair && is_k ? (int)rank * (per / 2) : 0, nbox = kPair && is_k ? per / 2 : per;
@@ -609,10 +653,10 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     const uint32_t panel = (uint32_t)nbox * box_bytes;  // bytes of a panel of the slot
     const int32_t* row = nullptr;
     int boxes = 0, unit = 0, t = 0, last_at = -1, tails = 0;
-    int blk[kPcKeys / 32];
+    int blk[kTile / 32];
     auto look_up = [&] {
 #pragma unroll
-      for (int i = 0; i < kPcKeys / 32; ++i) {
+      for (int i = 0; i < kTile / 32; ++i) {
         if (32 * i >= per) break;
         const int j = lane + 32 * i, b = t * per + j;
         blk[i] = j < per && b < boxes ? row[a.page.div((uint32_t)b * box)] : 0;
@@ -631,23 +675,23 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
           if (unit > 0 && !wait(smem_u32(&sm.q_empty), (unit - 1) & 1)) break;
           if (tc::elect_one()) {
             const uint32_t bar = lead(smem_u32(&sm.q_full));
-            const uint32_t bytes = (uint32_t)(kM * kPanels * p.tokens * a.group * 128);
+            const uint32_t bytes = (uint32_t)(kM * kPanels * p.box_tokens * a.group * 128);
             if constexpr (kPair) pc_expect(bar, bytes);
             else tc::mbar_expect_tx(bar, bytes);
 #pragma unroll 1
             for (int i = 0; i < kM * kPanels; ++i)
               pc_load_3d<kPair>(smem_u32(sm.q) + i * kPcRows * 128, &qmap, 64 * (i % kPanels), w.h * a.group,
-                                p.q_start[w.r] + (w.qb * kPcUnit + (kPair ? (int)rank : i / kPanels)) * p.tokens, bar);
+                                p.q_start[w.r] + (w.qb * Shape::kUnit + (kPair ? (int)rank : i / kPanels)) * p.tokens, bar);
           }
           __syncwarp();
           ++unit;
         }
       }
       const int first = t * per, h = w.h, here = min(per, max(0, boxes - first));
-      const int have = p.seq[w.r] - t * kPcKeys;  // keys of the request from the tile's first on
-      int cur[kPcKeys / 32];
+      const int have = p.seq[w.r] - t * kTile;  // keys of the request from the tile's first on
+      int cur[kTile / 32];
 #pragma unroll
-      for (int i = 0; i < kPcKeys / 32; ++i) {
+      for (int i = 0; i < kTile / 32; ++i) {
         cur[i] = blk[i];
         if (lane + 32 * i < here && (cur[i] < 0 || cur[i] >= a.num_blocks)) {
           flag_error(2u);
@@ -660,12 +704,12 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         w.next(a.hk);
         open = false;
       }
-      const int at = is_k ? pc_k_at<D>(tile) : pc_v_at<D>(tile, n_tiles), slot = at % kSlots;
+      const int at = is_k ? pc_k_at<kM>(tile) : pc_v_at<kM>(tile, n_tiles), slot = at % kSlots;
       const int live = max(0, min(nbox, here - box0));
       if (at >= kSlots && !wait(empty(slot), ((at / kSlots) - 1) & 1)) break;
       last_at = at;
       // a V tile past whose end anything may stand (0 * NaN) is completed here before it is announced
-      const bool tail = !is_k && have < kPcKeys;
+      const bool tail = !is_k && have < kTile;
       const uint32_t bar = tail ? smem_u32(&sm.tail) : lead(full(slot));
       const uint32_t bytes = (uint32_t)(live * pans) * box_bytes;
       if (tc::elect_one()) {
@@ -679,7 +723,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         const int j = box0 + i;
         int b = 0;
 #pragma unroll
-        for (int k = 0; k < kPcKeys / 32; ++k) {
+        for (int k = 0; k < kTile / 32; ++k) {
           if (32 * k >= per) break;
           const int v = __shfl_sync(0xffffffffu, cur[k], j & 31);
           if (j >> 5 == k) b = v;
@@ -697,7 +741,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
         if (!wait(bar, tails & 1)) break;
         ++tails;
         const int clear = max(have, 0);
-        for (int i = lane; i < (kPcKeys - clear) * 8 * pans; i += 32) {
+        for (int i = lane; i < (kTile - clear) * 8 * pans; i += 32) {
           const int key = clear + i / (8 * pans), c = i % (8 * pans);
           *reinterpret_cast<uint4*>(sm.ring[slot] + (c / 8) * panel + key * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
         }
@@ -712,7 +756,7 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
     // the releases of the last slots come to both CTAs of a pair: none may come to a CTA that ended
     if constexpr (kPair) {
       for (int i = max(0, n_tiles - 3); i < n_tiles; ++i) {
-        const int n = is_k ? pc_k_at<D>(i) : pc_v_at<D>(i, n_tiles);
+        const int n = is_k ? pc_k_at<kM>(i) : pc_v_at<kM>(i, n_tiles);
         if (n + kSlots >= 2 * n_tiles && n <= last_at && !wait(empty(n % kSlots), (n / kSlots) & 1)) break;
       }
       if (is_k && unit > 0) wait(smem_u32(&sm.q_empty), (unit - 1) & 1);
@@ -736,24 +780,29 @@ paged_chunk_kernel(const __grid_constant__ PagedArgs a, const __grid_constant__ 
   }
 }
 
-// Combine of the divided units, a warp per query row.
-template <int D, typename T>
-__global__ void __launch_bounds__(128) paged_chunk_combine_kernel(const __grid_constant__ PagedArgs a,
-                                                                  const __grid_constant__ PcPlan p,
-                                                                  const __grid_constant__ PcSplits splits) {
-  constexpr int kM = kPcUnit, E = D / 32;
+// Combine of the divided units.  W warps a row: one where units have few pieces
+// (4 rows a CTA), kPcMerge of them where a row has many (decode of few requests);
+// warp w takes pieces w, w + W, .. in worker order, the warps' sums are added in
+// warp order.  blockIdx.y: divided unit, blockIdx.x: rows of it.
+template <int D, typename T, bool kFew, int W>
+__global__ void __launch_bounds__(128) paged_merge_kernel(const __grid_constant__ PagedArgs a,
+                                                          const __grid_constant__ PcPlan p,
+                                                          const __grid_constant__ PcSplits splits) {
+  using Shape = PcShape<D, kFew>;
+  constexpr int E = D / 32, kRowsHere = 4 / W;
+  __shared__ float part[W > 1 ? W : 1][D], part_l[W > 1 ? W : 1];
   pdl_release();
-  const int lane = threadIdx.x & 31;
-  const int idx = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const PcSplit& u = splits.unit[idx / (kM * kPcRows)];
-  const int mt = idx / kPcRows % kM, row = idx % kPcRows;
-  const int tok = (u.qb * kM + mt) * p.tokens + row / a.group;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % W;
+  const int idx = blockIdx.x * kRowsHere + (threadIdx.x >> 5) / W;
+  const PcSplit& u = splits.unit[blockIdx.y];
+  const int mt = idx / kPcRows, row = idx % kPcRows;
+  const int tok = (u.qb * Shape::kUnit + mt) * p.tokens + row / a.group;
   pdl_wait();
-  if (row >= p.tokens * a.group || tok >= p.q_len[u.r]) return;
-  // a divided unit is its CTA's last piece except where the CTA began inside it
+  if (row >= p.tokens * a.group || tok >= p.q_len[u.r]) return;  // (uniform over the warps of a row)
+  // the unit is its first worker's last piece, unless that worker begins with it; the others begin inside it
+  const bool inside = p.start[u.c0].r == u.r && p.start[u.c0].h == u.h && p.start[u.c0].qb == u.qb;
   auto at = [&](int c) -> int64_t {
-    const bool first = c > u.c0 || (p.start[c].r == u.r && p.start[c].h == u.h && p.start[c].qb == u.qb);
-    return ((int64_t)(2 * c + (first ? 0 : 1)) * kM + mt) * kPcRows + row;
+    return ((int64_t)(2 * c + (c > u.c0 || inside ? 0 : 1)) * Shape::kUnit + mt) * kPcRows + row;
   };
   float M = -INFINITY;
   for (int c = u.c0 + lane; c <= u.c1; c += 32) M = fmaxf(M, a.part_ml[at(c)].x);
@@ -762,11 +811,11 @@ __global__ void __launch_bounds__(128) paged_chunk_combine_kernel(const __grid_c
   float total = 0.0f, acc[E];
 #pragma unroll
   for (int i = 0; i < E; ++i) acc[i] = 0.0f;
-#pragma unroll 2
-  for (int c = u.c0; c <= u.c1; ++c) {
+#pragma unroll 4
+  for (int c = u.c0 + warp; c <= u.c1; c += W) {
     const int64_t r = at(c);
     const float2 ml = a.part_ml[r];
-    const float f = pg_exp2(ml.x - base);
+    const float f = pg_exp2(ml.x - base);  // a piece without visible keys: 2^-inf = 0
     const float* src = a.part_o + r * D + E * lane;
     total = fmaf(f, ml.y, total);
 #pragma unroll
@@ -774,6 +823,19 @@ __global__ void __launch_bounds__(128) paged_chunk_combine_kernel(const __grid_c
       const float2 v = *reinterpret_cast<const float2*>(src + i);
       acc[i] = fmaf(f, v.x, acc[i]);
       acc[i + 1] = fmaf(f, v.y, acc[i + 1]);
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) part[warp][E * lane + i] = acc[i];
+    if (lane == 0) part_l[warp] = total;
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      total += part_l[w];
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc[i] += part[w][E * lane + i];
     }
   }
   const bool none = M == -INFINITY && total == 0.0f;

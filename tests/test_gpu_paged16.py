@@ -128,6 +128,16 @@ CASES = [
     ([128], [4096], dict(hq=8, hk=2, d=128, page=24)),
     ([40], [100], dict(hq=40, hk=1, d=256, page=128)),
     ([3], [20000], dict(hq=8, hk=1, d=256)),
+    # more than 32 key tiles per SM: few rows on the tensor-memory kernel
+    ([4, 1, 3], [41000, 5003, 130], dict(hq=48, hk=8)),
+    ([2, 1], [50000, 41], dict(hq=24, hk=8, d=128, dtype=torch.float16, page=48)),
+    ([1, 2], [39999, 9000], dict(hq=32, hk=16, d=64, dtype=torch.float16, page=16)),
+    # between 33 and 128 rows per kv head
+    ([20], [3000], dict()),
+    ([21, 6, 13], [21, 1000, 700], dict(page=24)),
+    ([9, 30], [500, 900], dict(hq=16, hk=4, d=128, dtype=torch.float16, page=16)),
+    ([17], [640], dict(hq=35, hk=5, d=64)),
+    ([1, 2], [333, 90], dict(hq=128, hk=1, d=64, page=32)),
 ]
 
 
@@ -266,6 +276,9 @@ WEIGHT_CASES = [
     ([300], [300], 64, dict(hq=12, hk=2, d=128, page=16)),
     ([90, 64], [1200, 64], 17, dict(hq=8, hk=1, d=64, dtype=torch.float16, page=5)),
     ([40], [30], None, dict()),
+    ([4, 2, 1], [40007, 300, 64], None, dict(hq=48, hk=8)),
+    ([2], [45000], 1, dict(hq=24, hk=8, d=128, dtype=torch.float16, page=16)),
+    ([20, 1], [700, 500], 3, dict()),
 ]
 
 

@@ -73,6 +73,7 @@ def test_nothing_to_do_is_accepted(lib):
 
 @pytest.mark.parametrize("kw,status,text", [
     (dict(dtype=0), 2, b"bf16 or fp16"), (dict(d=80), 2, b"64, 128, 256"), (dict(hq=23), 1, b"multiple of Hk"),
+    (dict(hq=520), 2, b"group 130 > 128"),
     (dict(qsl=(0, 2)), 1, b"query layout"), (dict(qsl=(1, 3)), 1, b"query layout"), (dict(qsl=(0, 4, 3), seqs=(5, 5)), 1, b"fall"),
     (dict(seqs=(-1,)), 1, b"negative"), (dict(scale=0.0), 1, b"scale"), (dict(scale=float("inf")), 1, b"scale"),
     (dict(seqs=(17,)), 1, b"cannot cover"), (dict(rows=0), 1, b"block-table rows"), (dict(bt=None), 1, b"block table"),
