@@ -13,8 +13,8 @@
 // own minimum and maximum first, so that neighbouring threads rarely count in
 // the same bin) and narrows it to one bin, three rounds at most.  Then each warp
 // walks its own stretch of the positions twice: it counts its kept keys, and
-// after one prefix sum over the warps numbers them, writes their list and moves
-// their weights.  A stretch of kEvCached weights is held in shared memory; a
+// after one prefix sum over the warps numbers them and writes their list; then the
+// list's weights move, coalesced.  A stretch of kEvCached weights is held in shared memory; a
 // longer request is read again for each round and walked stretch by stretch.
 //
 // evict_move_kernel moves the rows.  Bound by bytes.  To other pages every row
@@ -213,16 +213,19 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       const uint32_t below = (1u << lane) - 1u;
       const uint32_t rank = eq + __popc(eb & below);  // of an equal key
       const uint32_t j = j0 + __popc(sb & below) + (min(rank, need) - min(eq, need));
-      if ((sure || (same && rank < need)) && (int)j < n) {
-        kept[j] = i;
-        float* dst = ev_weight(a, dst_row, h, (int)j);
-        if (dst != nullptr) *dst = ev_w[i - first];
-      }
+      if ((sure || (same && rank < need)) && (int)j < n) kept[j] = i;
       const uint32_t eq_next = eq + __popc(eb);
       j0 += __popc(sb) + (min(eq_next, need) - min(eq, need));
       eq = eq_next;
     }
-    out += a_all + (min(equal + e_all, need) - min(equal, need));
+    const uint32_t out_end = min((uint32_t)n, out + a_all + (min(equal + e_all, need) - min(equal, need)));
+    __syncthreads();  // the stretch's list is written
+#pragma unroll 4
+    for (uint32_t j = out + tid; j < out_end; j += kEvThreads) {
+      float* dst = ev_weight(a, dst_row, h, (int)j);
+      if (dst != nullptr) *dst = ev_w[kept[j] - first];
+    }
+    out = out_end;
     equal += e_all;
   }
 }

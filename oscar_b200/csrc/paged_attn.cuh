@@ -256,22 +256,6 @@ struct PcWalk {
   }
 };
 
-OSCAR_DEVINL uint64_t f2_pack(float a, float b) {
-  return (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
-}
-OSCAR_DEVINL uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-OSCAR_DEVINL uint64_t f2_add(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-OSCAR_DEVINL float f2_lo(uint64_t a) { return __uint_as_float((uint32_t)a); }
-OSCAR_DEVINL float f2_hi(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
-
 OSCAR_DEVINL float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
