@@ -7,15 +7,18 @@
 // pages: the j-th kept position is never below j, so moving in ascending order
 // never overwrites a slot that is still to be read.
 //
-// evict_select_kernel (a CTA per request and head) finds the weight of the last
-// key that stays by histograms over order-preserving 32-bit keys: each round
-// spreads the range that still holds it, [lo, hi], over 2048 bins (the keys'
-// own minimum and maximum first, so that neighbouring threads rarely count in
-// the same bin) and narrows it to one bin, three rounds at most.  Then each warp
-// walks its own stretch of the positions twice: it counts its kept keys, and
-// after one prefix sum over the warps numbers them and writes their list; then the
-// list's weights move, coalesced.  A stretch of kEvCached weights is held in shared memory; a
-// longer request is read again for each round and walked stretch by stretch.
+// evict_select_kernel (a cluster of 8 CTAs per request and head, each with an eighth
+// of the positions) finds the weight of the last key that stays by histograms over
+// order-preserving 32-bit keys: each round spreads the range that still holds it,
+// [lo, hi], over 2048 bins (the keys' own minimum and maximum first, so that
+// neighbouring threads rarely count in the same bin) and narrows it to one bin,
+// three rounds at most; the CTAs add up each other's bins over distributed shared
+// memory.  Then each warp walks its own stretch of the positions twice: it counts
+// its kept keys, and after prefix sums over the warps and the CTAs numbers them
+// and writes their list; then the list's weights move, coalesced.  Bound by
+// instructions: one CTA per request and head took 48 us for 8 x 4 heads of 24580
+// keys and 26 us for 4 heads of 9256.  Up to 8 kEvCached weights are held in shared
+// memory; a longer request is read again for each round and walked piece by piece.
 //
 // evict_move_kernel moves the rows.  Bound by bytes.  To other pages every row
 // is independent.  In place a CTA owns a 128-byte slice of one head's K or V
@@ -24,13 +27,14 @@
 // reads are already in flight.
 #pragma once
 
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace oscar {
 
 constexpr int kEvReqs = 256;
 constexpr int kEvThreads = 1024;
-constexpr int kEvCached = 49152;  // weights in shared memory
+constexpr int kEvCached = 16384;  // weights in a CTA's shared memory
+constexpr int kEvCluster = 8;
 constexpr int kEvBins = 2048;
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvWaves = 8;  // rows per thread and step of the in-place move
@@ -63,41 +67,55 @@ OSCAR_DEVINL uint32_t ev_key(float w) {
   return (b & 0x80000000u) ? ~b : b | 0x80000000u;
 }
 
+// The weight of a position, or null outside the cache.  (The caller flags the error after its loop:
+// an atomic inside would keep the loop's loads from overlapping)
 OSCAR_DEVINL float* ev_weight(const EvictArgs& a, const int32_t* row, int h, int pos) {
   const int page = (int)a.page.div(pos);
-  const int64_t blk = row[page];
-  if (blk < 0 || blk >= a.num_blocks) {
-    flag_error(2u);
-    return nullptr;
-  }
+  const int64_t blk = __ldg(row + page);
+  if (blk < 0 || blk >= a.num_blocks) return nullptr;
   return a.weights + (blk * a.hk + h) * a.bs + (pos - page * a.bs);
+}
+
+OSCAR_DEVINL uint2 ev_remote2(uint32_t addr, uint32_t rank) {  // two words of CTA `rank`'s shared memory
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(pc_map(addr, rank)) : "memory");
+  return v;
 }
 
 __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_constant__ EvictArgs a,
                                                                   const __grid_constant__ EvictPlan p) {
   extern __shared__ __align__(16) float ev_w[];
-  __shared__ uint32_t bins[kEvBins];
+  __shared__ __align__(8) uint32_t bins[kEvBins];
   __shared__ uint32_t warp_sum[2][32];
-  __shared__ uint32_t range[2], pick[2];
+  __shared__ __align__(8) uint32_t mine[2];  // for the other CTAs: minimum and maximum, then kept and equal keys
+  __shared__ uint32_t pick[2];
   pdl_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r = blockIdx.x, h = blockIdx.y;
+  const int rank = (int)pc_rank();
+  const int r = blockIdx.x / kEvCluster, h = blockIdx.y;
   const int seq = p.seq[r];
   const int32_t* src_row = a.table + (int64_t)p.req_id[r] * a.table_stride;
   const int32_t* dst_row = a.dst + (int64_t)p.req_id[r] * a.dst_stride;
   int32_t* kept = a.kept + ((int64_t)p.req_id[r] * a.hk + h) * a.kept_stride;
   const int n = min(seq, a.keep);
   const bool all = seq <= a.keep;
-  if (tid == 0) range[0] = 0xffffffffu, range[1] = 0u;
+  constexpr int kPiece = kEvCluster * kEvCached;
+  bool bad = false;
+  if (tid == 0) mine[0] = 0xffffffffu, mine[1] = 0u;
   pdl_wait();
-  for (int j = n + tid; j < a.kept_stride; j += kEvThreads) kept[j] = -1;
-  // the weights of positions [first, first + kEvCached) to shared memory
+  for (int j = n + rank * kEvThreads + tid; j < a.kept_stride; j += kEvCluster * kEvThreads) kept[j] = -1;
+  // this CTA's positions of the piece that begins at `first`, and their weights to shared memory
+  int from = 0, to = 0;
   auto load = [&](int first) {
-    const int end = min(seq, first + kEvCached);
-#pragma unroll 8
-    for (int i = first + tid; i < end; i += kEvThreads) {
+    const int end = min(seq, first + kPiece);
+    const int per = ((end - first + kEvCluster - 1) / kEvCluster + 31) / 32 * 32;
+    from = min(end, first + rank * per);
+    to = min(end, from + per);
+#pragma unroll 4
+    for (int i = from + tid; i < to; i += kEvThreads) {
       const float* w = ev_weight(a, src_row, h, i);
-      ev_w[i - first] = w == nullptr ? 0.0f : *w;
+      bad = bad || w == nullptr;
+      ev_w[i - from] = w == nullptr ? 0.0f : *w;
     }
     __syncthreads();
   };
@@ -106,19 +124,19 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
   // the key value at which the list is full, and how many of the keys that equal it stay
   const int lo_pos = a.sink, hi_pos = seq - a.recent;
   uint32_t threshold = 0, need = (uint32_t)max(0, a.keep - a.sink - a.recent);
-  // calls f(key) for the keys between sink and recent, in any order
+  // calls f(key) for this CTA's keys between sink and recent, in any order
   auto each = [&](auto&& f) {
-    for (int first = 0; first < seq; first += kEvCached) {
-      if (seq > kEvCached) {
+    for (int first = 0; first < seq; first += kPiece) {
+      if (seq > kPiece) {
         __syncthreads();
         load(first);
       }
-      const int from = max(lo_pos, first), to = min(hi_pos, min(seq, first + kEvCached));
+      const int i0 = max(lo_pos, from), i1 = min(hi_pos, to);
 #pragma unroll 4
-      for (int i = from + tid; i < to; i += kEvThreads) f(ev_key(ev_w[i - first]));
+      for (int i = i0 + tid; i < i1; i += kEvThreads) f(ev_key(ev_w[i - from]));
     }
   };
-  if (!all && need > 0) {
+  if (!all && need > 0) {  // (the same for all CTAs of the cluster)
     uint32_t least = 0xffffffffu, most = 0u;
     each([&](uint32_t key) {
       least = min(least, key);
@@ -127,11 +145,12 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
-      atomicMin(&range[0], least);
-      atomicMax(&range[1], most);
+      atomicMin(&mine[0], least);
+      atomicMax(&mine[1], most);
     }
-    __syncthreads();
-    uint32_t lo = range[0], hi = range[1];
+    pc_cluster_sync();
+    const uint2 theirs = ev_remote2(smem_u32(mine), lane % kEvCluster);
+    uint32_t lo = __reduce_min_sync(0xffffffffu, theirs.x), hi = __reduce_max_sync(0xffffffffu, theirs.y);
 #pragma unroll 1
     while (lo < hi) {
       // bins of 2^shift keys, at most 2048 of them
@@ -141,10 +160,16 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       each([&](uint32_t key) {
         if (key >= lo && key <= hi) atomicAdd(&bins[(key - lo) >> shift], 1u);
       });
-      __syncthreads();
-      // count from the top: thread t holds bins 2 t' + 1 and 2 t' in descending order
+      pc_cluster_sync();
+      // count from the top: thread t holds bins 2 t' + 1 and 2 t' in descending order, of all CTAs
       const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
-      const uint32_t c1 = bins[b1], c0 = bins[b0];
+      uint32_t c1 = 0, c0 = 0;
+#pragma unroll
+      for (int c = 0; c < kEvCluster; ++c) {
+        const uint2 v = ev_remote2(smem_u32(&bins[b0]), c);
+        c0 += v.x;
+        c1 += v.y;
+      }
       uint32_t sum = c1 + c0;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -153,41 +178,40 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       }
       if (lane == 31) warp_sum[0][warp] = sum;
       __syncthreads();
-      uint32_t before = sum - (c1 + c0);
-      for (int w = 0; w < warp; ++w) before += warp_sum[0][w];
+      uint32_t before = lane < warp ? warp_sum[0][lane] : 0u;
+      before = __reduce_add_sync(0xffffffffu, before) + sum - (c1 + c0);
       if (before < need && before + c1 >= need) pick[0] = b1, pick[1] = need - before;
       else if (before + c1 < need && before + c1 + c0 >= need) pick[0] = b0, pick[1] = need - before - c1;
       __syncthreads();
       lo += pick[0] << shift;
       hi = min(hi, lo + ((1u << shift) - 1u));
       need = pick[1];
-      __syncthreads();
+      pc_cluster_sync();  // every CTA has read the bins
     }
     threshold = lo;
   }
 
   // ordered walk: the kept keys are the fixed ones, those above the threshold and the first `need`
   // that equal it
-  uint32_t out = 0, equal = 0;  // kept keys and equal keys of the stretches before
+  uint32_t out = 0, equal = 0;  // kept keys and equal keys of the pieces before
   const bool chooses = !all && a.keep > a.sink + a.recent;
-  for (int first = 0; first < seq; first += kEvCached) {
-    if (seq > kEvCached) {
+  for (int first = 0; first < seq; first += kPiece) {
+    if (seq > kPiece) {
       __syncthreads();
       load(first);
     }
-    const int end = min(seq, first + kEvCached);
-    const int per = ((end - first + 31) / 32 + 31) / 32 * 32;  // positions of a warp
-    const int from = first + warp * per, to = min(end, from + per);
+    const int per = ((to - from + 31) / 32 + 31) / 32 * 32;  // positions of a warp
+    const int w0 = min(to, from + warp * per), w1 = min(to, w0 + per);
     auto classify = [&](int i, bool& sure, bool& same) {
       sure = same = false;
-      if (i >= to) return;
+      if (i >= w1) return;
       const bool fixed = all || i < lo_pos || i >= hi_pos;
-      const uint32_t key = ev_key(ev_w[i - first]);
+      const uint32_t key = ev_key(ev_w[i - from]);
       sure = fixed || (chooses && key > threshold);
       same = !fixed && chooses && key == threshold;
     };
     uint32_t sures = 0, sames = 0;
-    for (int i0 = from; i0 < to; i0 += 32) {
+    for (int i0 = w0; i0 < w1; i0 += 32) {
       bool sure, same;
       classify(i0 + lane, sure, same);
       sures += __popc(__ballot_sync(0xffffffffu, sure));
@@ -195,7 +219,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     }
     if (lane == 0) warp_sum[0][warp] = sures, warp_sum[1][warp] = sames;
     __syncthreads();
-    // before this warp: kept keys that do not depend on the rank of equal ones, and equal keys
+    // before this warp in the CTA: kept keys that do not depend on the rank of equal ones, and equal keys
     uint32_t a_cnt = warp_sum[0][lane], e_cnt = warp_sum[1][lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -203,31 +227,43 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       if (lane >= o) a_cnt += x, e_cnt += y;
     }
     const uint32_t a_all = __shfl_sync(0xffffffffu, a_cnt, 31), e_all = __shfl_sync(0xffffffffu, e_cnt, 31);
-    uint32_t eq = equal + __shfl_sync(0xffffffffu, e_cnt, warp) - sames;
-    uint32_t j0 = out + __shfl_sync(0xffffffffu, a_cnt, warp) - sures + (min(eq, need) - min(equal, need));
-    for (int i0 = from; i0 < to; i0 += 32) {
+    if (tid == 0) mine[0] = a_all, mine[1] = e_all;
+    pc_cluster_sync();
+    // and in the CTAs before this one
+    const uint2 theirs = ev_remote2(smem_u32(mine), lane % kEvCluster);
+    const uint32_t a_before = __reduce_add_sync(0xffffffffu, lane < rank ? theirs.x : 0u);
+    const uint32_t e_before = equal + __reduce_add_sync(0xffffffffu, lane < rank ? theirs.y : 0u);
+    const uint32_t a_piece = __reduce_add_sync(0xffffffffu, lane < kEvCluster ? theirs.x : 0u);
+    const uint32_t e_piece = __reduce_add_sync(0xffffffffu, lane < kEvCluster ? theirs.y : 0u);
+    const uint32_t cta_out = out + a_before + (min(e_before, need) - min(equal, need));
+    uint32_t eq = e_before + __shfl_sync(0xffffffffu, e_cnt, warp) - sames;
+    uint32_t j0 = cta_out + __shfl_sync(0xffffffffu, a_cnt, warp) - sures + (min(eq, need) - min(e_before, need));
+    for (int i0 = w0; i0 < w1; i0 += 32) {
       const int i = i0 + lane;
       bool sure, same;
       classify(i, sure, same);
       const uint32_t sb = __ballot_sync(0xffffffffu, sure), eb = __ballot_sync(0xffffffffu, same);
       const uint32_t below = (1u << lane) - 1u;
-      const uint32_t rank = eq + __popc(eb & below);  // of an equal key
-      const uint32_t j = j0 + __popc(sb & below) + (min(rank, need) - min(eq, need));
-      if ((sure || (same && rank < need)) && (int)j < n) kept[j] = i;
+      const uint32_t order = eq + __popc(eb & below);  // of an equal key
+      const uint32_t j = j0 + __popc(sb & below) + (min(order, need) - min(eq, need));
+      if ((sure || (same && order < need)) && (int)j < n) kept[j] = i;
       const uint32_t eq_next = eq + __popc(eb);
       j0 += __popc(sb) + (min(eq_next, need) - min(eq, need));
       eq = eq_next;
     }
-    const uint32_t out_end = min((uint32_t)n, out + a_all + (min(equal + e_all, need) - min(equal, need)));
-    __syncthreads();  // the stretch's list is written
+    const uint32_t cta_end = min((uint32_t)n, cta_out + a_all + (min(e_before + e_all, need) - min(e_before, need)));
+    __syncthreads();  // this CTA's part of the list is written (and all weights of the piece are in shared memory)
 #pragma unroll 4
-    for (uint32_t j = out + tid; j < out_end; j += kEvThreads) {
+    for (uint32_t j = cta_out + tid; j < cta_end; j += kEvThreads) {
       float* dst = ev_weight(a, dst_row, h, (int)j);
-      if (dst != nullptr) *dst = ev_w[kept[j] - first];
+      bad = bad || dst == nullptr;
+      if (dst != nullptr) *dst = ev_w[kept[j] - from];
     }
-    out = out_end;
-    equal += e_all;
+    out = min((uint32_t)n, out + a_piece + (min(equal + e_piece, need) - min(equal, need)));
+    equal += e_piece;
+    pc_cluster_sync();  // the counts have been read; no CTA ends while another reads its shared memory
   }
+  if (bad) flag_error(2u);
 }
 
 // To other pages: a warp per kept row and K or V, 16 bytes per lane and step.

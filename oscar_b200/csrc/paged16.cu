@@ -595,12 +595,12 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
     for (; r < num_requests && p.num_req < oscar::kEvReqs; ++r) {
       p.req_id[p.num_req] = r;
       p.seq[p.num_req++] = seqs[r];
-      longest = std::max(longest, std::min(seqs[r], oscar::kEvCached));
+      longest = std::max(longest, std::min(oscar::kEvCached, (seqs[r] + oscar::kEvCluster - 1) / oscar::kEvCluster + 31));
       moved = std::max(moved, std::min(seqs[r], keep));
     }
     allow_smem<oscar::evict_select_kernel>(oscar::kEvCached * sizeof(float));
-    launch_pdl(oscar::evict_select_kernel, dim3(p.num_req, num_kv_heads), dim3(oscar::kEvThreads),
-               std::max(16, longest * (int)sizeof(float)), s, a, p);
+    launch_pdl_cluster(oscar::kEvCluster, oscar::evict_select_kernel, dim3(p.num_req * oscar::kEvCluster, num_kv_heads),
+                       dim3(oscar::kEvThreads), std::max(16, longest * (int)sizeof(float)), s, a, p);
     st = cuda_status("evict_select_kernel");
     if (st) return st;
     if (moved == 0) continue;

@@ -461,7 +461,8 @@ EVICT_CASES = [
     ([2500], 50, 25, 25, dict(hk=2, d=64, page=5, dtype=torch.float16)),     # nothing between sink and recent
     ([777], 1, 0, 0, dict(hk=8, d=64, page=1)),
     ([777], 776, 0, 1, dict(d=128, page=48, dtype=torch.float16)),
-    ([60000], 33000, 10, 100, dict(hk=1, d=64, page=64)),                    # more keys than shared memory holds
+    ([60000], 33000, 10, 100, dict(hk=1, d=64, page=64)),
+    ([150000, 300], 77000, 10, 100, dict(hk=1, d=64, page=64)),              # more keys than shared memory holds
 ]
 
 
