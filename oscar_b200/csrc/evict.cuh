@@ -37,6 +37,7 @@ constexpr int kEvCached = 16384;  // weights in a CTA's shared memory
 constexpr int kEvCluster = 8;
 constexpr int kEvBins = 2048;
 constexpr int kEvMoveThreads = 256;
+constexpr int kEvRows = 4;   // rows per thread and step of the copy
 constexpr int kEvWaves = 8;  // rows per thread and step of the in-place move
 
 struct EvictPlan {
@@ -266,7 +267,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
   if (bad) flag_error(2u);
 }
 
-// To other pages: a warp per kept row and K or V, 16 bytes per lane and step.
+// To other pages: 16 bytes of a kept row's K and V per lane, 4 rows in flight; the list and the
+// block tables of a step are read while the rows of the step before it move.
 __global__ void __launch_bounds__(kEvMoveThreads) evict_copy_kernel(const __grid_constant__ EvictArgs a,
                                                                     const __grid_constant__ EvictPlan p) {
   pdl_release();
@@ -276,32 +278,47 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_copy_kernel(const __grid
   const int32_t* src_row = a.table + (int64_t)p.req_id[r] * a.table_stride;
   const int32_t* dst_row = a.dst + (int64_t)p.req_id[r] * a.dst_stride;
   const int32_t* kept = a.kept + ((int64_t)p.req_id[r] * a.hk + h) * a.kept_stride;
-  const int c = threadIdx.x % lanes, rows = kEvMoveThreads / lanes;
+  const int c = threadIdx.x % lanes, rows = kEvMoveThreads / lanes, mine = threadIdx.x / lanes;
+  const int step = gridDim.x * rows * kEvRows;
+  uint8_t* const k = a.k + h * a.kh + 16 * c;
+  uint8_t* const v = a.v + h * a.vh + 16 * c;
   pdl_wait();
-#pragma unroll 1
-  for (int j0 = blockIdx.x * rows * 4; j0 < n; j0 += gridDim.x * rows * 4) {
-    uint4 kv[4], vv[4];
-    int64_t to_blk[4];
-    int to_off[4];
+  struct Move {
+    int sb, so, db, dof;  // source and destination block and place; sb < 0: nothing to move
+  } m[kEvRows];
+  auto look_up = [&](int j0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int j = j0 + i * rows + threadIdx.x / lanes;
-      to_blk[i] = -1;
+    for (int i = 0; i < kEvRows; ++i) {
+      const int j = j0 + i * rows + mine;
+      m[i].sb = -1;
       if (j >= n) continue;
-      const int s = kept[j];
-      const int64_t sb = src_row[a.page.div(s)], db = dst_row[a.page.div(j)];
+      const int s = kept[j], sp = (int)a.page.div(s), dp = (int)a.page.div(j);
+      const int sb = src_row[sp], db = dst_row[dp];
       if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;  // flagged by the selection
-      const int so = (int)a.page.mod(s);
-      kv[i] = *reinterpret_cast<const uint4*>(a.k + sb * a.kb + so * a.kt + h * a.kh + 16 * c);
-      vv[i] = *reinterpret_cast<const uint4*>(a.v + sb * a.vb + so * a.vt + h * a.vh + 16 * c);
-      to_blk[i] = db;
-      to_off[i] = (int)a.page.mod(j);
+      m[i] = Move{sb, s - sp * a.bs, db, j - dp * a.bs};
     }
+  };
+  int j0 = blockIdx.x * rows * kEvRows;
+  look_up(j0);
+#pragma unroll 1
+  for (; j0 < n; j0 += step) {
+    uint4 kv[kEvRows], vv[kEvRows];
+    int64_t to_k[kEvRows], to_v[kEvRows];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (to_blk[i] < 0) continue;
-      *reinterpret_cast<uint4*>(a.k + to_blk[i] * a.kb + to_off[i] * a.kt + h * a.kh + 16 * c) = kv[i];
-      *reinterpret_cast<uint4*>(a.v + to_blk[i] * a.vb + to_off[i] * a.vt + h * a.vh + 16 * c) = vv[i];
+    for (int i = 0; i < kEvRows; ++i) {
+      to_k[i] = -1;
+      if (m[i].sb < 0) continue;
+      kv[i] = __ldcs(reinterpret_cast<const uint4*>(k + m[i].sb * a.kb + m[i].so * a.kt));
+      vv[i] = __ldcs(reinterpret_cast<const uint4*>(v + m[i].sb * a.vb + m[i].so * a.vt));
+      to_k[i] = m[i].db * a.kb + m[i].dof * a.kt;
+      to_v[i] = m[i].db * a.vb + m[i].dof * a.vt;
+    }
+    look_up(j0 + step);
+#pragma unroll
+    for (int i = 0; i < kEvRows; ++i) {
+      if (to_k[i] < 0) continue;
+      __stcs(reinterpret_cast<uint4*>(k + to_k[i]), kv[i]);
+      __stcs(reinterpret_cast<uint4*>(v + to_v[i]), vv[i]);
     }
   }
 }

@@ -609,9 +609,12 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
                  dim3(oscar::kEvMoveThreads), 0, s, a, p);
       st = cuda_status("evict_move_kernel");
     } else {
-      const int rows = oscar::kEvMoveThreads / (a.row_bytes / 16) * 4;
-      launch_pdl(oscar::evict_copy_kernel, dim3((moved + rows - 1) / rows, p.num_req * num_kv_heads),
-                 dim3(oscar::kEvMoveThreads), 0, s, a, p);
+      // about eight CTAs per SM over all heads, each with several steps
+      const int rows = oscar::kEvMoveThreads / (a.row_bytes / 16) * oscar::kEvRows;
+      const int heads = p.num_req * num_kv_heads, most = (moved + rows - 1) / rows;
+      const int want = (8 * std::max(device_info().sms, 1) + heads - 1) / heads;
+      launch_pdl(oscar::evict_copy_kernel, dim3(std::min(most, std::max(want, 1)), heads), dim3(oscar::kEvMoveThreads), 0, s,
+                 a, p);
       st = cuda_status("evict_copy_kernel");
     }
     if (st) return st;
