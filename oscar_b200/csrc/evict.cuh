@@ -10,15 +10,18 @@
 // evict_select_kernel (a cluster of 8 CTAs per request and head, each with an eighth
 // of the positions) finds the weight of the last key that stays by histograms over
 // order-preserving 32-bit keys: each round spreads the range that still holds it,
-// [lo, hi], over 2048 bins (the keys' own minimum and maximum first, so that
+// [lo, hi], over 256 bins (the keys' own minimum and maximum first, so that
 // neighbouring threads rarely count in the same bin) and narrows it to one bin,
-// three rounds at most; the CTAs add up each other's bins over distributed shared
-// memory.  Then each warp walks its own stretch of the positions twice: it counts
-// its kept keys, and after prefix sums over the warps and the CTAs numbers them
-// and writes their list; then the list's weights move, coalesced.  Bound by
-// instructions: one CTA per request and head took 48 us for 8 x 4 heads of 24580
-// keys and 26 us for 4 heads of 9256.  Up to 8 kEvCached weights are held in shared
-// memory; a longer request is read again for each round and walked piece by piece.
+// four rounds at most; the CTAs add up each other's bins over distributed shared
+// memory (2048 bins and three rounds: those reads cost more than a round saves).
+// Then each warp walks its own stretch of the positions twice: it counts its kept
+// keys, and after prefix sums over the warps and the CTAs numbers them and writes
+// their list; then the list's weights move, coalesced.  Bound by instructions: one
+// CTA per request and head took 48 us for 8 x 4 heads of 24580 keys and 26 us for 4
+// heads of 9256.  With the copy, 8 x 4 heads of 24580 keys cut to 12288 take 178 us
+// (512 threads a CTA: 183), 4 heads of 9256 cut to 4096 take 25 us.  Up to 8 kEvCached
+// weights are held in shared memory; a longer request is read again for each round
+// and walked piece by piece.
 //
 // evict_move_kernel moves the rows.  Bound by bytes.  To other pages every row
 // is independent.  In place a CTA owns a 128-byte slice of one head's K or V
@@ -35,7 +38,7 @@ constexpr int kEvReqs = 256;
 constexpr int kEvThreads = 1024;
 constexpr int kEvCached = 16384;  // weights in a CTA's shared memory
 constexpr int kEvCluster = 8;
-constexpr int kEvBins = 2048;
+constexpr int kEvBins = 256;
 constexpr int kEvMoveThreads = 256;
 constexpr int kEvRows = 4;   // rows per thread and step of the copy
 constexpr int kEvWaves = 8;  // rows per thread and step of the in-place move
@@ -77,6 +80,11 @@ OSCAR_DEVINL float* ev_weight(const EvictArgs& a, const int32_t* row, int h, int
   return a.weights + (blk * a.hk + h) * a.bs + (pos - page * a.bs);
 }
 
+OSCAR_DEVINL uint32_t ev_remote(uint32_t addr, uint32_t rank) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(pc_map(addr, rank)) : "memory");
+  return v;
+}
 OSCAR_DEVINL uint2 ev_remote2(uint32_t addr, uint32_t rank) {  // two words of CTA `rank`'s shared memory
   uint2 v;
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(pc_map(addr, rank)) : "memory");
@@ -88,7 +96,10 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
   extern __shared__ __align__(16) float ev_w[];
   __shared__ __align__(8) uint32_t bins[kEvBins];
   __shared__ uint32_t warp_sum[2][32];
-  __shared__ __align__(8) uint32_t mine[2];  // for the other CTAs: minimum and maximum, then kept and equal keys
+  // for the other CTAs; two places, since with all keys equal nothing but the walk's own barrier lies
+  // between a slow CTA's read of the range and a fast CTA's counts
+  __shared__ __align__(8) uint32_t range[2];   // minimum and maximum
+  __shared__ __align__(8) uint32_t counts[2];  // kept and equal keys of a piece
   __shared__ uint32_t pick[2];
   pdl_release();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -102,7 +113,7 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
   const bool all = seq <= a.keep;
   constexpr int kPiece = kEvCluster * kEvCached;
   bool bad = false;
-  if (tid == 0) mine[0] = 0xffffffffu, mine[1] = 0u;
+  if (tid == 0) range[0] = 0xffffffffu, range[1] = 0u;
   pdl_wait();
   for (int j = n + rank * kEvThreads + tid; j < a.kept_stride; j += kEvCluster * kEvThreads) kept[j] = -1;
   // this CTA's positions of the piece that begins at `first`, and their weights to shared memory
@@ -146,32 +157,31 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     least = __reduce_min_sync(0xffffffffu, least);
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) {
-      atomicMin(&mine[0], least);
-      atomicMax(&mine[1], most);
+      atomicMin(&range[0], least);
+      atomicMax(&range[1], most);
     }
     pc_cluster_sync();
-    const uint2 theirs = ev_remote2(smem_u32(mine), lane % kEvCluster);
+    const uint2 theirs = ev_remote2(smem_u32(range), lane % kEvCluster);
     uint32_t lo = __reduce_min_sync(0xffffffffu, theirs.x), hi = __reduce_max_sync(0xffffffffu, theirs.y);
 #pragma unroll 1
     while (lo < hi) {
-      // bins of 2^shift keys, at most 2048 of them
-      const int shift = max(0, 32 - __clz(hi - lo) - 11);
+      // bins of 2^shift keys, at most 256 of them
+      const int shift = max(0, 32 - __clz(hi - lo) - 8);
       for (int i = tid; i < kEvBins; i += kEvThreads) bins[i] = 0;
       __syncthreads();
       each([&](uint32_t key) {
         if (key >= lo && key <= hi) atomicAdd(&bins[(key - lo) >> shift], 1u);
       });
       pc_cluster_sync();
-      // count from the top: thread t holds bins 2 t' + 1 and 2 t' in descending order, of all CTAs
-      const int b1 = kEvBins - 1 - 2 * tid, b0 = b1 - 1;
-      uint32_t c1 = 0, c0 = 0;
+      // count from the top: thread t holds bin 255 - t of all CTAs
+      static_assert(kEvBins <= kEvThreads, "a thread per bin");
+      const int bin = kEvBins - 1 - tid;
+      uint32_t own = 0;
+      if (bin >= 0) {
 #pragma unroll
-      for (int c = 0; c < kEvCluster; ++c) {
-        const uint2 v = ev_remote2(smem_u32(&bins[b0]), c);
-        c0 += v.x;
-        c1 += v.y;
+        for (int t = 0; t < kEvCluster; ++t) own += ev_remote(smem_u32(&bins[bin]), t);
       }
-      uint32_t sum = c1 + c0;
+      uint32_t sum = own;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t x = __shfl_up_sync(0xffffffffu, sum, o);
@@ -180,12 +190,11 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       if (lane == 31) warp_sum[0][warp] = sum;
       __syncthreads();
       uint32_t before = lane < warp ? warp_sum[0][lane] : 0u;
-      before = __reduce_add_sync(0xffffffffu, before) + sum - (c1 + c0);
-      if (before < need && before + c1 >= need) pick[0] = b1, pick[1] = need - before;
-      else if (before + c1 < need && before + c1 + c0 >= need) pick[0] = b0, pick[1] = need - before - c1;
+      before = __reduce_add_sync(0xffffffffu, before) + sum - own;
+      if (before < need && before + own >= need) pick[0] = bin, pick[1] = need - before;
       __syncthreads();
       lo += pick[0] << shift;
-      hi = min(hi, lo + ((1u << shift) - 1u));
+      hi = lo + min(hi - lo, (1u << shift) - 1u);  // (lo + 2^shift may pass 32 bits)
       need = pick[1];
       pc_cluster_sync();  // every CTA has read the bins
     }
@@ -201,7 +210,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
       __syncthreads();
       load(first);
     }
-    const int per = ((to - from + 31) / 32 + 31) / 32 * 32;  // positions of a warp
+    constexpr int kWarps = kEvThreads / 32;
+    const int per = ((to - from + kWarps - 1) / kWarps + 31) / 32 * 32;  // positions of a warp
     const int w0 = min(to, from + warp * per), w1 = min(to, w0 + per);
     auto classify = [&](int i, bool& sure, bool& same) {
       sure = same = false;
@@ -221,17 +231,17 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     if (lane == 0) warp_sum[0][warp] = sures, warp_sum[1][warp] = sames;
     __syncthreads();
     // before this warp in the CTA: kept keys that do not depend on the rank of equal ones, and equal keys
-    uint32_t a_cnt = warp_sum[0][lane], e_cnt = warp_sum[1][lane];
+    uint32_t a_cnt = lane < kWarps ? warp_sum[0][lane] : 0u, e_cnt = lane < kWarps ? warp_sum[1][lane] : 0u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const uint32_t x = __shfl_up_sync(0xffffffffu, a_cnt, o), y = __shfl_up_sync(0xffffffffu, e_cnt, o);
       if (lane >= o) a_cnt += x, e_cnt += y;
     }
     const uint32_t a_all = __shfl_sync(0xffffffffu, a_cnt, 31), e_all = __shfl_sync(0xffffffffu, e_cnt, 31);
-    if (tid == 0) mine[0] = a_all, mine[1] = e_all;
+    if (tid == 0) counts[0] = a_all, counts[1] = e_all;
     pc_cluster_sync();
     // and in the CTAs before this one
-    const uint2 theirs = ev_remote2(smem_u32(mine), lane % kEvCluster);
+    const uint2 theirs = ev_remote2(smem_u32(counts), lane % kEvCluster);
     const uint32_t a_before = __reduce_add_sync(0xffffffffu, lane < rank ? theirs.x : 0u);
     const uint32_t e_before = equal + __reduce_add_sync(0xffffffffu, lane < rank ? theirs.y : 0u);
     const uint32_t a_piece = __reduce_add_sync(0xffffffffu, lane < kEvCluster ? theirs.x : 0u);

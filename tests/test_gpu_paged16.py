@@ -521,6 +521,27 @@ def test_evict_cache(seqs, keep, sink, recent, opts, values, in_place):
     assert kernels.device_error(dev) == 0
 
 
+def test_evict_equal_weights_in_many_requests():
+    """All keys weigh the same: the range of the weights is one value, and the CTAs that share a
+    request go straight from its exchange to that of the counts."""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    for base in (33, 300, 2000):
+        seqs = [base + 7 * r for r in range(48)]
+        keep = base // 2
+        kc, vc, table = make_pool(gen, seqs, 16, 4, 64, torch.bfloat16, poison=False)
+        for value in (0.0, 1.5, math.nan):
+            for _ in range(3):
+                w = torch.full((kc.shape[0], 4, 16), value, device="cuda")
+                kept = kernels.evict_cache(kc, vc, w, table, seqs, keep, sink=2, recent=5)
+                for r, seq in enumerate(seqs):
+                    want = list(range(keep - 5)) + list(range(seq - 5, seq))
+                    assert kept[r].tolist() == [want] * 4
+    assert kernels.device_error(dev) == 0
+
+
 def test_evict_strided_caches():
     from oscar_b200 import kernels
 
