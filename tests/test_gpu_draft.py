@@ -1,0 +1,149 @@
+"""DraftLayer: prompt, draft steps, eviction and steps after it, against a plain
+64-bit restatement that keeps every head's rows in lists.
+
+Tolerance: the rows that reach the attention are 16-bit; a rounding that falls
+the other way moves a key or value by one unit (2 u relative).  Scores then move
+by at most 2 u sum |q k| scale = SHIFT below, which weighs the output like
+test_gpu_paged16's score error; the rest is that test's bound."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from gpu_helpers import need_gpu
+
+pytestmark = pytest.mark.gpu
+
+HQ, HK, D, PAGE, ROT = 8, 2, 64, 16, 32
+U = torch.finfo(torch.bfloat16).eps / 2
+
+
+def norm_rope(x, w, cos_sin, positions):
+    x = x.double()
+    y = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+    row = cos_sin.double()[positions][:, None]
+    c, s, h = row[..., :ROT // 2], row[..., ROT // 2:], ROT // 2
+    return torch.cat([y[..., :h] * c - y[..., h:ROT] * s, y[..., h:ROT] * c + y[..., :h] * s, y[..., ROT:]], -1)
+
+
+class Plain:
+    """Rows, weights and original positions per request and head."""
+
+    def __init__(self, n):
+        self.k = [[torch.zeros(0, D, dtype=torch.float64, device="cuda") for _ in range(HK)] for _ in range(n)]
+        self.v = [[torch.zeros(0, D, dtype=torch.float64, device="cuda") for _ in range(HK)] for _ in range(n)]
+        self.w = [[torch.zeros(0, dtype=torch.float64, device="cuda") for _ in range(HK)] for _ in range(n)]
+
+    def step(self, q, k, v, lens):
+        outs, sizes, at = [], [], 0
+        for r, m in enumerate(lens):
+            o = torch.zeros(m, HQ, D, dtype=torch.float64, device="cuda")
+            size = torch.zeros_like(o)
+            for h in range(HK):
+                self.k[r][h] = torch.cat([self.k[r][h], k[at:at + m, h]])
+                self.v[r][h] = torch.cat([self.v[r][h], v[at:at + m, h]])
+                self.w[r][h] = torch.cat([self.w[r][h], torch.zeros(m, dtype=torch.float64, device="cuda")])
+                g = slice(h * (HQ // HK), (h + 1) * (HQ // HK))
+                x = torch.einsum("mgd,kd->mgk", q[at:at + m, g], self.k[r][h]) * D**-0.5
+                n = self.k[r][h].shape[0]
+                hidden = torch.arange(n, device="cuda")[None] > torch.arange(n - m, n, device="cuda")[:, None]
+                p = torch.softmax(x.masked_fill(hidden[:, None], -math.inf), -1)
+                o[:, g] = torch.einsum("mgk,kd->mgd", p, self.v[r][h])
+                size[:, g] = torch.einsum("mgk,kd->mgd", p, self.v[r][h].abs())
+                self.w[r][h] += p.sum((0, 1))
+            outs.append(o)
+            sizes.append(size)
+            at += m
+        return torch.cat(outs), torch.cat(sizes)
+
+    def take(self, kept):
+        for r in range(len(self.k)):
+            for h in range(HK):
+                c = kept[r, h][kept[r, h] >= 0].long()
+                self.k[r][h], self.v[r][h], self.w[r][h] = self.k[r][h][c], self.v[r][h][c], self.w[r][h][c]
+
+
+def test_prompt_steps_eviction_and_steps_after_it():
+    from oscar_b200 import kernels
+    from oscar_b200.draft import DraftLayer, slots_of
+
+    dev = need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    n, width = 3, 16
+    pool = torch.full((n * width + 2, 2, PAGE, HK, D), math.nan, device="cuda").to(torch.bfloat16)
+    perm = torch.randperm(n * width, generator=gen, device="cuda")
+    table = perm.to(torch.int32).view(n, width)
+    wq, wk = (torch.randn(D, generator=gen, device="cuda") * 0.1 for _ in range(2))
+    angle = torch.arange(400, device="cuda", dtype=torch.float64)[:, None] / 1e4 ** (
+        torch.arange(0, ROT, 2, device="cuda", dtype=torch.float64) / ROT)
+    cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float()
+    layer = DraftLayer(HQ, (pool[:, 0], pool[:, 1]), wq, wk, cos_sin, weight_offset=1.0, keep=40, sink=3, recent=8)
+    plain = Plain(n)
+    cached, position = [0] * n, [0] * n
+
+    def step(lens):
+        nonlocal cached, position
+        total = sum(lens)
+        qkv = torch.randn(total, HQ + 2 * HK, D, generator=gen, device="cuda").to(torch.bfloat16)
+        q, k, v = qkv.split([HQ, HK, HK], 1)
+        positions = torch.cat([torch.arange(p, p + m, device="cuda") for p, m in zip(position, lens)])
+        cached = [c + m for c, m in zip(cached, lens)]
+        position = [p + m for p, m in zip(position, lens)]
+        qsl = np.concatenate([[0], np.cumsum(lens)])
+        out, lse = layer.forward(q, k, v, positions, slots_of(table, lens, cached, PAGE), table, qsl, cached)
+        assert torch.isfinite(out.float()).all() and torch.isfinite(lse).all()
+        bf = lambda t: t.to(torch.bfloat16).double()  # noqa: E731
+        want, size = plain.step(bf(norm_rope(q, wq, cos_sin, positions)), bf(norm_rope(k, wk, cos_sin, positions)),
+                                v.double(), lens)
+        # sum |q k| scale <= |q| |k| scale with norms of at most 1.5 sqrt(D)
+        shift = 2 * U * 2.25 * D * D**-0.5
+        assert ((out.double() - want).abs() <= U * (size + want.abs()) * 1.01 + 2 * (shift + 2e-4) * size).all()
+
+    step([100, 61, 30])
+    for _ in range(3):
+        step([2, 1, 4])
+    # the layer's weights are those of the plain steps, so the same keys stay
+    before = cached
+    new, kept = layer.evict(table, cached)
+    assert new == [40, 40, 40] and kept.shape == (n, HK, 40)
+    for r in range(n):
+        for h in range(HK):
+            c = kept[r, h].long()
+            assert c[:3].tolist() == [0, 1, 2] and c[-8:].tolist() == list(range(before[r] - 8, before[r]))
+            w = plain.w[r][h].clone()
+            w[:3] = w[-8:] = math.inf
+            out_of = torch.ones(before[r], dtype=torch.bool, device="cuda")
+            out_of[c] = False
+            # (weights carry errors of a few 1e-3 through 16-bit rows: the split may differ between near ties)
+            assert w[out_of].max() <= w[c].min() * 1.05
+    plain.take(kept)
+    cached = new
+    for _ in range(3):
+        step([1, 3, 2])
+    # into other pages
+    dst = torch.full((n, 3), -1, dtype=torch.int32, device="cuda")
+    used = set(table[:, :3].flatten().tolist())
+    free = [b for b in perm.tolist() if b not in used]
+    for r in range(n):
+        dst[r] = torch.tensor(free[3 * r:3 * r + 3], dtype=torch.int32)
+    new, kept = layer.evict(table, cached, dst_table=dst)
+    plain.take(kept)
+    table = torch.cat([dst, torch.tensor(free[9:9 + n], dtype=torch.int32, device="cuda")[:, None]], 1)
+    cached = new
+    step([4, 1, 1])
+    assert kernels.device_error(dev) == 0
+
+
+def test_draft_layer_refusals():
+    from oscar_b200.draft import DraftLayer
+
+    need_gpu()
+    pool = torch.zeros(2, 4, PAGE, HK, D, dtype=torch.bfloat16, device="cuda")
+    w, t = torch.zeros(D, device="cuda"), torch.zeros(8, ROT, device="cuda")
+    with pytest.raises(ValueError, match="multiple"):
+        DraftLayer(7, pool, w, w, t)
+    with pytest.raises(ValueError, match="sink and recent"):
+        DraftLayer(HQ, pool, w, w, t, keep=10, sink=8, recent=8)
+    with pytest.raises(ValueError, match="keeps no weights"):
+        DraftLayer(HQ, pool, w, w, t).evict(torch.zeros(1, 4, dtype=torch.int32, device="cuda"), [5])
