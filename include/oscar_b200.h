@@ -367,7 +367,7 @@ int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  * already holds their keys and values: query i of request r sees keys
  * [0, seqs[r] - q_len + i] (q_len = qsl[r + 1] - qsl[r]); a row that sees none
  * gets 0 and LSE -inf.  out [n, Hq, D] in the queries' type, lse [n, Hq] fp32
- * natural log.  qsl / seqs: HOST int32.  Slots past seqs[r] may hold anything.
+ * natural log.  At most 128 query heads per kv head.  qsl / seqs: HOST int32.  Slots past seqs[r] may hold anything.
  * A non-finite value row reaches every row of its request whose 64-key (or
  * 128-key) tile it shares, also the earlier ones of the same chunk.
  *

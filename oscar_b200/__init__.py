@@ -10,6 +10,7 @@ Package layout:
   config.py     OSCAR_ASCEND_* configuration
   rotation.py   per-layer rotation checkpoints
   mtp_shadow.py MTP draft-layer bf16 shadow pool
+  draft.py      attention step of a 16-bit paged (draft) layer
   synthetic.py  seeded synthetic workloads (tests, bench)
 """
 from . import config, format, rotation  # noqa: F401

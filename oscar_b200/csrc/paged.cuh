@@ -115,7 +115,9 @@ OSCAR_DEVINL bool pg_wait(int& abort, uint32_t bar, uint32_t parity) {
 // The keys' attention weights of requests with many query rows: scores are
 // recomputed.  CTA = (request, 64-key tile) x kv head, K tile in shared memory;
 // warp w takes the observed rows' 16-row blocks w, w + 8, ... that see the tile
-// and sums p = exp2(s - m) / l over its rows in registers.
+// and sums p = exp2(s - m) / l over its rows in registers.  Bound by the latency
+// of the query loads, so they are 16 bytes wide (384 rows on 11304 keys, 4 heads,
+// D 256: about 50 us; 4-byte loads of the fragments in their own order 85 us).
 template <int D, typename T>
 __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __grid_constant__ PagedArgs a,
                                                                         const __grid_constant__ KeyPlan p,
@@ -131,15 +133,22 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
   const int q_len = p.q_len[r], seq = p.seq[r];
   const int32_t* row = a.table + (int64_t)p.req_id[r] * a.table_stride;
   pdl_wait();
-  for (int i = tid; i < kPgKeys * (D / 8); i += 32 * kPgWarps) {
-    const int key = i / (D / 8), c = i % (D / 8);
-    uint4 v = make_uint4(0, 0, 0, 0);
+  constexpr int kLoads = kPgKeys * (D / 8) / (32 * kPgWarps);
+  uint4 kv[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int key = (i * 32 * kPgWarps + tid) / (D / 8), c = tid % (D / 8);
+    kv[i] = make_uint4(0, 0, 0, 0);
     if (key0 + key < seq) {
       const int64_t blk = row[a.page.div(key0 + key)];
       if (blk >= 0 && blk < a.num_blocks)
-        v = *reinterpret_cast<const uint4*>(k_cache + blk * kcb + (int64_t)a.page.mod(key0 + key) * kct + h * kch + 8 * c);
+        kv[i] = *reinterpret_cast<const uint4*>(k_cache + blk * kcb + (int64_t)a.page.mod(key0 + key) * kct + h * kch + 8 * c);
     }
-    *reinterpret_cast<uint4*>(pg_raw + (c / 8) * (kPgKeys * 128) + pg_swz(key, c % 8)) = v;
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int key = (i * 32 * kPgWarps + tid) / (D / 8), c = tid % (D / 8);
+    *reinterpret_cast<uint4*>(pg_raw + key * (2 * D) + ((c ^ (key & 1) << 2) << 4)) = kv[i];
   }
   __syncthreads();
   const int qr = lane >> 2, qc = lane & 3;
@@ -149,7 +158,6 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
   float sum[kPgKeys / 8][2];
 #pragma unroll
   for (int n = 0; n < kPgKeys / 8; ++n) sum[n][0] = sum[n][1] = 0.0f;
-  const uint32_t kb = smem_u32(pg_raw);
 #pragma unroll 1
   for (int rb = row_first + 16 * warp; rb < row_end; rb += 16 * kPgWarps) {
     float s[kPgKeys / 8][4];
@@ -170,18 +178,18 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
       st[hf] = a.stats[t * a.hq + head];
       lim[hf] = live ? seq - q_len + tok + 1 : 0;
     }
+    // A product's k order is free as long as both operands share it: lane qc holds dims 8 qc .. 8 qc + 7 of
+    // each 32, one 16-byte load per row, as k 2 qc, 2 qc + 1, 2 qc + 8, 2 qc + 9 of two steps.
 #pragma unroll 4
-    for (int d0 = 0; d0 < D; d0 += 16) {
-      uint32_t qa[4];
+    for (int d0 = 0; d0 < D; d0 += 32) {
+      const uint4 q0 = *reinterpret_cast<const uint4*>(src[0] + d0 + 8 * qc);
+      const uint4 q1 = *reinterpret_cast<const uint4*>(src[1] + d0 + 8 * qc);
+      const uint32_t qa[4] = {q0.x, q1.x, q0.y, q1.y}, qb[4] = {q0.z, q1.z, q0.w, q1.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qa[i] = *reinterpret_cast<const uint32_t*>(src[i & 1] + d0 + 8 * (i >> 1) + 2 * qc);
-#pragma unroll
-      for (int n = 0; n < kPgKeys / 8; n += 2) {
-        uint32_t b0, b1, b2, b3;
-        ldmatrix_x4(kb + (d0 / 64) * (kPgKeys * 128) + pg_swz(8 * n + (lane & 7) + 8 * (lane >> 4), (d0 % 64) / 8 + ((lane >> 3) & 1)),
-                    b0, b1, b2, b3);
-        Mma<T>::run(s[n], qa, b0, b1);
-        Mma<T>::run(s[n + 1], qa, b2, b3);
+      for (int n = 0; n < kPgKeys / 8; ++n) {
+        const uint4 k = *reinterpret_cast<const uint4*>(pg_raw + (8 * n + qr) * (2 * D) + (((d0 / 8 + qc) ^ (qr & 1) << 2) << 4));
+        Mma<T>::run(s[n], qa, k.x, k.y);
+        Mma<T>::run(s[n], qb, k.z, k.w);
       }
     }
 #pragma unroll
@@ -219,7 +227,8 @@ __global__ void __launch_bounds__(32 * kPgWarps) paged_mass_rows_kernel(const __
 // The keys' attention weights from stored scores (few query rows): a thread per
 // (key, kv head) sums exp2(s - m) / l over the observed rows.  A key of the
 // chunk itself starts from zero, an older one adds to what it has.  Bound by
-// reading the scores, 8 rows in flight per thread.
+// reading the scores, 8 rows in flight per thread (8 x 24580 keys, 24 rows, 4
+// heads: 76 MB in 19.5 us).
 // (tiles of request r: [head][key tile], numbered as the attention's)
 __global__ void __launch_bounds__(kPgKeys) paged_mass_kernel(const __grid_constant__ PagedArgs a,
                                                              const __grid_constant__ KeyPlan p) {

@@ -16,6 +16,10 @@
 // at most 46 (measured on resident data); it also leaves room for 2.5 tiles of K
 // and V instead of 1.25 beside the queries.
 //
+// Measured (Hq 24 / Hk 4 / D 256, bf16): kFew, 8 x 4 tokens on 24580: 131 us, 6.1
+// TB/s (0.94 of the measured copy); 8192 tokens on 17448: 1.97-2.03 ms, 1330-1370
+// TFLOP/s (0.98-1.0 of the sustained library rate, at the power cap's clock).
+//
 // Bounds.  kFew: HBM; the keys stream through shared memory once, 64-key tiles,
 // and the products of 128 padded rows take half of the time their bytes do
 // (mma.sync on the live rows took more: its operand reads alone filled the
@@ -35,8 +39,10 @@
 //   O += P V  : A = P in tensor memory, B = V, MN-major, 128-byte swizzle.
 // The running maximum moves only when a score exceeds it by kPgHeadroom (log2
 // units); then the thread rescales its row of O in tensor memory.  P is rounded to
-// the values' type (the product takes one type): 2^-9 (bf16) or 2^-12 of each
-// probability, below the rounding of the result.
+// the values' type (the product takes one type), at most 2^-8 (bf16) or 2^-11 of
+// each probability and averaged by the sum over keys: the result's error against
+// 64 bits is 0.0023 relative (bf16), 0.0017 being its own rounding.  The row sums
+// take P as it was before.
 //
 // Warps: 4 softmax per row tile, one MMA issuer, two TMA producers (K and Q; V)
 // that fill one ring of slots in the order the MMAs use them, in boxes of 64
