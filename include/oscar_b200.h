@@ -71,6 +71,12 @@ int oscar_set_attention_path(int path);
  * the switch keeps both parity-tested.  Other values: status 1. */
 int oscar_set_rotation_path(int path);
 
+/* Limit of one bounded wait of the oscar_paged_attention kernels, in tries of up to
+ * a millisecond: -1 = the default (4096).  A wait that runs out latches device
+ * error 16 and ends the launch early with whatever it has written; the switch keeps
+ * that end tested.  Values below -1: status 1. */
+int oscar_set_wait_limit(int tries);
+
 /* Synchronises `stream`, returns and clears the device-side bounds flag of the
  * current device: 0 = clean, otherwise a bitmask (1 = slot out of range,
  * 2 = block-table entry out of range, 8 = merge target row out of range,

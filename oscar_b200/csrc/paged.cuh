@@ -58,6 +58,7 @@ struct PagedArgs {
   float* scores;          // [tile][kPgFewRows][64] scaled scores in log2 units, or null
   float* weights;         // [num_blocks, hk, bs], or null
   int observe;            // the last `observe` tokens of a request weigh the keys
+  uint32_t tries;         // of a bounded wait
 };
 
 OSCAR_DEVINL int pg_find(const int* begin, int n, int x) {
@@ -88,9 +89,8 @@ OSCAR_DEVINL uint32_t pg_swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (
 
 // Bounded wait of a CTA whose roles never leave early: the first time-out sets
 // the CTA's abort flag, after which every wait returns soon and the warps run
-// to the end through their (always complete) barriers.  A waiting warp suspends
-// for up to a millisecond a try: polls take shared-memory cycles from the
-// tensor cores' operands (2570 against 2430 us on the longest chunk).
+// to the end through their (always complete) barriers.  A waiting warp suspends for up to a millisecond a try: polls take shared-memory
+// cycles from the tensor cores' operands (2570 against 2430 us on the longest chunk).
 constexpr uint32_t kPgTries = 4096;
 OSCAR_DEVINL bool pg_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
@@ -101,13 +101,23 @@ OSCAR_DEVINL bool pg_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-OSCAR_DEVINL bool pg_wait(int& abort, uint32_t bar, uint32_t parity) {
+OSCAR_DEVINL bool pg_wait(int& abort, uint32_t bar, uint32_t parity, uint32_t tries) {
   if (tc::mbar_test(bar, parity)) return true;
-  for (uint32_t i = 0; i < kPgTries; ++i) {
+  for (uint32_t i = 0; i < tries; ++i) {
     if (pg_try(bar, parity)) return true;
     if (*reinterpret_cast<volatile int*>(&abort) != 0) return false;
   }
   *reinterpret_cast<volatile int*>(&abort) = 1;
+  flag_error(16u);
+  return false;
+}
+
+// For what is in flight already and needs no warp to complete (copies, products), whether or not
+// the CTA has been aborted: at most a quarter of a second.
+constexpr uint32_t kPgDrainTries = 256;
+OSCAR_DEVINL bool pg_drain(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kPgDrainTries; ++i)
+    if (pg_try(bar, parity)) return true;
   flag_error(16u);
   return false;
 }

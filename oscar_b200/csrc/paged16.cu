@@ -2,6 +2,7 @@
 // include/oscar_b200.h): head norm + rotation + cache write, attention over
 // the paged cache with the keys' accumulated weights, eviction by weight.
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 
@@ -32,6 +33,8 @@ using oscar_host::encode_tiled;
 using oscar_host::fail;
 using oscar_host::launch_pdl;
 using oscar_host::launch_pdl_cluster;
+
+std::atomic<uint32_t> g_wait_tries{oscar::kPgTries};
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -434,6 +437,12 @@ int launch_paged_d(int d, const PagedCall& c, const PagedBatch& b) {
 
 extern "C" {
 
+int oscar_set_wait_limit(int tries) {
+  if (tries < -1) return fail(OSCAR_ERR_INVALID, "the wait limit must be -1 (default) or a number of tries");
+  g_wait_tries.store(tries < 0 ? oscar::kPgTries : (uint32_t)tries);
+  return OSCAR_OK;
+}
+
 int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs, int32_t num_requests,
                                         int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                                         int32_t weighted) {
@@ -502,6 +511,7 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.scale_log2 = scale * 1.4426950408889634f;
   a.weights = weights;
   a.observe = weights != nullptr ? observe : 0;
+  a.tries = g_wait_tries.load(std::memory_order_relaxed);
   c.k_cache = k_cache, c.kcb = k_stride_block, c.kct = k_stride_token, c.kch = k_stride_head;
   c.n = n_tokens;
   c.stream = reinterpret_cast<cudaStream_t>(stream);

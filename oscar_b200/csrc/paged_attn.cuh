@@ -104,6 +104,9 @@ struct PcSmem {
   // full, q_full, p_full: of a pair, the first CTA's are used by both
   unsigned long long full[S::kSlots], empty[S::kSlots];
   unsigned long long q_full, q_empty, s_full[2], p_full[2], o_done[2], tail, end;
+  // what this CTA has announced on the barriers above: the latest ring position of each slot (-1: none)
+  // and the number of units whose queries it has
+  int at[S::kSlots], units;
   uint32_t tmem;
   int abort;
 };
@@ -230,6 +233,38 @@ OSCAR_DEVINL void pc_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y,
   }
 }
 
+// Sets the abort flag of the pair's other CTA, whose waits then return soon too
+OSCAR_DEVINL void pc_abort(uint32_t cluster_addr) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(cluster_addr), "r"(1) : "memory");
+}
+OSCAR_DEVINL int pc_peek(uint32_t cluster_addr) {
+  int v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];\n" : "=r"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// After an abort, by a warp of the CTA that owns `full` and `q_full`, once every producer has stopped:
+// waits for the copies that still write shared memory.  A slot is announced again only after its last
+// phase was consumed, so at most the phase of the latest position is open; where only one CTA of a pair
+// has announced it, the other one's arrival is made up for, so that the phase ends with the bytes.
+// (V tiles that are completed by hand count on `tail`, which their producer has drained.)
+template <bool kPair, int kSlots, typename Smem>
+OSCAR_DEVINL void pc_drain_loads(Smem& sm, int lane) {
+  if (lane > kSlots) return;
+  const bool is_q = lane == kSlots;
+  int* const mine = is_q ? &sm.units : &sm.at[lane];
+  const uint32_t bar = is_q ? smem_u32(&sm.q_full) : smem_u32(&sm.full[lane]);
+  int n = *reinterpret_cast<volatile int*>(mine);
+  if constexpr (kPair) {
+    const int theirs = pc_peek(pc_map(smem_u32(mine), 1));
+    if (theirs != n) {
+      tc::mbar_arrive(bar);
+      n = max(n, theirs);
+    }
+  }
+  if (is_q ? n > 0 : n >= 0) pg_drain(bar, (is_q ? n - 1 : n / kSlots) & 1);
+}
+
 // The pieces of units of one worker, walked alike by every role.
 template <typename Shape>
 struct PcWalk {
@@ -334,6 +369,8 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       tc::mbar_init(smem_u32(&sm.q_empty), 1);
       tc::mbar_init(smem_u32(&sm.tail), 1);
       tc::mbar_init(smem_u32(&sm.end), 1);
+      for (int i = 0; i < kSlots; ++i) sm.at[i] = -1;
+      sm.units = 0;
       sm.abort = 0;
       tc::mbar_fence_init();
     }
@@ -358,7 +395,9 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
   tc::tc_fence_after();
   const uint32_t tmem = sm.tmem;
   auto wait = [&](uint32_t bar, uint32_t parity) -> bool {  // warp-uniform
-    return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
+    const bool ok = pg_wait(sm.abort, bar, parity, a.tries);
+    if (kPair && !ok) pc_abort(pc_map(smem_u32(&sm.abort), rank ^ 1));  // (it cannot end before this warp does)
+    return __all_sync(0xffffffffu, ok);
   };
   PcWalk<Shape> w(p, worker);  // (the plan is an argument)
   const int n_tiles = w.left, tile0 = p.first[worker];
@@ -555,9 +594,6 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
     // needs beside P is waited for before P where its slot was released by earlier steps, so that
     // both products go out back to back; a new unit's queries come only once the S before it is
     // complete and are waited for after the PV
-    auto wait_all = [&](uint32_t bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, pg_wait(sm.abort, bar, parity));
-    };
     // S runs two jobs ahead of O and may belong to the next unit
     PcWalk<Shape> ws = w;                               // unit of the next S
     int unit = 0;                                // its number
@@ -570,13 +606,13 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       const int o_mt = kM == 2 ? jo & 1 : 0, s_mt = kM == 2 ? js & 1 : 0;
       const int v_at = pc_v_at<kM>(kM == 2 ? jo >> 1 : jo, n_tiles), v_slot = v_at % kSlots;
       const int k_at = pc_k_at<kM>(kM == 2 ? js >> 1 : js), k_slot = k_at % kSlots;
-      if (jo >= 0 && o_mt == 0 && !wait_all(full(v_slot), (v_at / kSlots) & 1)) break;
+      if (jo >= 0 && o_mt == 0 && !wait(full(v_slot), (v_at / kSlots) & 1)) break;
       if (js < jobs && s_open && s_mt == 0) {
-        if (!wait_all(full(k_slot), (k_at / kSlots) & 1)) break;
+        if (!wait(full(k_slot), (k_at / kSlots) & 1)) break;
         tc::tc_fence_after();
       }
       if (jo >= 0) {
-        if (!wait_all(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
+        if (!wait(smem_u32(&sm.p_full[jo & 1]), (jo >> 1) & 1)) break;
         tc::tc_fence_after();
         if (tc::elect_one()) {
           const uint64_t vd = dv + (uint64_t)v_slot * kSlotStep;
@@ -597,7 +633,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       }
       if (js < jobs) {
         if (!s_open) {
-          if (!wait_all(smem_u32(&sm.q_full), unit & 1) || !wait_all(full(k_slot), (k_at / kSlots) & 1)) break;
+          if (!wait(smem_u32(&sm.q_full), unit & 1) || !wait(full(k_slot), (k_at / kSlots) & 1)) break;
           tc::tc_fence_after();
           s_open = true;
         }
@@ -628,7 +664,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
     // CTA has come before that CTA ends)
     if (rank == 0 && tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
     __syncwarp();
-    wait_all(smem_u32(&sm.end), 0);
+    wait(smem_u32(&sm.end), 0);
   } else {
     // ================= producers: one warp fetches K (and Q), one V, each in the order of use.
     // Lane i holds the pages of boxes i, i + 32, .. of the next tile, looked up while the tile
@@ -665,6 +701,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
           if (unit > 0 && !wait(smem_u32(&sm.q_empty), (unit - 1) & 1)) break;
           if (tc::elect_one()) {
             const uint32_t bar = lead(smem_u32(&sm.q_full));
+            sm.units = unit + 1;
             const uint32_t bytes = (uint32_t)(kM * kPanels * p.box_tokens * a.group * 128);
             if constexpr (kPair) pc_expect(bar, bytes);
             else tc::mbar_expect_tx(bar, bytes);
@@ -703,6 +740,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       const uint32_t bar = tail ? smem_u32(&sm.tail) : lead(full(slot));
       const uint32_t bytes = (uint32_t)(live * pans) * box_bytes;
       if (tc::elect_one()) {
+        if (!tail) sm.at[slot] = at;
         if (kPair && !tail) pc_expect(bar, bytes);
         else tc::mbar_expect_tx(bar, bytes);
       }
@@ -728,7 +766,10 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       }
       __syncwarp();
       if (tail) {
-        if (!wait(bar, tails & 1)) break;
+        if (!wait(bar, tails & 1)) {
+          pg_drain(bar, tails & 1);
+          break;
+        }
         ++tails;
         const int clear = max(have, 0);
         for (int i = lane; i < (kTile - clear) * 8 * pans; i += 32) {
@@ -738,6 +779,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
         tc::fence_async_smem();
         __syncwarp();
         if (lane == 0) {
+          sm.at[slot] = at;
           if constexpr (kPair) pc_arrive<true>(lead(full(slot)));
           else tc::mbar_arrive(full(slot));
         }
@@ -751,18 +793,24 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
       }
       if (is_k && unit > 0) wait(smem_u32(&sm.q_empty), (unit - 1) & 1);
     }
-    // no copy may still be writing shared memory when the CTA ends.  The MMA warp has waited for
-    // all of them unless a wait timed out
-    if (*reinterpret_cast<volatile int*>(&sm.abort) != 0) {
-      for (int n = max(0, last_at - kSlots + 1); n <= last_at; ++n) tc::mbar_wait(full(n % kSlots), (n / kSlots) & 1);
-      if (is_k && unit > 0) tc::mbar_wait(smem_u32(&sm.q_full), (unit - 1) & 1);
-    }
   }
 
   __syncwarp();
   tc::tc_fence_before();
-  if constexpr (kPair) pc_cluster_sync();  // neither CTA's barriers, tensor or shared memory are used from here on
+  // every role has issued what it will.  Without an abort all copies and products have been waited
+  // for, and neither CTA's barriers, tensor or shared memory are used from here on
+  if constexpr (kPair) pc_cluster_sync();
   else __syncthreads();
+  if (*reinterpret_cast<volatile int*>(&sm.abort) != 0) {  // (the same for both CTAs of a pair)
+    if (warp == kMma) {
+      pg_drain(smem_u32(&sm.end), 0);
+      __syncwarp();
+      if (rank == 0) pc_drain_loads<kPair, kSlots>(sm, lane);
+      else __nanosleep(100000);  // the other releases of the products that `end` followed are on their way
+    }
+    __syncwarp();
+    if constexpr (kPair) pc_cluster_sync();  // the first CTA counts the second one's copies
+  }
   if (warp == kMma) {
     tc::tc_fence_after();
     if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;\n" ::"r"(tmem) : "memory");

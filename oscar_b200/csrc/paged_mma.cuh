@@ -62,8 +62,8 @@ OSCAR_DEVINL void ps_produce(Smem& sm, const PagedArgs& a, const PcPlan& p, cons
       const uint32_t bytes = (uint32_t)live * box_bytes * kPanels;
       const uint32_t fk = smem_u32(&sm.full_k[st]), fv = smem_u32(&sm.full_v[st]);
       if (it >= kSt) {
-        const bool k_free = pg_wait(sm.abort, smem_u32(&sm.empty_k[st]), phase ^ 1);
-        const bool v_free = pg_wait(sm.abort, smem_u32(&sm.empty_v[st]), phase ^ 1);
+        const bool k_free = pg_wait(sm.abort, smem_u32(&sm.empty_k[st]), phase ^ 1, a.tries);
+        const bool v_free = pg_wait(sm.abort, smem_u32(&sm.empty_v[st]), phase ^ 1, a.tries);
         if (!__all_sync(0xffffffffu, k_free && v_free)) {
           ok = false;  // gave up: issue nothing more
           break;
@@ -185,7 +185,7 @@ paged_attn_mma_kernel(const __grid_constant__ PagedArgs a, const __grid_constant
       const uint32_t phase = (it / Smem::kStages) & 1;
       const int key0 = t * kPgKeys;
       const int buf = it & 1;
-      pg_wait(sm.abort, smem_u32(&sm.full_k[st]), phase);
+      pg_wait(sm.abort, smem_u32(&sm.full_k[st]), phase, a.tries);
       // ---- S of this warp's rows and keys: two MMA chains (the dims' halves of each
       // 32 for 8 keys, or 2 x 8 keys)
       float s2[2][4];
@@ -285,7 +285,7 @@ paged_attn_mma_kernel(const __grid_constant__ PagedArgs a, const __grid_constant
       l[0] += pl[0];
       l[1] += pl[1];
       // ---- O += P V over this warp's dims
-      pg_wait(sm.abort, smem_u32(&sm.full_v[st]), phase);
+      pg_wait(sm.abort, smem_u32(&sm.full_v[st]), phase, a.tries);
       const int have = seq - key0;  // keys of the request in this tile
       if (have < kPgKeys) {
         // the rest of the last page (or what an earlier tile left) may hold anything: 0 * NaN

@@ -721,6 +721,13 @@ def set_rotation_path(path: str) -> None:
     check(_native.lib().oscar_set_rotation_path(_ROT_PATHS[path]))
 
 
+def set_wait_limit(tries: int = -1) -> None:
+    """Limit of one bounded wait of the paged_attention kernels in tries of up
+    to a millisecond (-1: the default).  A wait that runs out latches device
+    error 16 and ends the launch early (debug)."""
+    check(_native.lib().oscar_set_wait_limit(int(tries)))
+
+
 def device_error(device=None) -> int:
     """Synchronise and return/clear the kernels' bounds-violation flag (debug)."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)

@@ -267,6 +267,37 @@ def test_paged_attention_other_stream_and_preallocated_out():
     assert got.data_ptr() == out.data_ptr() and torch.equal(got, want)
 
 
+@pytest.mark.parametrize("lens,seqs,opts", [
+    ([300], [5000], dict()),                                     # pairs of CTAs
+    ([700, 90], [900, 4000], dict(hq=16, d=128)),                # two row tiles per CTA
+    ([300], [3000], dict(hq=16, d=64, dtype=torch.float16, page=16)),
+    ([20, 13], [3000, 21], dict()),                              # one row tile
+    ([4, 1], [41000, 5003], dict(hq=48, hk=8)),                  # few rows on the tensor-memory kernel
+    ([2, 1], [50000, 41], dict(hq=24, hk=8, d=128, page=48)),
+    ([4, 1], [3000, 70], dict()),                                # and on mma.sync
+])
+def test_paged_attention_ends_when_a_wait_runs_out(lens, seqs, opts):
+    """With no patience at all the first wait that is not over ends the launch: it flags that, leaves
+    nothing in flight, and the next launch is as ever."""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, opts)
+    want, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+    assert kernels.device_error(dev) == 0
+    for _ in range(3):
+        try:
+            kernels.set_wait_limit(0)
+            for _ in range(4):
+                kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+            assert kernels.device_error(dev) == 16
+        finally:
+            kernels.set_wait_limit()
+        got, lse2 = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+        assert torch.equal(got, want) and torch.equal(lse, lse2)
+        assert kernels.device_error(dev) == 0
+
+
 WEIGHT_CASES = [
     ([1], [1000], None, dict()),
     ([4, 1, 0, 2], [2000, 65, 70, 1], None, dict()),

@@ -85,6 +85,12 @@ def test_paged_attention_refusals(lib, kw, status, text):
     assert text in lib.oscar_last_error()
 
 
+def test_wait_limit(lib):
+    assert lib.oscar_set_wait_limit(-2) == 1
+    assert b"wait limit" in lib.oscar_last_error()
+    assert lib.oscar_set_wait_limit(5) == 0 and lib.oscar_set_wait_limit(-1) == 0
+
+
 def test_workspace_of_invalid_lists(lib):
     assert lib.oscar_paged_attention_workspace(ints(0, 4, 3), ints(1, 1), 2, 24, 4, 256, 0) < 0
     assert lib.oscar_paged_attention_workspace(ints(0, 4), ints(9), 1, 24, 5, 256, 0) < 0
