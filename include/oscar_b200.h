@@ -73,8 +73,9 @@ int oscar_set_rotation_path(int path);
 
 /* Limit of one bounded wait of the oscar_paged_attention kernels, in tries of up to
  * a millisecond: -1 = the default (4096).  A wait that runs out latches device
- * error 16 and ends the launch early with whatever it has written; the switch keeps
- * that end tested.  Values below -1: status 1. */
+ * error 16 and ends the launch early with whatever it has written.  It is the limit of
+ * one step of a pipeline, not of a launch, which may take any time; the switch
+ * keeps both tested.  Values below -1: status 1. */
 int oscar_set_wait_limit(int tries);
 
 /* Synchronises `stream`, returns and clears the device-side bounds flag of the

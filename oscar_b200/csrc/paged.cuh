@@ -89,8 +89,11 @@ OSCAR_DEVINL uint32_t pg_swz(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (
 
 // Bounded wait of a CTA whose roles never leave early: the first time-out sets
 // the CTA's abort flag, after which every wait returns soon and the warps run
-// to the end through their (always complete) barriers.  A waiting warp suspends for up to a millisecond a try: polls take shared-memory
-// cycles from the tensor cores' operands (2570 against 2430 us on the longest chunk).
+// to the end through their (always complete) barriers.  The limit is for one
+// step of a pipeline (microseconds): no wait of this kind may span a launch,
+// which may take any time.  A waiting warp suspends for up to a millisecond a
+// try: polls take shared-memory cycles from the tensor cores' operands (2570
+// against 2430 us on the longest chunk).
 constexpr uint32_t kPgTries = 4096;
 OSCAR_DEVINL bool pg_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;

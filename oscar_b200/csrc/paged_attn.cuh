@@ -660,11 +660,12 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
         }
       }
     }
-    // no MMA may be in flight when the tensor memory is freed (of a pair, the arrival at the second
-    // CTA has come before that CTA ends)
-    if (rank == 0 && tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
-    __syncwarp();
-    wait(smem_u32(&sm.end), 0);
+    // no MMA may be in flight when the tensor memory is freed
+    if (rank == 0) {
+      if (tc::elect_one()) pc_commit<kPair>(smem_u32(&sm.end));
+      __syncwarp();
+      wait(smem_u32(&sm.end), 0);
+    }
   } else {
     // ================= producers: one warp fetches K (and Q), one V, each in the order of use.
     // Lane i holds the pages of boxes i, i + 32, .. of the next tile, looked up while the tile
@@ -801,6 +802,10 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
   // for, and neither CTA's barriers, tensor or shared memory are used from here on
   if constexpr (kPair) pc_cluster_sync();
   else __syncthreads();
+  // (the second CTA's `end` comes here: its MMA warp issues nothing, and from the kernel's start it
+  // would wait for the whole stream, which no limit of a wait suits)
+  if (kPair && rank == 1 && warp == kMma) pg_drain(smem_u32(&sm.end), 0);
+  __syncwarp();
   if (*reinterpret_cast<volatile int*>(&sm.abort) != 0) {  // (the same for both CTAs of a pair)
     if (warp == kMma) {
       pg_drain(smem_u32(&sm.end), 0);

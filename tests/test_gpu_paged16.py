@@ -298,6 +298,32 @@ def test_paged_attention_ends_when_a_wait_runs_out(lens, seqs, opts):
         assert kernels.device_error(dev) == 0
 
 
+def test_paged_attention_longer_than_a_wait():
+    """Waits are limited per step of a pipeline, not per launch: a launch that takes several
+    times the limit ends as usual.  (The limit is 8 tries of at most a millisecond; 5e13
+    operations take over 30 ms.)"""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    m, seq = 32768, 81920
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    kc, vc, table = make_pool(gen, [seq], 128, 4, 256, torch.bfloat16)
+    q = randn(gen, m, 24, 256, dtype=torch.bfloat16)
+    want, lse = kernels.paged_attention(q, kc, vc, table, [0, m], [seq], 1 / 16)
+    try:
+        kernels.set_wait_limit(8)
+        got, lse2 = kernels.paged_attention(q, kc, vc, table, [0, m], [seq], 1 / 16)
+        assert kernels.device_error(dev) == 0
+    finally:
+        kernels.set_wait_limit()
+    assert torch.equal(got, want) and torch.equal(lse, lse2)
+    # the first and last tokens against 64 bits
+    for t0 in (0, m - 4):
+        n = seq - m + t0 + 4
+        rows = attention64(q[t0:t0 + 4], kc, vc, table, [4], [n], 1 / 16)
+        check_attention(q, want[t0:t0 + 4], lse[t0:t0 + 4], rows, [n])
+
+
 WEIGHT_CASES = [
     ([1], [1000], None, dict()),
     ([4, 1, 0, 2], [2000, 65, 70, 1], None, dict()),
