@@ -423,6 +423,10 @@ def _cuda_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
     return index
 
 
+# the library launches on the current device, which therefore has to be the tensors'
+_current_device = torch.cuda.current_device
+
+
 def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
     """[n, heads, D] with contiguous, 16-byte aligned head vectors (a copy of t where its layout has none)."""
     if stride[2] != 1 or (stride[0] | stride[1]) % 8 or t.data_ptr() % 16:
@@ -488,6 +492,11 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
     if write != (v_cache is not None) or write != (slot_mapping is not None) or (write and v is None):
         raise ValueError("qk_norm_rope: v, caches and slot_mapping come together")
     index = _cuda_index(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, slot_mapping, out_q, out_k)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, weight_offset=weight_offset,
+                                interleaved=interleaved, k_cache=k_cache, v_cache=v_cache, slot_mapping=slot_mapping,
+                                out_q=out_q, out_k=out_k)
     w_dtype, cs_dtype, cs_shape = q_weight.dtype, cos_sin.dtype, cos_sin.shape
     if q_weight.shape != (d,) or k_weight.shape != (d,) or w_dtype != k_weight.dtype:
         raise ValueError(f"qk_norm_rope: the weights must be two [{d}] tensors of one type")
@@ -560,6 +569,9 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
     n, hq, d = q_shape
     nb, bs, hk = c_shape[:3]
     index = _cuda_index(q, k_cache, v_cache, table, weights, out)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, weights=weights, observe=observe, out=out)
     ks, vs = _cache16("paged_attention", k_cache, v_cache, dtype, hk, d)
     qsl_a, seqs_a = _host_ints(qsl), _host_ints(seqs)
     if qsl_a.ndim != 1 or seqs_a.ndim != 1 or qsl_a.size != seqs_a.size + 1 or qsl_a[0] != 0 or qsl_a[-1] != n:
@@ -607,6 +619,9 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     if dtype not in _HALF:
         raise ValueError(f"evict_cache: unsupported cache type {dtype}")
     index = _cuda_index(k_cache, v_cache, weights, table, dst_table)
+    if index != _current_device():
+        with torch.cuda.device(index):
+            return evict_cache(k_cache, v_cache, weights, table, seqs, keep, sink=sink, recent=recent, dst_table=dst_table)
     ks, vs = _cache16("evict_cache", k_cache, v_cache, dtype, hk, d)
     if weights.shape != (nb, hk, bs) or weights.dtype != torch.float32 or not weights.is_contiguous():
         raise ValueError(f"evict_cache: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")

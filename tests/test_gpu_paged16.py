@@ -324,6 +324,43 @@ def test_paged_attention_longer_than_a_wait():
         check_attention(q, want[t0:t0 + 4], lse[t0:t0 + 4], rows, [n])
 
 
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
+    """With another device current, every call makes the tensors' device current around its work.  (The
+    other device is pretended: one is enough, and nothing is ever launched on a wrong one.)"""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    current, entered = [1], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    q, kc, vc, table, qsl, scale = make_call([2], [300], dict())
+    w = torch.zeros(kc.shape[0], 4, 128, device="cuda")
+    rope = make_rope(2, dict())
+    calls = [lambda: kernels.paged_attention(q, kc, vc, table, qsl, [300], scale)[0],
+             lambda: kernels.qk_norm_rope(*rope[:2], None, *rope[3:5], 1e-6, *rope[5:7])[0],
+             lambda: kernels.evict_cache(kc, vc, w, table, [300], 300)]
+    want = [call() for call in calls]
+    monkeypatch.setattr(kernels, "_current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for call, x in zip(calls, want):
+        entered.clear()
+        assert torch.equal(call(), x)
+        assert entered == [0] and current == [1]
+        current[0] = 0
+        assert torch.equal(call(), x) and entered == [0]
+        current[0] = 1
+
+
 WEIGHT_CASES = [
     ([1], [1000], None, dict()),
     ([4, 1, 0, 2], [2000, 65, 70, 1], None, dict()),
