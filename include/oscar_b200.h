@@ -413,6 +413,7 @@ int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs,
  * [num_requests, num_kv_heads, kept_cols] int32: the kept positions, -1 past
  * a request's list.  Pages written here must belong to one request of the call
  * only, and dst pages must not be source pages (unless dst_table is NULL).
+ * Weights that another stream writes meanwhile leave the choice undefined.
  * The pages' keys carry their position rotation with them. */
 int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t num_blocks, int32_t block_size,
                       int32_t num_kv_heads, int64_t k_stride_block, int64_t k_stride_token, int64_t k_stride_head,

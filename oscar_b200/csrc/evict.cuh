@@ -163,11 +163,15 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     pc_cluster_sync();
     const uint2 theirs = ev_remote2(smem_u32(range), lane % kEvCluster);
     uint32_t lo = __reduce_min_sync(0xffffffffu, theirs.x), hi = __reduce_max_sync(0xffffffffu, theirs.y);
+    // Every round leaves one bin of at most 1 / 128 of the range, so there are four at most, and all
+    // CTAs take the same bin, since they add up the same counts.  (Keys read again from memory that
+    // somebody is writing may have too few for `need`: then the lowest bin is as good as any)
 #pragma unroll 1
     while (lo < hi) {
       // bins of 2^shift keys, at most 256 of them
       const int shift = max(0, 32 - __clz(hi - lo) - 8);
       for (int i = tid; i < kEvBins; i += kEvThreads) bins[i] = 0;
+      if (tid == 0) pick[0] = 0, pick[1] = need;
       __syncthreads();
       each([&](uint32_t key) {
         if (key >= lo && key <= hi) atomicAdd(&bins[(key - lo) >> shift], 1u);
@@ -274,6 +278,8 @@ __global__ void __launch_bounds__(kEvThreads) evict_select_kernel(const __grid_c
     equal += e_piece;
     pc_cluster_sync();  // the counts have been read; no CTA ends while another reads its shared memory
   }
+  // (as above: places that keys read again have left empty)
+  for (int j = (int)out + rank * kEvThreads + tid; j < n; j += kEvCluster * kEvThreads) kept[j] = -1;
   if (bad) flag_error(2u);
 }
 
@@ -303,6 +309,7 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_copy_kernel(const __grid
       m[i].sb = -1;
       if (j >= n) continue;
       const int s = kept[j], sp = (int)a.page.div(s), dp = (int)a.page.div(j);
+      if (s < 0) continue;
       const int sb = src_row[sp], db = dst_row[dp];
       if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;  // flagged by the selection
       m[i] = Move{sb, s - sp * a.bs, db, j - dp * a.bs};
@@ -362,7 +369,7 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const __grid
       const int j = j0 + i * kRows + threadIdx.x / 8;
       if (j >= n) continue;
       const int s = kept[j];
-      const uint8_t* from = s == j ? nullptr : slot(s);
+      const uint8_t* from = s == j || s < 0 ? nullptr : slot(s);
       if (from != nullptr) y[i] = *reinterpret_cast<const uint4*>(from);
     }
   };
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_move_kernel(const __grid
       const int j = j0 + i * kRows + threadIdx.x / 8;
       if (j >= n) continue;
       const int s = kept[j];
-      if (s == j || slot(s) == nullptr) continue;
+      if (s == j || s < 0 || slot(s) == nullptr) continue;
       uint8_t* to = slot(j);
       if (to != nullptr) *reinterpret_cast<uint4*>(to) = y[i];
     }

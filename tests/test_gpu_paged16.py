@@ -636,6 +636,44 @@ def test_evict_equal_weights_in_many_requests():
     assert kernels.device_error(dev) == 0
 
 
+@pytest.mark.parametrize("in_place", [True, False])
+def test_evict_ends_while_another_stream_writes_the_weights(in_place):
+    """A caller's mistake: more keys than shared memory holds are read again in each round, here from
+    weights that change meanwhile.  What stays is then undefined, but the call ends, lists positions
+    of the request in order and moves nothing else."""
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    seq, keep, page = 300000, 120000, 64
+    fresh = -(-keep // page)
+    kc, vc, table = make_pool(gen, [seq], page, 1, 64, torch.bfloat16, spare=fresh, poison=False)
+    nb = kc.shape[0]
+    used = torch.zeros(nb, dtype=torch.bool, device="cuda")
+    used[table[0, :-(-seq // page)].long()] = True
+    dst = None if in_place else (~used).nonzero().flatten().to(torch.int32)[None, :fresh].contiguous()
+    w = torch.rand(nb, 1, page, generator=gen, device="cuda")
+    spare_k = kc[~used].clone()
+    side = torch.cuda.Stream()
+    lists = []
+    torch.cuda.synchronize()
+    for scale in (1.0, 1e6, 1e-6, 1.0, 1e3, 1e-3):
+        with torch.cuda.stream(side):
+            for _ in range(20):
+                w.uniform_().mul_(scale)
+                w.neg_()
+        for _ in range(4):
+            lists.append(kernels.evict_cache(kc, vc, w, table, [seq], keep, sink=5, recent=9, dst_table=dst))
+        torch.cuda.synchronize()
+    for kept in lists:
+        kept = kept.flatten()
+        there = kept[kept >= 0]
+        assert (there[1:] > there[:-1]).all() and there[-1] < seq and (kept[there.numel():] == -1).all()
+    if in_place:
+        assert torch.equal(kc[~used], spare_k)
+    assert kernels.device_error(dev) == 0
+
+
 def test_evict_strided_caches():
     from oscar_b200 import kernels
 
