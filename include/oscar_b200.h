@@ -344,7 +344,8 @@ int64_t oscar_decode_layer_step_scratch(int64_t n_tokens, int32_t num_q_heads, i
  * Caches are [num_blocks, block_size, num_kv_heads, head_dim] with strides in
  * ELEMENTS (rows of head_dim contiguous, 16-byte aligned; pages, tokens and
  * heads at any stride, e.g. the K half of a [blocks, 2, ...] pool), head_dim
- * 64, 128 or 256, any block size.  Slots and positions are int64.
+ * 64, 128 or 256, any block size, at most 2^30 cached tokens per request.
+ * Slots and positions are int64.
  *
  * oscar_qk_norm_rope: RMS norm of every query and key head, position rotation
  * and cache write in one pass.  Per head x:

@@ -34,6 +34,12 @@ using oscar_host::fail;
 using oscar_host::launch_pdl;
 using oscar_host::launch_pdl_cluster;
 
+// Positions and tiles are counted in 32 bits, with room for what is added to them: a request's
+// cached tokens, its 64-key tiles over all heads and those of a launch, and the tiles of a call's
+// query blocks (over 74 pairs of CTAs or more).
+constexpr int32_t kMaxLength = 1 << 30;
+constexpr int64_t kMaxKeyTiles = (int64_t)1 << 30, kMaxWork = (int64_t)1 << 38;
+
 std::atomic<uint32_t> g_wait_tries{oscar::kPgTries};
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -186,6 +192,10 @@ struct PagedBatch {
   oscar::PcSplits splits;  // its divided units
 };
 
+inline int64_t key_tiles(int32_t seq, int hk) {
+  return std::max<int64_t>(1, ((int64_t)seq + oscar::kPgKeys - 1) / oscar::kPgKeys) * hk;
+}
+
 // Divides the tiles of all units over the workers.  A unit costs its tiles and
 // kUnitCost more (queries, first products, epilogue: about 9000 cycles against
 // 4100 a tile at D 128 and 7000 against 2600 at D 256, from clock traces), so that
@@ -242,9 +252,12 @@ int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const
   b.cls = cls;
   p.num_req = 0;
   int r = r0;
+  int64_t tiles = 0;
   for (; r < num && p.num_req < oscar::kPgReqs; ++r) {
     const int len = qsl[r + 1] - qsl[r];
     if (len == 0 || paged_class(len, group) != cls) continue;
+    tiles += key_tiles(seqs[r], hk);
+    if (p.num_req > 0 && tiles > kMaxKeyTiles) break;
     const int i = p.num_req++;
     p.req_id[i] = r;
     p.q_start[i] = qsl[r];
@@ -278,9 +291,16 @@ int check_paged(const int32_t* qsl, const int32_t* seqs, int32_t num_requests, i
   if (hq / hk > oscar::kPcRows) return fail(OSCAR_ERR_UNSUPPORTED, "paged_attention: GQA group %d > %d", hq / hk, oscar::kPcRows);
   if (num_requests < 0 || !qsl || (num_requests > 0 && !seqs) || qsl[0] != 0 || qsl[num_requests] != n_tokens)
     return fail(OSCAR_ERR_INVALID, "paged_attention: invalid query layout");
-  for (int r = 0; r < num_requests; ++r)
+  int64_t work = 0;
+  for (int r = 0; r < num_requests; ++r) {
     if (qsl[r] > qsl[r + 1] || seqs[r] < 0)
       return fail(OSCAR_ERR_INVALID, "paged_attention: query starts must not fall and lengths not be negative");
+    if (qsl[r] == qsl[r + 1]) continue;
+    const int64_t tiles = key_tiles(seqs[r], hk), tokens = oscar::kPcRows / (hq / hk);
+    work += tiles * ((qsl[r + 1] - qsl[r] + tokens - 1) / tokens);
+    if (seqs[r] > kMaxLength || tiles > kMaxKeyTiles || work > kMaxWork)
+      return fail(OSCAR_ERR_UNSUPPORTED, "paged_attention: lengths of request %d too long for one call", r);
+  }
   return OSCAR_OK;
 }
 
@@ -572,6 +592,7 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
   bool any = false;
   for (int r = 0; r < num_requests; ++r) {
     if (seqs[r] < 0) return fail(OSCAR_ERR_INVALID, "evict_cache: lengths must not be negative");
+    if (seqs[r] > kMaxLength) return fail(OSCAR_ERR_UNSUPPORTED, "evict_cache: length of request %d too long", r);
     const int n = std::min(seqs[r], keep);
     most = std::max(most, n);
     any = any || n > 0;

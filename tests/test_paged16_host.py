@@ -85,6 +85,21 @@ def test_paged_attention_refusals(lib, kw, status, text):
     assert text in lib.oscar_last_error()
 
 
+def test_lengths_that_32_bits_of_positions_do_not_hold(lib):
+    top = 2**31 - 1
+    wide = dict(cols=2**27, stride=2**27)
+    assert evict(lib, seqs=(5, top), rows=2, **wide) == 2 and b"request 1 too long" in lib.oscar_last_error()
+    assert evict(lib, seqs=(2**30 + 1,), **wide) == 2
+    for seqs in ((top,), (2**30 + 1,)):
+        assert attention(lib, seqs=seqs, **wide) == 2 and b"too long" in lib.oscar_last_error()
+        assert lib.oscar_paged_attention_workspace(ints(0, 3), ints(*seqs), 1, 24, 4, 256, 0) < 0
+    # a prompt of 2^26 tokens; one of 2^20 fits
+    assert lib.oscar_paged_attention_workspace(ints(0, 2**26), ints(2**26), 1, 24, 4, 256, 0) < 0
+    assert lib.oscar_paged_attention_workspace(ints(0, 2**20), ints(2**20), 1, 24, 4, 256, 0) > 0
+    # many heads
+    assert lib.oscar_paged_attention_workspace(ints(0, 1), ints(2**29), 1, 512, 256, 64, 0) < 0
+
+
 def test_wait_limit(lib):
     assert lib.oscar_set_wait_limit(-2) == 1
     assert b"wait limit" in lib.oscar_last_error()
