@@ -388,6 +388,10 @@ int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  * Requests may share pages of history (their masses add up); the order of
  * these additions is not fixed, everything else is deterministic.
  *
+ * out may be q itself (the same rows at the same places), but not where weights
+ * are asked for and a request has more than 32 query rows per kv head, whose
+ * scores are computed again.
+ *
  * workspace: 32-byte aligned (as out), at least
  * oscar_paged_attention_workspace() bytes of the same lists (< 0: invalid lists). */
 int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,

@@ -519,6 +519,15 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   if (!aligned16(q) || (reinterpret_cast<uintptr_t>(out) & 31) || (reinterpret_cast<uintptr_t>(workspace) & 31) ||
       (q_token_stride | q_head_stride) % 8)
     return fail(OSCAR_ERR_INVALID, "paged_attention: query rows must be 16-byte, output and workspace 32-byte aligned");
+  if (weights != nullptr) {
+    bool again = false;  // are queries read after outputs were written?
+    for (int r = 0; r < num_requests; ++r)
+      again = again || (qsl[r + 1] > qsl[r] && paged_class(qsl[r + 1] - qsl[r], num_q_heads / num_kv_heads) != kFew);
+    const auto q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+    const auto q1 = q0 + 2 * ((n_tokens - 1) * q_token_stride + (num_q_heads - 1) * q_head_stride + head_dim);
+    if (again && o0 < q1 && q0 < o0 + 2 * n_tokens * num_q_heads * head_dim)
+      return fail(OSCAR_ERR_INVALID, "paged_attention: out must not overlap q where the keys are weighed");
+  }
   PagedCall c{};
   oscar::PagedArgs& a = c.args;
   a.q = q, a.q_tok = q_token_stride, a.q_head = q_head_stride;

@@ -434,6 +434,15 @@ def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
     return t
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do the memory ranges of two tensors meet?"""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    first, last = ([t.data_ptr() for t in (a, b)],
+                   [t.data_ptr() + t.element_size() * sum((n - 1) * s for n, s in zip(t.shape, t.stride())) for t in (a, b)])
+    return first[0] <= last[1] and first[1] <= last[0]
+
+
 def _cache16(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, dtype, hk: int, d: int) -> tuple:
     """Strides of the two caches, [blocks, tokens, hk, d] of `dtype` with contiguous rows."""
     shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
@@ -554,7 +563,7 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
 
     q [n, Hq, D]; caches [blocks, tokens, Hk, D] of q's type (strided views
     are fine); ``table`` [requests, pages]; ``qsl`` / ``seqs`` are host lists
-    or int32 arrays as in ``slab_attention``.
+    or int32 arrays as in ``slab_attention``; ``out`` may be q.
 
     ``weights`` [blocks, Hk, tokens] fp32 accumulates the attention weight of
     every cached key, summed over the heads of its group and the last
@@ -587,6 +596,8 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
         out = q.new_empty(q_shape)
     elif out.shape != q_shape or out.dtype != dtype or not out.is_contiguous() or out.data_ptr() % 32:
         raise ValueError(f"paged_attention: out must be contiguous, 32-byte aligned {list(q_shape)} of {dtype}")
+    elif _overlap(q, out) and (weights is not None or q.data_ptr() != out.data_ptr() or q.stride() != out.stride()):
+        q = q.clone()  # the keys' weights read the queries again; other overlaps are other rows'
     lse = q.new_empty((n, hq), dtype=torch.float32)
     lib = _native.lib()
     qsl_p, seqs_p, b = qsl_a.ctypes.data, seqs_a.ctypes.data, seqs_a.size

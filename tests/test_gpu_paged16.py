@@ -407,6 +407,26 @@ def test_key_weights(lens, seqs, observe, opts):
     assert kernels.device_error(dev) == 0
 
 
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("lens,seqs", [([3, 2], [700, 90]), ([20], [500]), ([150, 300], [700, 300])])
+def test_out_in_place_of_the_queries(lens, seqs, weighted):
+    """The attended rows may replace the queries, also where the keys' weights read those again;
+    a buffer that meets them elsewhere is as good."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, dict())
+    weights = [torch.zeros(kc.shape[0], 4, 128, device="cuda") if weighted else None for _ in range(3)]
+    want, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale, weights=weights[0])
+    n = q.shape[0]
+    over = torch.empty(n + 7, 24, 256, dtype=q.dtype, device="cuda")
+    for (query, out), w in zip(((over[:n], over[:n]), (over[:n], over[7:])), weights[1:]):
+        query.copy_(q)
+        got, lse2 = kernels.paged_attention(query, kc, vc, table, qsl, seqs, scale, weights=w, out=out)
+        assert got.data_ptr() == out.data_ptr() and torch.equal(got, want) and torch.equal(lse, lse2)
+        assert w is None or torch.equal(w, weights[0])
+
+
 def test_key_weights_of_shared_history_add_up():
     from oscar_b200 import kernels
 

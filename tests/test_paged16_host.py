@@ -106,6 +106,15 @@ def test_wait_limit(lib):
     assert lib.oscar_set_wait_limit(5) == 0 and lib.oscar_set_wait_limit(-1) == 0
 
 
+def test_out_over_the_queries_where_keys_are_weighed(lib):
+    long = dict(qsl=(0, 9), seqs=(16,), n=9, wsb=0)
+    for out in (FAKE, FAKE + 9 * 6144 * 2 - 32, FAKE - 9 * 6144 * 2 + 32):
+        assert attention(lib, out=out, w=FAKE, **long) == 1 and b"overlap q" in lib.oscar_last_error()
+    for kw in (dict(out=FAKE, w=None), dict(out=FAKE + 9 * 6144 * 2, w=FAKE), dict(out=FAKE - 9 * 6144 * 2, w=FAKE)):
+        attention(lib, **kw, **long)  # (goes on to what needs a GPU)
+        assert b"overlap q" not in lib.oscar_last_error()
+
+
 def test_workspace_of_invalid_lists(lib):
     assert lib.oscar_paged_attention_workspace(ints(0, 4, 3), ints(1, 1), 2, 24, 4, 256, 0) < 0
     assert lib.oscar_paged_attention_workspace(ints(0, 4), ints(9), 1, 24, 5, 256, 0) < 0
