@@ -413,11 +413,11 @@ int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs,
  * tokens between them the keep - sink - recent heaviest (ties: the lower
  * position; a NaN weight is above every number), in order.  Their K, V and
  * weight slots move to positions 0, 1, ... of the pages of dst_table, or of
- * block_table itself (dst_table NULL: in place).  Shorter requests keep all.
+ * block_table itself (dst_table NULL or block_table: in place).  Shorter requests keep all.
  * The new length is min(seqs[r], keep).  seqs: HOST.  kept
  * [num_requests, num_kv_heads, kept_cols] int32: the kept positions, -1 past
  * a request's list.  Pages written here must belong to one request of the call
- * only, and dst pages must not be source pages (unless dst_table is NULL).
+ * only, and dst pages must not be source pages (unless in place).
  * Weights that another stream writes meanwhile leave the choice undefined.
  * The pages' keys carry their position rotation with them. */
 int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t num_blocks, int32_t block_size,

@@ -596,7 +596,7 @@ int oscar_evict_cache(void* k_cache, void* v_cache, int32_t head_dim, int64_t nu
     st = check_cache("evict_cache", v_cache, num_blocks, block_size, num_kv_heads, head_dim, v_stride_block,
                      v_stride_token, v_stride_head);
   if (st) return st;
-  const bool in_place = dst_table == nullptr;
+  const bool in_place = dst_table == nullptr || (dst_table == block_table && dst_stride == bt_stride);
   int most = 0;
   bool any = false;
   for (int r = 0; r < num_requests; ++r) {

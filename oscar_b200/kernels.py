@@ -620,7 +620,8 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     heaviest of the others by ``weights`` [blocks, Hk, tokens] stay in order
     (ties: the lower position).  Their K, V and weight slots move to the front
     of the request's pages, or to the pages of ``dst_table`` (for pages shared
-    with other requests, which must not be overwritten).  ``seqs``: host list.
+    with other requests, which must not be overwritten; ``table`` itself: the
+    request's own).  ``seqs``: host list.
     Returns the kept positions [requests, Hk, min(keep, max(seqs))] int32 (-1
     past a request's list); the new lengths are min(seqs, keep)."""
     shape, dtype = k_cache.shape, k_cache.dtype
@@ -639,10 +640,10 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     seqs_a = _host_ints(seqs)
     if seqs_a.ndim != 1:
         raise ValueError("evict_cache: seqs must be a list of lengths")
-    table = _table32("evict_cache", table)
+    source, table = table, _table32("evict_cache", table)
     rows, cols = table.shape
     dst_p, dst_rows, dst_cols, dst_stride = None, 0, 0, 0
-    if dst_table is not None:
+    if dst_table is not None and (dst_table.data_ptr() != source.data_ptr() or dst_table.stride() != source.stride()):
         dst = _table32("evict_cache", dst_table)
         dst_p, (dst_rows, dst_cols), dst_stride = dst.data_ptr(), dst.shape, dst.stride(0)
     places = max(0, min(int(keep), int(seqs_a.max(initial=0))))

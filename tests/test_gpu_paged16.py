@@ -694,6 +694,22 @@ def test_evict_ends_while_another_stream_writes_the_weights(in_place):
     assert kernels.device_error(dev) == 0
 
 
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64])
+def test_evict_to_the_table_it_came_from_is_in_place(kind):
+    from oscar_b200 import kernels
+
+    need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(14)
+    seqs = [9000, 20000]
+    kc, vc, table = make_pool(gen, seqs, 32, 4, 128, torch.bfloat16, poison=False)
+    w = torch.rand(kc.shape[0], 4, 32, generator=gen, device="cuda")
+    k2, v2, w2 = kc.clone(), vc.clone(), w.clone()
+    table = table.to(kind)
+    a = kernels.evict_cache(kc, vc, w, table, seqs, 7000, sink=3, recent=7)
+    b = kernels.evict_cache(k2, v2, w2, table, seqs, 7000, sink=3, recent=7, dst_table=table)
+    assert torch.equal(a, b) and torch.equal(kc, k2) and torch.equal(vc, v2) and torch.equal(w, w2)
+
+
 def test_evict_strided_caches():
     from oscar_b200 import kernels
 
