@@ -356,7 +356,7 @@ int64_t oscar_decode_layer_step_scratch(int64_t n_tokens, int32_t num_q_heads, i
  * in fp32, rounded once.  q -> out_q; k -> out_k (may be NULL with caches) and
  * with caches k -> k_cache, v -> v_cache at slot_mapping[t] (slot < 0: not
  * written).  Weights and cos_sin are fp32 or of the heads' type.  out_q / out_k
- * may be q / k.  A position outside the table latches device error 64 and a
+ * may be q / k; their rows must not overlap.  A position outside the table latches device error 64 and a
  * slot outside the cache bit 1; neither is written.  rot_dim: a multiple of
  * 16.  v, out_k and the caches may be NULL. */
 int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,

@@ -48,6 +48,15 @@ bool half_dtype(int32_t dtype) { return dtype == OSCAR_DTYPE_BF16 || dtype == OS
 
 bool kernel_head_dim(int32_t d) { return d == 64 || d == 128 || d == 256; }
 
+// Are the rows of [n, heads, d] at these strides apart from one another?
+bool rows_apart(int64_t n, int64_t heads, int64_t d, int64_t token_stride, int64_t head_stride) {
+  if (n < 2) return heads < 2 || head_stride >= d;
+  if (heads < 2) return token_stride >= d;
+  const bool nested = token_stride >= head_stride;  // heads within a token's stride, or tokens within a head's
+  return nested ? head_stride >= d && token_stride >= (heads - 1) * head_stride + d
+                : token_stride >= d && head_stride >= (n - 1) * token_stride + d;
+}
+
 // One cache of [num_blocks, block_size, hk, D] elements with strides in elements.
 int check_cache(const char* what, const void* cache, int64_t num_blocks, int32_t bs, int32_t hk, int32_t d, int64_t sb,
                 int64_t st, int64_t sh) {
@@ -130,6 +139,9 @@ extern "C" int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t
       (v != nullptr && (v_token_stride | v_head_stride) % 8) ||
       (out_k != nullptr && (out_k_token_stride | out_k_head_stride) % 8) || cos_sin_stride % 8 || cos_sin_stride < rot_dim)
     return fail(OSCAR_ERR_INVALID, "qk_norm_rope: heads, weights and cos / sin rows must be 16-byte aligned");
+  if (!rows_apart(n_tokens, num_q_heads, head_dim, out_q_token_stride, out_q_head_stride) ||
+      (out_k != nullptr && !rows_apart(n_tokens, num_kv_heads, head_dim, out_k_token_stride, out_k_head_stride)))
+    return fail(OSCAR_ERR_INVALID, "qk_norm_rope: output rows overlap");
   oscar::HeadNormArgs a{};
   a.q = q, a.k = k, a.v = v;
   a.q_tok = q_token_stride, a.q_head = q_head_stride;

@@ -521,6 +521,22 @@ def test_qk_norm_rope(n, opts, layout):
     assert kernels.device_error(dev) == 0
 
 
+@pytest.mark.parametrize("n", [1, 5])
+def test_qk_norm_rope_output_layouts(n):
+    """Outputs with heads before tokens, and one token at a stride of its own."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, k, v, wq, wk, cos_sin, positions, o, gen = make_rope(n, dict())
+    want_q, want_k = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions)
+    oq = torch.zeros(24, n, 256, dtype=q.dtype, device="cuda").transpose(0, 1)
+    ok = torch.zeros(4, n, 256, dtype=q.dtype, device="cuda").transpose(0, 1)
+    got_q, got_k = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions, out_q=oq, out_k=ok)
+    assert got_q.data_ptr() == oq.data_ptr() and torch.equal(oq, want_q) and torch.equal(ok, want_k)
+    with pytest.raises(ValueError, match="overlap"):
+        kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions, out_q=oq[:, :1].expand(n, 24, 256))
+
+
 def test_qk_norm_rope_extremes():
     """Zero heads stay zero, an inf or NaN stays in its head, no tokens is no work."""
     from oscar_b200 import kernels

@@ -64,6 +64,21 @@ def test_qk_norm_rope_refusals(lib, kw, status, text):
         _native.check(status)
 
 
+@pytest.mark.parametrize("kw", [
+    dict(oqh=128), dict(oqt=256), dict(oqt=0), dict(oqh=0), dict(oqt=23 * 256 + 248), dict(ok=FAKE, okt=0, okh=256),
+    dict(ok=FAKE, okt=1024, okh=248), dict(oqt=256, oqh=768),
+])
+def test_overlapping_outputs_are_refused(lib, kw):
+    assert rope(lib, **kw) == 1 and b"output rows overlap" in lib.oscar_last_error()
+
+
+def test_outputs_in_any_order_are_accepted(lib):
+    n = 2**31  # refused before anything is launched, but only after the outputs
+    for kw in (dict(oqt=6144), dict(oqt=256, oqh=256 * n), dict(hq=1, hk=1, oqt=256, oqh=0, kkh=0),
+               dict(ok=FAKE, okt=256, okh=256 * n)):
+        assert rope(lib, n=n, **kw) == 2 and b"too many tokens" in lib.oscar_last_error()
+
+
 def test_nothing_to_do_is_accepted(lib):
     assert rope(lib, n=0) == 0
     assert attention(lib, qsl=(0, 0), n=0) == 0
