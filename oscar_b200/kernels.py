@@ -460,7 +460,10 @@ def _host_ints(values) -> np.ndarray:
         return values
     if isinstance(values, torch.Tensor):
         values = values.cpu().numpy()
-    return np.ascontiguousarray(values, dtype=np.int32)
+    out = np.ascontiguousarray(values, dtype=np.int32)
+    if isinstance(values, np.ndarray) and not np.array_equal(out, values):  # (numpy wraps and cuts without a word)
+        raise ValueError("query starts and lengths must be whole numbers of 32 bits")
+    return out
 
 
 def _table32(name: str, table: torch.Tensor) -> torch.Tensor:
@@ -646,12 +649,18 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     if dst_table is not None and (dst_table.data_ptr() != source.data_ptr() or dst_table.stride() != source.stride()):
         dst = _table32("evict_cache", dst_table)
         dst_p, (dst_rows, dst_cols), dst_stride = dst.data_ptr(), dst.shape, dst.stride(0)
-    places = max(0, min(int(keep), int(seqs_a.max(initial=0))))
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError("evict_cache: keep must be at least 1 and hold the sink and recent tokens")
+    longest = int(seqs_a.max(initial=0))
+    if keep > longest:  # nothing goes, and the numbers may pass 32 bits
+        keep, sink, recent = max(longest, 1), 0, 0
+    places = min(keep, longest)
     kept = k_cache.new_empty((seqs_a.size, hk, places), dtype=torch.int32)
     check(_native.lib().oscar_evict_cache(
         k_cache.data_ptr(), v_cache.data_ptr(), d, nb, bs, hk, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         weights.data_ptr(), table.data_ptr(), rows, cols, table.stride(0), dst_p, dst_rows, dst_cols, dst_stride,
-        seqs_a.ctypes.data, seqs_a.size, int(keep), int(sink), int(recent), kept.data_ptr(), places, _raw_stream(index)))
+        seqs_a.ctypes.data, seqs_a.size, keep, sink, recent, kept.data_ptr(), places, _raw_stream(index)))
     return kept
 
 

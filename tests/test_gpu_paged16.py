@@ -726,6 +726,38 @@ def test_evict_to_the_table_it_came_from_is_in_place(kind):
     assert torch.equal(a, b) and torch.equal(kc, k2) and torch.equal(vc, v2) and torch.equal(w, w2)
 
 
+def test_evict_limits_past_32_bits_keep_everything():
+    from oscar_b200 import kernels
+
+    need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    kc, vc, table = make_pool(gen, [500, 9], 32, 2, 64, torch.bfloat16, poison=False)
+    w = torch.rand(kc.shape[0], 2, 32, generator=gen, device="cuda")
+    k0, w0 = kc.clone(), w.clone()
+    for keep, sink, recent in ((2**32 + 100, 2**32 + 1, 3), (2**31, 0, 2**31), (2**40, 64, 256), (501, 400, 101)):
+        kept = kernels.evict_cache(kc, vc, w, table, [500, 9], keep, sink=sink, recent=recent)
+        assert kept[0, 0].tolist() == list(range(500)) and kept[1, 1].tolist() == list(range(9)) + [-1] * 491
+        assert torch.equal(kc, k0) and torch.equal(w, w0)
+    with pytest.raises(ValueError, match="keep"):
+        kernels.evict_cache(kc, vc, w, table, [500, 9], 2**32, sink=2**32, recent=1)
+
+
+def test_lists_past_32_bits_are_refused():
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, kc, vc, table, qsl, scale = make_call([2], [300], dict())
+    w = torch.zeros(kc.shape[0], 4, 128, device="cuda")
+    for seqs in (np.array([2**32 + 300]), torch.tensor([2**32 + 300]), np.array([300.5])):
+        with pytest.raises(ValueError, match="32 bits"):
+            kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale)
+        with pytest.raises(ValueError, match="32 bits"):
+            kernels.evict_cache(kc, vc, w, table, seqs, 100)
+    want, _ = kernels.paged_attention(q, kc, vc, table, qsl, [300], scale)
+    got, _ = kernels.paged_attention(q, kc, vc, table, torch.from_numpy(qsl).long(), np.array([300]), scale)
+    assert torch.equal(got, want)
+
+
 def test_evict_strided_caches():
     from oscar_b200 import kernels
 
