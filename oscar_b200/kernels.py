@@ -434,6 +434,11 @@ def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
     return t
 
 
+def _vector16(t: torch.Tensor) -> torch.Tensor:
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do the memory ranges of two tensors meet?"""
     if a.numel() == 0 or b.numel() == 0:
@@ -466,12 +471,18 @@ def _host_ints(values) -> np.ndarray:
     return out
 
 
-def _table32(name: str, table: torch.Tensor) -> torch.Tensor:
+def _table32(name: str, table: torch.Tensor) -> tuple:
+    """The block table as int32 rows apart from one another, and their stride."""
     if table.ndim != 2:
         raise ValueError(f"{name}: the block table must be [requests, pages]")
     if table.dtype != torch.int32:
         table = table.to(torch.int32)
-    return table if table.stride(1) == 1 else table.contiguous()
+    (rows, cols), (stride, step) = table.shape, table.stride()
+    if rows < 2:
+        stride = cols  # one row has no stride of its own
+    if (step != 1 and cols > 1) or stride < cols:  # (an expanded row among them)
+        return table.clone(memory_format=torch.contiguous_format), cols
+    return table, stride
 
 
 def _long(t: torch.Tensor) -> torch.Tensor:
@@ -486,7 +497,8 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
 
     q [n, Hq, D], k / v [n, Hk, D] (bf16 or fp16; views of a fused projection
     are fine); weights [D] and ``cos_sin`` [max_positions, rot] (cosines, then
-    sines) in fp32 or the heads' type; ``positions`` [n].  ``weight_offset``
+    sines) in fp32 or the heads' type (what is not 16-byte aligned is copied
+    first); ``positions`` [n].  ``weight_offset``
     1 is the zero-centred weight (1 + w).  Pairs (i, i + rot/2) rotate, or
     neighbours (2i, 2i + 1) with ``interleaved``.  Without caches the keys come
     back (v is not needed); with them k and v go to ``slot_mapping`` (slots
@@ -519,9 +531,9 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
     qt, kt, ct = q.stride(), k.stride(), cos_sin.stride()
     q, k = _rows16(q, qt), _rows16(k, kt)
     qt, kt = q.stride(), k.stride()
-    q_weight, k_weight, positions = q_weight.contiguous(), k_weight.contiguous(), _long(positions)
-    if ct[1] != 1 or ct[0] % 8:
-        cos_sin = cos_sin.contiguous()
+    q_weight, k_weight, positions = _vector16(q_weight), _vector16(k_weight), _long(positions)
+    if ct[1] != 1 or ct[0] % 8 or ct[0] < cs_shape[1] or cos_sin.data_ptr() % 16:
+        cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
         ct = cos_sin.stride()
     if out_q is None:
         out_q = q.new_empty(q_shape)  # (a third less host time than torch.empty)
@@ -588,7 +600,7 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
     qsl_a, seqs_a = _host_ints(qsl), _host_ints(seqs)
     if qsl_a.ndim != 1 or seqs_a.ndim != 1 or qsl_a.size != seqs_a.size + 1 or qsl_a[0] != 0 or qsl_a[-1] != n:
         raise ValueError("paged_attention: invalid query layout")
-    table = _table32("paged_attention", table)
+    table, ts = _table32("paged_attention", table)
     if weights is not None and (weights.shape != (nb, hk, bs) or weights.dtype != torch.float32
                                 or not weights.is_contiguous()):
         raise ValueError(f"paged_attention: weights must be contiguous fp32 [{nb}, {hk}, {bs}]")
@@ -608,10 +620,10 @@ def paged_attention(q, k_cache, v_cache, table, qsl, seqs, scale, *, weights=Non
     if need < 0:
         check(_native.ERR_INVALID)
     ws = q.new_empty(max(need, 16), dtype=torch.uint8)
-    qs, (rows, cols), ts = q.stride(), table.shape, table.stride()
+    qs, (rows, cols) = q.stride(), table.shape
     check(lib.oscar_paged_attention(
         q.data_ptr(), qs[0], qs[1], code, n, hq, hk, d, k_cache.data_ptr(), v_cache.data_ptr(), nb, bs, ks[0], ks[1],
-        ks[2], vs[0], vs[1], vs[2], table.data_ptr(), rows, cols, ts[0], qsl_p, seqs_p, b, scale,
+        ks[2], vs[0], vs[1], vs[2], table.data_ptr(), rows, cols, ts, qsl_p, seqs_p, b, scale,
         None if weights is None else weights.data_ptr(), 0x7FFFFFFF if observe is None else min(int(observe), 0x7FFFFFFF),
         out.data_ptr(), lse.data_ptr(), ws.data_ptr(), need, _raw_stream(index)))
     return out, lse
@@ -643,12 +655,12 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     seqs_a = _host_ints(seqs)
     if seqs_a.ndim != 1:
         raise ValueError("evict_cache: seqs must be a list of lengths")
-    source, table = table, _table32("evict_cache", table)
+    source, (table, ts) = table, _table32("evict_cache", table)
     rows, cols = table.shape
     dst_p, dst_rows, dst_cols, dst_stride = None, 0, 0, 0
     if dst_table is not None and (dst_table.data_ptr() != source.data_ptr() or dst_table.stride() != source.stride()):
-        dst = _table32("evict_cache", dst_table)
-        dst_p, (dst_rows, dst_cols), dst_stride = dst.data_ptr(), dst.shape, dst.stride(0)
+        dst, dst_stride = _table32("evict_cache", dst_table)
+        dst_p, (dst_rows, dst_cols) = dst.data_ptr(), dst.shape
     keep, sink, recent = int(keep), int(sink), int(recent)
     if keep < 1 or sink < 0 or recent < 0 or sink + recent > keep:
         raise ValueError("evict_cache: keep must be at least 1 and hold the sink and recent tokens")
@@ -659,7 +671,7 @@ def evict_cache(k_cache, v_cache, weights, table, seqs, keep: int, *, sink: int 
     kept = k_cache.new_empty((seqs_a.size, hk, places), dtype=torch.int32)
     check(_native.lib().oscar_evict_cache(
         k_cache.data_ptr(), v_cache.data_ptr(), d, nb, bs, hk, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        weights.data_ptr(), table.data_ptr(), rows, cols, table.stride(0), dst_p, dst_rows, dst_cols, dst_stride,
+        weights.data_ptr(), table.data_ptr(), rows, cols, ts, dst_p, dst_rows, dst_cols, dst_stride,
         seqs_a.ctypes.data, seqs_a.size, keep, sink, recent, kept.data_ptr(), places, _raw_stream(index)))
     return kept
 

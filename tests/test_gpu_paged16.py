@@ -521,6 +521,55 @@ def test_qk_norm_rope(n, opts, layout):
     assert kernels.device_error(dev) == 0
 
 
+def test_qk_norm_rope_weights_and_tables_at_any_place():
+    """Views that begin between the 16-byte boundaries, and one row of the table for all positions."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, k, v, wq, wk, cos_sin, positions, o, gen = make_rope(6, dict())
+
+    def odd(t, by):
+        flat = torch.zeros(t.numel() + by, dtype=t.dtype, device="cuda")[by:]
+        return flat.view(t.shape).copy_(t)
+
+    want = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions)
+    got = kernels.qk_norm_rope(q, k, None, odd(wq, 1), odd(wk, 3), 1e-6, odd(cos_sin, 1), positions)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    wide = torch.zeros(500, 72, device="cuda")
+    wide[:, 5:69] = cos_sin
+    got = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, wide[:, 5:69], positions)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    same = torch.full_like(positions, 7)
+    want = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, same)
+    got = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin[7:8].expand(500, -1), positions)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_block_tables_of_any_strides():
+    """An expanded row (requests with all their pages in common), one row at a stride of its own, columns."""
+    from oscar_b200 import kernels
+
+    need_gpu()
+    q, kc, vc, table, qsl, scale = make_call([1, 1, 1], [300, 300, 300], dict(page=64))
+    shared = table[:1].repeat(3, 1)
+    want, lse = kernels.paged_attention(q, kc, vc, shared, qsl, [300] * 3, scale)
+    for t in (table[:1].expand(3, -1), shared.t().contiguous().t(), shared.long(), torch.stack([shared, shared], 2)[..., 1]):
+        got, lse2 = kernels.paged_attention(q, kc, vc, t, qsl, [300] * 3, scale)
+        assert torch.equal(got, want) and torch.equal(lse, lse2)
+    one = shared.as_strided((1, shared.shape[1]), (0, 1))
+    got, _ = kernels.paged_attention(q[:1], kc, vc, one, [0, 1], [300], scale)
+    again, _ = kernels.paged_attention(q[:1], kc, vc, shared, [0, 1], [300], scale)
+    assert torch.equal(got, again)
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    w = torch.rand(kc.shape[0], 4, 64, generator=gen, device="cuda")
+    k2, v2, w2 = kc.clone(), vc.clone(), w.clone()
+    a = kernels.evict_cache(kc, vc, w, shared[:1], [300], 100)
+    b = kernels.evict_cache(k2, v2, w2, one, [300], 100)
+    assert torch.equal(a, b) and torch.equal(w, w2)
+    # (slots past the request hold NaN)
+    assert torch.equal(kc.view(torch.int16), k2.view(torch.int16)) and torch.equal(vc.view(torch.int16), v2.view(torch.int16))
+
+
 @pytest.mark.parametrize("n", [1, 5])
 def test_qk_norm_rope_output_layouts(n):
     """Outputs with heads before tokens, and one token at a stride of its own."""
