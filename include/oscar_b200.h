@@ -393,7 +393,9 @@ int oscar_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_str
  * scores are computed again.
  *
  * workspace: 32-byte aligned (as out), at least
- * oscar_paged_attention_workspace() bytes of the same lists (< 0: invalid lists). */
+ * oscar_paged_attention_workspace() bytes of the same lists (< 0: invalid lists):
+ * at most 320 MiB and 8 bytes per token and query head.  (Requests whose stored
+ * scores would pass 256 MiB together run in several launches.) */
 int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_stride, int32_t dtype,
                           int64_t n_tokens, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                           const void* k_cache, const void* v_cache, int64_t num_blocks, int32_t block_size,

@@ -55,7 +55,8 @@ struct PagedArgs {
   float scale_log2;       // scale * log2(e)
   float* part_o;          // [piece][row][D] unnormalised
   float2* part_ml;        // [piece][row] (maximum, sum)
-  float* scores;          // [tile][kPgFewRows][64] scaled scores in log2 units, or null
+  float* scores;          // [tile][score_rows][64] scaled scores in log2 units, or null
+  int score_rows;         // the most query rows of a request
   float* weights;         // [num_blocks, hk, bs], or null
   int observe;            // the last `observe` tokens of a request weigh the keys
   uint32_t tries;         // of a bounded wait
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kPgKeys) paged_mass_kernel(const __grid_consta
   __syncthreads();
   if (blk < 0 || blk >= a.num_blocks) return;  // past the request, or flagged by the attention pass
   float sum = 0.0f;
-  const float* s = a.scores + (int64_t)blockIdx.x * kPgFewRows * kPgKeys + threadIdx.x;
+  const float* s = a.scores + (int64_t)blockIdx.x * a.score_rows * kPgKeys + threadIdx.x;
 #pragma unroll 8
   for (int i = first; i < rows; ++i) sum = fmaf(pg_exp2(s[i * kPgKeys] - st[i].x), st[i].y, sum);
   float* w = a.weights + (blk * a.hk + h) * a.bs + (key - page * a.bs);

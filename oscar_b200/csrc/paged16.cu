@@ -179,8 +179,19 @@ namespace {
 // head, one row tile, scores stored where the keys are weighed.  kOne: one row
 // tile.  kChunk: q-blocks of two row tiles.
 enum PagedClass { kFew = 0, kOne = 1, kChunk = 2, kClasses = 3 };
-inline PagedClass paged_class(int64_t len, int group) {
-  if (len * group <= oscar::kPgFewRows) return kFew;
+
+// Scores that a launch stores at most: its requests are as many as that takes, and one that alone
+// passes it has its scores computed again instead (kOne).  8 requests of 4 x 6 rows on 24580 keys
+// and 4 heads have 76 MB.
+constexpr int64_t kScoreBytes = (int64_t)256 << 20;
+
+inline int64_t key_tiles(int32_t seq, int hk) {
+  return std::max<int64_t>(1, ((int64_t)seq + oscar::kPgKeys - 1) / oscar::kPgKeys) * hk;
+}
+inline int64_t score_bytes(int64_t tiles, int64_t rows) { return tiles * rows * oscar::kPgKeys * (int64_t)sizeof(float); }
+
+inline PagedClass paged_class(int64_t len, int32_t seq, int group, int hk, bool weighted) {
+  if (len * group <= oscar::kPgFewRows && !(weighted && score_bytes(key_tiles(seq, hk), len * group) > kScoreBytes)) return kFew;
   return len <= oscar::kPcRows / group ? kOne : kChunk;
 }
 
@@ -200,13 +211,10 @@ struct PagedBatch {
   PagedClass cls;
   int64_t tiles;
   int pieces;              // most pieces of a divided unit
+  int rows;                // most query rows per kv head of a request
   oscar::PcPlan plan;
   oscar::PcSplits splits;  // its divided units
 };
-
-inline int64_t key_tiles(int32_t seq, int hk) {
-  return std::max<int64_t>(1, ((int64_t)seq + oscar::kPgKeys - 1) / oscar::kPgKeys) * hk;
-}
 
 // Divides the tiles of all units over the workers.  A unit costs its tiles and
 // kUnitCost more (queries, first products, epilogue: about 9000 cycles against
@@ -259,17 +267,20 @@ void plan_units(PagedBatch& b, int hk, int sms) {
 }
 
 int paged_batch(PagedBatch& b, PagedClass cls, int r0, const int32_t* qsl, const int32_t* seqs, int num, int group,
-                int hk, int d, int sms) {
+                int hk, int d, bool weighted, int sms) {
   oscar::PcPlan& p = b.plan;
   b.cls = cls;
+  b.rows = 0;
   p.num_req = 0;
   int r = r0;
   int64_t tiles = 0;
   for (; r < num && p.num_req < oscar::kPgReqs; ++r) {
     const int len = qsl[r + 1] - qsl[r];
-    if (len == 0 || paged_class(len, group) != cls) continue;
+    if (len == 0 || paged_class(len, seqs[r], group, hk, weighted) != cls) continue;
     tiles += key_tiles(seqs[r], hk);
-    if (p.num_req > 0 && tiles > kMaxKeyTiles) break;
+    const int rows = std::max(b.rows, (int)std::min<int64_t>((int64_t)len * group, INT_MAX));
+    if (p.num_req > 0 && (tiles > kMaxKeyTiles || (weighted && cls == kFew && score_bytes(tiles, rows) > kScoreBytes))) break;
+    b.rows = rows;
     const int i = p.num_req++;
     p.req_id[i] = r;
     p.q_start[i] = qsl[r];
@@ -294,7 +305,7 @@ PagedSpace paged_space(const PagedBatch& b, int64_t n, int hq, int d, bool weigh
   const int64_t pieces = (int64_t)2 * b.plan.ctas * oscar::kPcRows * (b.cls == kChunk ? 2 : 1);
   s.part_ml = round256(pieces * (int64_t)sizeof(float2));
   s.part_o = round256(pieces * d * (int64_t)sizeof(float));
-  if (weighted && b.cls == kFew) s.scores = b.tiles * oscar::kPgFewRows * oscar::kPgKeys * (int64_t)sizeof(float);
+  if (weighted && b.cls == kFew) s.scores = score_bytes(b.tiles, b.rows);
   return s;
 }
 
@@ -428,17 +439,15 @@ int launch_paged(const PagedCall& c, const PagedBatch& b) {
   using Shape = oscar::PcShape<D, kFewRows>;
   const oscar::PagedArgs& a = c.args;
   const oscar::PcPlan& p = b.plan;
-  int most = 0;  // tokens of a request
-  for (int i = 0; i < p.num_req; ++i) most = std::max(most, p.q_len[i]);
   int st;
   if (b.cls == kFew && b.tiles <= kMmaTiles * device_info().sms)
-    st = most * a.group <= 16 ? launch_mma<D, T, 1>(c, b) : launch_mma<D, T, 2>(c, b);
+    st = b.rows <= 16 ? launch_mma<D, T, 1>(c, b) : launch_mma<D, T, 2>(c, b);
   else
     st = launch_tc<D, T, kFewRows>(c, b);
   if (st) return st;
   if (b.splits.n > 0) {
     int rows = Shape::kUnit * oscar::kPcRows;  // of a unit
-    if (kFewRows) rows = most * a.group;
+    if (kFewRows) rows = b.rows;
     // four warps a row from nine pieces on: with one, a row's pieces come one after another (28
     // against 10 us for one request's 24 rows in 37 pieces); below, they would mostly idle
     if (b.pieces > 8)
@@ -486,7 +495,7 @@ int64_t oscar_paged_attention_workspace(const int32_t* qsl, const int32_t* seqs,
   for (int cls = 0; cls < kClasses; ++cls)
     for (int r = 0; r < num_requests;) {
       r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, num_q_heads / num_kv_heads, num_kv_heads, head_dim,
-                      device_info().sms);
+                      weighted != 0, device_info().sms);
       if (b.plan.num_req > 0)
         need = std::max(need, paged_space(b, qsl[num_requests], num_q_heads, head_dim, weighted != 0).total());
     }
@@ -534,7 +543,8 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   if (weights != nullptr) {
     bool again = false;  // are queries read after outputs were written?
     for (int r = 0; r < num_requests; ++r)
-      again = again || (qsl[r + 1] > qsl[r] && paged_class(qsl[r + 1] - qsl[r], num_q_heads / num_kv_heads) != kFew);
+      again = again || (qsl[r + 1] > qsl[r] && paged_class(qsl[r + 1] - qsl[r], seqs[r], num_q_heads / num_kv_heads,
+                                                           num_kv_heads, true) != kFew);
     const auto q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
     const auto q1 = q0 + 2 * ((n_tokens - 1) * q_token_stride + (num_q_heads - 1) * q_head_stride + head_dim);
     if (again && o0 < q1 && q0 < o0 + 2 * n_tokens * num_q_heads * head_dim)
@@ -567,7 +577,7 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   for (int cls = 0; cls < kClasses; ++cls)
     for (int r = 0; r < num_requests;) {
       r = paged_batch(b, (PagedClass)cls, r, qsl, seqs, num_requests, a.group, num_kv_heads, head_dim,
-                      device_info().sms);
+                      weights != nullptr, device_info().sms);
       if (b.plan.num_req == 0) continue;
       if (!query_map(&c.qmap, q, dtype, n_tokens, num_q_heads, head_dim, q_token_stride, q_head_stride, a.group,
                      b.plan.box_tokens))
@@ -580,6 +590,7 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
       a.stats = weights != nullptr ? reinterpret_cast<float2*>(at) : nullptr;
       a.part_ml = reinterpret_cast<float2*>(at + space.stats);
       a.part_o = reinterpret_cast<float*>(at + space.stats + space.part_ml);
+      a.score_rows = b.rows;
       a.scores = space.scores ? reinterpret_cast<float*>(at + space.stats + space.part_ml + space.part_o) : nullptr;
       st = dtype == OSCAR_DTYPE_BF16 ? launch_paged_d<__nv_bfloat16>(head_dim, c, b)
                                      : launch_paged_d<__half>(head_dim, c, b);

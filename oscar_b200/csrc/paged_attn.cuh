@@ -461,7 +461,7 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
         }
         if constexpr (kFew) {
           if (a.scores != nullptr && live) {
-            float4* dst = reinterpret_cast<float4*>(a.scores + ((int64_t)(tile0 + job) * kPgFewRows + row) * kPgKeys);
+            float4* dst = reinterpret_cast<float4*>(a.scores + ((int64_t)(tile0 + job) * a.score_rows + row) * kPgKeys);
 #pragma unroll
             for (int c = 0; c < kTile; c += 4)
               dst[c / 4] = make_float4(__uint_as_float(s[c]) * scale, __uint_as_float(s[c + 1]) * scale,

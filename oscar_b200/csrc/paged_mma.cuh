@@ -234,7 +234,7 @@ paged_attn_mma_kernel(const __grid_constant__ PagedArgs a, const __grid_constant
         mw[hf] = best;
         grow = grow || best > own_max(hf) + kPgHeadroom;
         if (a.scores != nullptr && 16 * my_rt + 8 * hf + qr < nrows) {
-          float* dst = a.scores + ((tile0 + it) * kPgFewRows + 16 * my_rt + 8 * hf + qr) * kPgKeys + my_key + 2 * qc;
+          float* dst = a.scores + ((tile0 + it) * a.score_rows + 16 * my_rt + 8 * hf + qr) * kPgKeys + my_key + 2 * qc;
 #pragma unroll
           for (int e = 0; e < kOwn; e += 2) *reinterpret_cast<float2*>(dst + 4 * e) = make_float2(s[hf][e], s[hf][e + 1]);
         }

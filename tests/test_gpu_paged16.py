@@ -427,6 +427,30 @@ def test_out_in_place_of_the_queries(lens, seqs, weighted):
         assert w is None or torch.equal(w, weights[0])
 
 
+@pytest.mark.parametrize("lens,seqs,observe,opts", [
+    # together beyond what a launch stores: several launches
+    ([8] * 5, [150000, 140001, 9, 170000, 64], None, dict(hq=32, hk=8, d=64, page=64)),
+    # each alone beyond it: scores computed again
+    ([4, 1, 4], [270000, 100, 262145], 1, dict(hq=64, hk=8, d=64, page=64)),
+])
+def test_key_weights_of_more_scores_than_are_stored(lens, seqs, observe, opts):
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    q, kc, vc, table, qsl, scale = make_call(lens, seqs, opts)
+    nb, page, hk = kc.shape[:3]
+    weights = torch.zeros(nb, hk, page, device="cuda")
+    out, lse = kernels.paged_attention(q, kc, vc, table, qsl, seqs, scale, weights=weights, observe=observe)
+    want = attention64(q, kc, vc, table, lens, seqs, scale, observe)
+    check_attention(q, out, lse, want, seqs)
+    for r, seq in enumerate(seqs):
+        p = torch.arange(seq, device="cuda")
+        mass = want[3][r]
+        got = weights[table[r].long()[p // page], :, p % page].T.double()
+        assert ((got - mass).abs() <= 2 * SCORE * mass + 2.0**-23 * mass).all()
+    assert kernels.device_error(dev) == 0
+
+
 def test_key_weights_of_shared_history_add_up():
     from oscar_b200 import kernels
 

@@ -130,6 +130,16 @@ def test_out_over_the_queries_where_keys_are_weighed(lib):
         assert b"overlap q" not in lib.oscar_last_error()
 
 
+@pytest.mark.parametrize("lens,seqs,hq,hk,d", [
+    ([4] * 64, [32768] * 64, 24, 4, 256), ([4] * 256, [24580] * 256, 24, 4, 256), ([1, 4] * 200, [100000] * 400, 32, 8, 128),
+    ([4], [2**22], 24, 4, 256), ([1] * 3, [2**23, 100, 2**20], 64, 16, 64), ([8192, 4, 70], [17448, 10**6, 10**6], 24, 4, 256),
+])
+def test_workspace_is_bounded(lib, lens, seqs, hq, hk, d):
+    qsl = np.concatenate([[0], np.cumsum(lens)])
+    need = [lib.oscar_paged_attention_workspace(ints(*qsl), ints(*seqs), len(seqs), hq, hk, d, weighted) for weighted in (0, 1)]
+    assert 0 < need[0] < need[1] <= (320 << 20) + 8 * hq * int(qsl[-1])
+
+
 def test_workspace_of_invalid_lists(lib):
     assert lib.oscar_paged_attention_workspace(ints(0, 4, 3), ints(1, 1), 2, 24, 4, 256, 0) < 0
     assert lib.oscar_paged_attention_workspace(ints(0, 4), ints(9), 1, 24, 5, 256, 0) < 0
