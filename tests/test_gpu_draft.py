@@ -135,6 +135,133 @@ def test_prompt_steps_eviction_and_steps_after_it():
     assert kernels.device_error(dev) == 0
 
 
+class Rows:
+    """Per request and head: the rows that the cache holds, in 64 bits, and the keys' weights."""
+
+    def __init__(self, n, hq, hk, d, observe):
+        self.hq, self.hk, self.d, self.observe = hq, hk, d, observe
+        none = lambda *shape: torch.zeros(*shape, dtype=torch.float64, device="cuda")  # noqa: E731
+        self.k = [[none(0, d) for _ in range(hk)] for _ in range(n)]
+        self.v = [[none(0, d) for _ in range(hk)] for _ in range(n)]
+        self.w = [[none(0) for _ in range(hk)] for _ in range(n)]
+
+    def step(self, q, k, v, lens):
+        g = self.hq // self.hk
+        out, size = torch.zeros_like(q), torch.zeros_like(q)
+        lse = torch.zeros(q.shape[:2], dtype=torch.float64, device="cuda")
+        at = 0
+        for r, m in enumerate(lens):
+            for h in range(self.hk):
+                self.k[r][h] = torch.cat([self.k[r][h], k[at:at + m, h]])
+                self.v[r][h] = torch.cat([self.v[r][h], v[at:at + m, h]])
+                self.w[r][h] = torch.cat([self.w[r][h], torch.zeros(m, dtype=torch.float64, device="cuda")])
+                n, heads = self.k[r][h].shape[0], slice(h * g, (h + 1) * g)
+                x = torch.einsum("mgd,kd->mgk", q[at:at + m, heads], self.k[r][h]) * self.d**-0.5
+                hidden = torch.arange(n, device="cuda")[None] > torch.arange(n - m, n, device="cuda")[:, None]
+                x = x.masked_fill(hidden[:, None], -math.inf)
+                z = torch.logsumexp(x, -1)
+                p = torch.exp(x - z[..., None])
+                out[at:at + m, heads] = torch.einsum("mgk,kd->mgd", p, self.v[r][h])
+                size[at:at + m, heads] = torch.einsum("mgk,kd->mgd", p, self.v[r][h].abs())
+                lse[at:at + m, heads] = z
+                self.w[r][h] = self.w[r][h] + p[max(0, m - (self.observe or m)):].sum((0, 1))
+            at += m
+        return out, size, lse
+
+    def take(self, kept):
+        for r in range(len(self.k)):
+            for h in range(self.hk):
+                c = kept[r, h][kept[r, h] >= 0].long()
+                self.k[r][h], self.v[r][h], self.w[r][h] = self.k[r][h][c], self.v[r][h][c], self.w[r][h][c]
+
+
+@pytest.mark.parametrize("hq,hk,d,page,rot,dtype,observe", [
+    (8, 2, 64, 16, 32, torch.bfloat16, None), (24, 4, 256, 32, 64, torch.bfloat16, 2), (12, 3, 128, 48, 128, torch.float16, 1),
+    (16, 2, 256, 128, 128, torch.float16, None),
+])
+def test_layer_on_the_rows_it_caches(hq, hk, d, page, rot, dtype, observe):
+    """As above, but every part against what it was given.  The rows that the layer caches and attends
+    are read back (queries: the norm alone on the same inputs) and checked against the norm and rotation
+    in 64 bits within one rounding; outputs, LSE and weights are then those of these very rows.
+
+    Bound of a score: |q|, |k| < 1.5 sqrt(D) (norm weights under 1.5), so D products summed in fp32 are
+    off by at most D 2^-24 2.25 D D^-1/2; the exponential, its argument and the sum of at most 400 terms
+    add less than 3e-5.  A probability carries that twice (its own and the sum's)."""
+    from oscar_b200 import kernels
+    from oscar_b200.draft import DraftLayer, slots_of
+    from test_gpu_paged16 import check_rows, kept64, rope64
+
+    dev = need_gpu()
+    u, err = torch.finfo(dtype).eps / 2, 2.25 * d**1.5 * 2.0**-24 + 3e-5
+    gen = torch.Generator(device="cuda").manual_seed(21)
+    n, width, keep, sink, recent = 3, -(-250 // page), 90, 5, 20
+    fresh = -(-keep // page) + 1
+    pool = torch.full((n * (width + fresh) + 1, 2, page, hk, d), math.nan, device="cuda").to(dtype)
+    perm = torch.randperm(pool.shape[0], generator=gen, device="cuda").to(torch.int32)
+    table, dst = perm[:n * width].view(n, width), perm[n * width:n * (width + fresh)].view(n, fresh)
+    wq, wk = (torch.rand(d, generator=gen, device="cuda") - 0.5 for _ in range(2))
+    angle = torch.arange(400, device="cuda", dtype=torch.float64)[:, None] / 1e4 ** (
+        torch.arange(0, rot, 2, device="cuda", dtype=torch.float64) / rot)
+    cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float()
+    kc, vc = pool[:, 0], pool[:, 1]
+    layer = DraftLayer(hq, (kc, vc), wq, wk, cos_sin, weight_offset=1.0, keep=keep, sink=sink, recent=recent, observe=observe)
+    rows, cached, position, steps = Rows(n, hq, hk, d, observe), [0] * n, [0] * n, 0
+
+    def held(r):  # pages and places of a request's cached tokens
+        p = torch.arange(cached[r], device="cuda")
+        return table[r].long()[p // page], p % page
+
+    def check_cache():
+        for r in range(n):
+            blk, off = held(r)
+            for h in range(hk):
+                assert torch.equal(kc[blk, off, h].double(), rows.k[r][h])
+                assert torch.equal(vc[blk, off, h].double(), rows.v[r][h])
+                w = layer.weights[blk, h, off].double()
+                assert ((w - rows.w[r][h]).abs() <= (2 * err + steps * 2.0**-23) * rows.w[r][h]).all()
+
+    def step(lens):
+        nonlocal cached, position, steps
+        qkv = torch.randn(sum(lens), hq + 2 * hk, d, generator=gen, device="cuda").to(dtype)
+        q, k, v = qkv.split([hq, hk, hk], 1)
+        positions = torch.cat([torch.arange(p, p + m, device="cuda") for p, m in zip(position, lens)])
+        cached, position, steps = [c + m for c, m in zip(cached, lens)], [p + m for p, m in zip(position, lens)], steps + 1
+        slots = slots_of(table, lens, cached, page)
+        qsl = np.concatenate([[0], np.cumsum(lens)])
+        out, lse = layer.forward(q, k, v, positions, slots, table, qsl, cached)
+        q16, k16 = kernels.qk_norm_rope(q, k, None, wq, wk, 1e-6, cos_sin, positions, weight_offset=1.0)
+        for got, x, w in ((q16, q, wq), (k16, k, wk)):
+            check_rows(got, *rope64(x, w, 1.0, 1e-6, cos_sin, positions, False), dtype)
+        assert torch.equal(kc[slots // page, slots % page], k16) and torch.equal(vc[slots // page, slots % page], v)
+        want, size, z = rows.step(q16.double(), k16.double(), v.double(), lens)
+        tiny = max(cached) * 2.0**-25 * 6.0 if dtype == torch.float16 else 0.0
+        assert ((out.double() - want).abs() <= u * (size + want.abs()) * 1.01 + 2 * err * size + tiny).all()
+        assert ((lse.double() - z).abs() <= 2 * err).all()
+        check_cache()
+
+    def evict(to):
+        nonlocal cached, table
+        before = [layer.weights[held(r)[0], :, held(r)[1]].T.cpu().numpy() for r in range(n)]
+        cached, kept = layer.evict(table, cached, dst_table=to)
+        for r in range(n):
+            for h in range(hk):
+                c = kept64(before[r][h], keep, sink, recent)
+                assert kept[r, h][kept[r, h] >= 0].tolist() == c.tolist() and cached[r] == c.size
+        rows.take(kept)
+        table = table if to is None else to
+        check_cache()
+
+    step([100, 61, 30])
+    for _ in range(3):
+        step([2, 1, 4])
+    evict(None)
+    for _ in range(3):
+        step([1, 3, 30])
+    evict(dst)
+    step([4, 1, 1])
+    assert kernels.device_error(dev) == 0
+
+
 def test_draft_layer_refusals():
     from oscar_b200.draft import DraftLayer
 
