@@ -381,7 +381,6 @@ struct PagedCall {
   CUtensorMap qmap, kmap, vmap;
   const void* k_cache;
   int64_t kcb, kct, kch;
-  int64_t n;
   cudaStream_t stream;
 };
 
@@ -564,7 +563,6 @@ int oscar_paged_attention(const void* q, int64_t q_token_stride, int64_t q_head_
   a.observe = weights != nullptr ? observe : 0;
   a.tries = g_wait_tries.load(std::memory_order_relaxed);
   c.k_cache = k_cache, c.kcb = k_stride_block, c.kct = k_stride_token, c.kch = k_stride_head;
-  c.n = n_tokens;
   c.stream = reinterpret_cast<cudaStream_t>(stream);
   // without any key nothing is loaded: the maps only have to be valid
   const void* kb = any ? k_cache : q;

@@ -400,9 +400,9 @@ paged_attn_tc_kernel(const __grid_constant__ PagedArgs a, const __grid_constant_
     return __all_sync(0xffffffffu, ok);
   };
   PcWalk<Shape> w(p, worker);  // (the plan is an argument)
-  const int n_tiles = w.left, tile0 = p.first[worker];
+  const int n_tiles = w.left;
+  [[maybe_unused]] const int tile0 = p.first[worker];
   pdl_wait();
-  (void)tile0;
 
   if (warp < kMma) {
     // ================= softmax: thread = query row of row tile `wg`

@@ -262,6 +262,51 @@ def test_layer_on_the_rows_it_caches(hq, hk, d, page, rot, dtype, observe):
     assert kernels.device_error(dev) == 0
 
 
+def test_step_replayed_from_a_graph():
+    """A captured step attends the lengths it was captured with, on whatever its buffers hold."""
+    from oscar_b200 import kernels
+    from oscar_b200.draft import DraftLayer, slots_of
+
+    dev = need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    lens, seqs, page = [3, 150, 1], [700, 400, 90], 32
+    table = torch.randperm(66, generator=gen, device="cuda").to(torch.int32).view(3, 22)
+    start = torch.randn(2, 66, page, 4, 256, generator=gen, device="cuda").to(torch.bfloat16)
+    wq = torch.randn(256, generator=gen, device="cuda") * 0.1
+    angle = torch.arange(800, device="cuda")[:, None] / 1e4 ** (torch.arange(0, 64, 2, device="cuda") / 64)
+    cos_sin = torch.cat([angle.cos(), angle.sin()], 1)
+    qkv = torch.zeros(154, 32, 256, dtype=torch.bfloat16, device="cuda")
+    positions = torch.zeros(154, dtype=torch.int64, device="cuda")
+    slots, qsl = slots_of(table, lens, seqs, page), [0, 3, 153, 154]
+
+    def layer_on(pool):
+        return DraftLayer(24, pool, wq, wq, cos_sin, weight_offset=1.0, keep=80, sink=4, recent=16)
+
+    def step(layer):
+        out = layer.forward(qkv[:, :24], qkv[:, 24:28], qkv[:, 28:], positions, slots, table, qsl, seqs)
+        return *out, layer.evict(table, seqs)[1]
+
+    captured = layer_on(start.clone())
+    step(captured)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(captured)
+    for _ in range(3):
+        qkv.copy_(torch.randn(qkv.shape, generator=gen, device="cuda"))
+        positions.copy_(torch.randint(0, 800, (154,), generator=gen, device="cuda"))
+        for t, s in ((captured.k_cache, start[0]), (captured.v_cache, start[1])):
+            t.copy_(s)
+        captured.weights.zero_()
+        graph.replay()
+        eager = layer_on(start.clone())
+        want = step(eager)
+        for x, y in zip((*got, captured.k_cache, captured.v_cache, captured.weights),
+                        (*want, eager.k_cache, eager.v_cache, eager.weights)):
+            assert torch.equal(x, y)
+    assert kernels.device_error(dev) == 0
+    del graph
+
+
 def test_draft_layer_refusals():
     from oscar_b200.draft import DraftLayer
 
