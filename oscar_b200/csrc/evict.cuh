@@ -308,10 +308,10 @@ __global__ void __launch_bounds__(kEvMoveThreads) evict_copy_kernel(const __grid
       const int j = j0 + i * rows + mine;
       m[i].sb = -1;
       if (j >= n) continue;
-      const int s = kept[j], sp = (int)a.page.div(s), dp = (int)a.page.div(j);
-      if (s < 0) continue;
+      const int s = kept[j], sp = (int)a.page.div(max(s, 0)), dp = (int)a.page.div(j);
       const int sb = src_row[sp], db = dst_row[dp];
-      if (sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;  // flagged by the selection
+      // an empty place, or a block that the selection has flagged (one test: the loads stay in flight)
+      if (s < 0 || sb < 0 || sb >= a.num_blocks || db < 0 || db >= a.num_blocks) continue;
       m[i] = Move{sb, s - sp * a.bs, db, j - dp * a.bs};
     }
   };

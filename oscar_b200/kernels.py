@@ -424,7 +424,7 @@ def _cuda_index(first: torch.Tensor, *others: torch.Tensor | None) -> int:
 
 
 # the library launches on the current device, which therefore has to be the tensors'
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
@@ -432,11 +432,6 @@ def _rows16(t: torch.Tensor, stride: tuple) -> torch.Tensor:
     if stride[2] != 1 or (stride[0] | stride[1]) % 8 or t.data_ptr() % 16:
         return t.clone(memory_format=torch.contiguous_format)
     return t
-
-
-def _vector16(t: torch.Tensor) -> torch.Tensor:
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -531,10 +526,14 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
     qt, kt, ct = q.stride(), k.stride(), cos_sin.stride()
     q, k = _rows16(q, qt), _rows16(k, kt)
     qt, kt = q.stride(), k.stride()
-    q_weight, k_weight, positions = _vector16(q_weight), _vector16(k_weight), _long(positions)
-    if ct[1] != 1 or ct[0] % 8 or ct[0] < cs_shape[1] or cos_sin.data_ptr() % 16:
+    q_weight, k_weight, positions = q_weight.contiguous(), k_weight.contiguous(), _long(positions)
+    wq_p, wk_p, cs_p = q_weight.data_ptr(), k_weight.data_ptr(), cos_sin.data_ptr()
+    if (wq_p | wk_p) % 16:
+        q_weight, k_weight = q_weight.clone(), k_weight.clone()
+        wq_p, wk_p = q_weight.data_ptr(), k_weight.data_ptr()
+    if ct[1] != 1 or ct[0] % 8 or ct[0] < cs_shape[1] or cs_p % 16:
         cos_sin = cos_sin.clone(memory_format=torch.contiguous_format)
-        ct = cos_sin.stride()
+        ct, cs_p = cos_sin.stride(), cos_sin.data_ptr()
     if out_q is None:
         out_q = q.new_empty(q_shape)  # (a third less host time than torch.empty)
     elif out_q.shape != q_shape or out_q.dtype != dtype or out_q.stride(2) != 1:
@@ -563,7 +562,7 @@ def qk_norm_rope(q, k, v, q_weight, k_weight, eps, cos_sin, positions, *, weight
         ok, ok_p = out_k.stride(), out_k.data_ptr()
     check(_native.lib().oscar_qk_norm_rope(
         q.data_ptr(), qt[0], qt[1], k.data_ptr(), kt[0], kt[1], v_p, vt[0], vt[1], code, n, hq, hk, d,
-        q_weight.data_ptr(), k_weight.data_ptr(), _DTYPES[w_dtype], eps, weight_offset, cos_sin.data_ptr(),
+        wq_p, wk_p, _DTYPES[w_dtype], eps, weight_offset, cs_p,
         _DTYPES[cs_dtype], ct[0], cs_shape[0], cs_shape[1], 1 if interleaved else 0, positions.data_ptr(),
         out_q.data_ptr(), oq[0], oq[1], ok_p, ok[0], ok[1], kc_p, vc_p, nb, bs, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         slots_p, _raw_stream(index)))
