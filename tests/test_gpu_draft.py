@@ -307,6 +307,51 @@ def test_step_replayed_from_a_graph():
     del graph
 
 
+def test_two_threads_on_streams_of_their_own():
+    """Calls of two host threads share no state of the library: each gets what it gets alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from oscar_b200 import kernels
+
+    dev = need_gpu()
+    gen = torch.Generator(device="cuda").manual_seed(31)
+    jobs = []
+    for lens, seqs, d in (([3, 200], [900, 1500], 256), ([150, 2, 40], [700, 2000, 64], 128)):
+        pages = [-(-s // 32) for s in seqs]
+        table = torch.zeros(len(seqs), max(pages), dtype=torch.int32, device="cuda")
+        perm = torch.randperm(sum(pages), generator=gen, device="cuda").to(torch.int32)
+        for r, n in enumerate(pages):
+            table[r, :n] = perm[sum(pages[:r]):sum(pages[:r]) + n]
+        q, k = (torch.randn(sum(lens), h, d, generator=gen, device="cuda").to(torch.bfloat16) for h in (24, 4))
+        pool = torch.randn(2, sum(pages), 32, 4, d, generator=gen, device="cuda").to(torch.bfloat16)
+        jobs.append((q, k, pool, table, np.concatenate([[0], np.cumsum(lens)]).astype(np.int32), seqs, torch.ones(d, device="cuda"),
+                     torch.randn(100, 64, generator=gen, device="cuda"), torch.arange(sum(lens), device="cuda") % 100))
+
+    def work(job, stream):
+        q, k, pool, table, qsl, seqs, w, cos_sin, positions = job
+        results = []
+        with torch.cuda.stream(stream):
+            for _ in range(8):
+                kc, vc = pool.clone()
+                weights = torch.zeros(kc.shape[0], 4, 32, device="cuda")
+                x, y = kernels.qk_norm_rope(q, k, None, w, w, 1e-6, cos_sin, positions)
+                out = kernels.paged_attention(x, kc, vc, table, qsl, seqs, 0.1, weights=weights)
+                kept = kernels.evict_cache(kc, vc, weights, table, seqs, 300, sink=3, recent=40)
+                results.append((x, y, *out, kept, kc, vc, weights))
+        stream.synchronize()
+        return results
+
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    alone = [work(job, stream) for job, stream in zip(jobs, streams)]
+    with ThreadPoolExecutor(2) as pool:
+        together = list(pool.map(work, jobs, streams))
+    for a, b in zip(alone, together):
+        for x, y in zip(a, b):
+            assert all(torch.equal(s, t) for s, t in zip(x, y))
+    assert kernels.device_error(dev) == 0
+
+
 def test_draft_layer_refusals():
     from oscar_b200.draft import DraftLayer
 
