@@ -23,11 +23,14 @@
 // weights are held in shared memory; a longer request is read again for each round
 // and walked piece by piece.
 //
-// evict_move_kernel moves the rows.  Bound by bytes.  To other pages every row
-// is independent.  In place a CTA owns a 128-byte slice of one head's K or V
+// To other pages every row is independent and evict_copy_kernel is bound by bytes.
+// In place (evict_move_kernel) a CTA owns a 128-byte slice of one head's K or V
 // rows and walks the list in ascending order: it holds 256 rows' slices in
 // registers between the read and the write of a step, and the next step's
-// reads are already in flight.
+// reads are already in flight.  A step's chain of loads (list, table, row) and
+// the few CTAs of a request (32 with 4 heads at D 256) keep it from the bytes'
+// rate: 8 x 24580 keys cut to 12288 take 441 us, one request's 9256 cut to 4096
+// 138 us (181 and 30 us to other pages, timed the same way).
 #pragma once
 
 #include "paged_attn.cuh"

@@ -31,7 +31,8 @@ struct KeyPlan {  // the keys of a launch's requests in 64-key tiles
 };
 
 // Division by the page size without a divide (it sits in the producers' serial path, where
-// one costs 150 cycles): q = (mulhi(mul, n) + n) >> shift for n < 2^31, with
+// one costs 150 cycles), by the method of Granlund and Montgomery (Division by Invariant
+// Integers using Multiplication, 1994): q = (mulhi(mul, n) + n) >> shift for n < 2^31, with
 // shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1.
 struct FastDiv {
   uint32_t d, mul, shift;

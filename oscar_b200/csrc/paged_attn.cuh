@@ -17,14 +17,16 @@
 // and V instead of 1.25 beside the queries.
 //
 // Measured (Hq 24 / Hk 4 / D 256, bf16): kFew, 8 x 4 tokens on 24580: 131 us, 6.1
-// TB/s (0.94 of the measured copy); 8192 tokens on 17448: 1.97-2.03 ms, 1330-1370
-// TFLOP/s (0.98-1.0 of the sustained library rate, at the power cap's clock).
+// TB/s (0.94 of the measured copy); 8192 tokens on 17448: 1.95-2.03 ms, 1330-1380
+// TFLOP/s (0.98-1.02 of the sustained library rate, at the power cap's clock).
 //
 // Bounds.  kFew: HBM; the keys stream through shared memory once, 64-key tiles,
 // and the products of 128 padded rows take half of the time their bytes do
 // (mma.sync on the live rows took more: its operand reads alone filled the
 // shared-memory bandwidth that the copies leave).  Else D 256: the tensor pipe;
-// D <= 128: the exponentials (128 x 128 per row tile at 16 per cycle and SM).
+// D <= 128: the softmax warps, which read each score twice (at D 128 a tile takes
+// 4100 cycles, while its products and its 2 x 128 x 128 exponentials, 16 per cycle,
+// take 2048 each; 8192 tokens on 17448: 1.21 ms at D 128, 1.10 ms at D 64).
 //
 // Tile.  Jobs alternate between two score buffers: with one row tile per CTA job j
 // is key tile j, with two it is key tile j / 2 of row tile j % 2.  The MMA warp

@@ -28,7 +28,11 @@ class DraftLayer:
     as ``kernels.qk_norm_rope``.  ``keep``: cached tokens per request that
     :meth:`evict` leaves (None: weights are not kept); ``sink`` / ``recent``: of
     these, the first and last ones that always stay; ``observe``: the last
-    tokens of a step that weigh the keys (None: all)."""
+    tokens of a step that weigh the keys (None: all).
+
+    Memory beside the caches: with ``keep`` 4 bytes per cache slot and head for
+    the weights, and during a step the queries' copy, the output and a
+    workspace of at most 320 MiB and 8 bytes per token and query head."""
 
     def __init__(self, num_heads: int, kv_cache, q_weight, k_weight, cos_sin, *, eps: float = 1e-6,
                  weight_offset: float = 0.0, interleaved: bool = False, scale: float | None = None,
